@@ -21,6 +21,7 @@ FCR_NCCL_ID_BYTES = 128
 
 FCR_F16, FCR_BF16, FCR_F32 = 0, 1, 2
 FCR_SUM, FCR_MEAN, FCR_MAX = 0, 1, 2
+FCR_KV_16BIT, FCR_KV_FP8, FCR_KV_INT8 = 0, 1, 2
 REDUCTION_CODES = {"sum": FCR_SUM, "mean": FCR_MEAN, "max": FCR_MAX}
 
 EXPORTS = (
@@ -48,6 +49,11 @@ EXPORTS = (
     "fcr_comm_destroy",
     "fcr_sharded_workspace_bytes",
     "fcr_colreduce_sharded",
+    "fcr_qk_norm_rope",
+    "fcr_kv_append",
+    "fcr_kv_read",
+    "fcr_tree_workspace_bytes",
+    "fcr_tree_attention",
 )
 
 
@@ -98,6 +104,55 @@ class Shard(C.Structure):
         ("row_lo", C.c_int32 * 2), ("row_hi", C.c_int32 * 2),
         ("needs_reduce", C.c_int32),
     ]
+
+
+class Rope(C.Structure):
+    """Mirror of ``fcr_rope``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("Hq", C.c_int32), ("Hk", C.c_int32), ("M", C.c_int32), ("D", C.c_int32),
+        ("rotary", C.c_int32),
+        ("q_strides", C.c_int64 * 4),
+        ("k_strides", C.c_int64 * 4),
+        ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("position_bits", C.c_int32),
+        ("position_strides", C.c_int64 * 2),
+        ("eps", C.c_float),
+    ]
+
+
+class KvCache(C.Structure):
+    """Mirror of ``fcr_kv_cache``."""
+
+    _fields_ = [
+        ("B", C.c_int32), ("H", C.c_int32), ("N", C.c_int32), ("D", C.c_int32),
+        ("format", C.c_int32), ("dtype", C.c_int32),
+        ("k_strides", C.c_int64 * 4),
+        ("v_strides", C.c_int64 * 4),
+        ("k_scale_strides", C.c_int64 * 3),
+        ("v_scale_strides", C.c_int64 * 3),
+    ]
+
+
+class Tree(C.Structure):
+    """Mirror of ``fcr_tree``."""
+
+    _fields_ = [
+        ("Hq", C.c_int32), ("M", C.c_int32),
+        ("q_strides", C.c_int64 * 4),
+        ("index_bits", C.c_int32),
+        ("mask_strides", C.c_int64 * 2),
+        ("scale", C.c_float),
+    ]
+
+
+_STRIDES4 = C.c_int64 * 4
+
+
+def strides4(strides):
+    """A (B, H, rows, D) tensor's strides; the innermost one is 1 (or of a dimension of one element)."""
+    return _STRIDES4(strides[0], strides[1], strides[2], 1)
 
 
 def _load() -> C.CDLL:
@@ -161,6 +216,19 @@ def _load() -> C.CDLL:
                                           C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p,
                                           C.c_void_p]
     lib.fcr_colreduce_sharded.restype = C.c_int
+    lib.fcr_qk_norm_rope.argtypes = [C.POINTER(Rope)] + [C.c_void_p] * 9
+    lib.fcr_qk_norm_rope.restype = C.c_int
+    lib.fcr_kv_append.argtypes = [C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                  C.POINTER(C.c_int64), C.c_void_p, C.POINTER(C.c_int64), C.c_int32, C.c_void_p,
+                                  C.c_void_p, C.c_int32, C.c_void_p]
+    lib.fcr_kv_append.restype = C.c_int
+    lib.fcr_kv_read.argtypes = [C.POINTER(KvCache), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fcr_kv_read.restype = C.c_int
+    lib.fcr_tree_workspace_bytes.argtypes = [C.POINTER(KvCache), C.POINTER(Tree), C.c_int32]
+    lib.fcr_tree_workspace_bytes.restype = C.c_size_t
+    lib.fcr_tree_attention.argtypes = [C.POINTER(KvCache), C.POINTER(Tree)] + [C.c_void_p] * 10 + [C.c_size_t, C.c_void_p]
+    lib.fcr_tree_attention.restype = C.c_int
     return lib
 
 

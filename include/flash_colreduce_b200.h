@@ -376,6 +376,114 @@ int fcr_topk(const void* scores, int32_t dtype, int32_t rows, int32_t n, int32_t
 int fcr_select_above(const void* scores, int32_t dtype, int32_t rows, int32_t n, float threshold,
                      void* indices, int32_t index_bits, int32_t* counts, void* stream);
 
+/*
+ * ---- What a serving program does around the column reduction ----------------
+ * Queries and keys are normalised and rotated, keys and values are written to a
+ * cache (optionally in 8 bits) and read back, and drafted tokens attend the
+ * cache.  The reference has none of this; its README names the token pruning
+ * that these feed.  All launches go to `stream`; nothing synchronises,
+ * allocates or keeps a pointer, and every call may be captured into a graph.
+ */
+
+/*
+ * Norm of every head's queries and keys and rotation by position, in one pass:
+ *   y = x * rsqrt(mean_d x_d^2 + eps) * w_d   (a null weight: y = x)
+ *   (a, b) -> (a cos t - b sin t, a sin t + b cos t),  t = position * inv_freq[i]
+ * for i < rotary / 2, on the pairs (i, i + rotary / 2) or, with `interleaved`,
+ * (2 i, 2 i + 1); dimensions from `rotary` on are not rotated.  q: (B,Hq,M,D),
+ * k: (B,Hk,M,D) with innermost stride 1 and any others; Hq or Hk may be 0.
+ * Outputs are contiguous and must not overlap the inputs.  Computed in fp32
+ * (the angle in fp64) and rounded once.
+ */
+typedef struct fcr_rope {
+  int32_t B, Hq, Hk, M, D;       /* D <= 256 */
+  int32_t rotary;                /* even, 0 <= rotary <= D */
+  int64_t q_strides[4];          /* elements, (B,H,M,D) */
+  int64_t k_strides[4];
+  int32_t dtype;                 /* fcr_dtype of q, k and the outputs */
+  int32_t weight_dtype;          /* dtype, or FCR_F32 */
+  int32_t interleaved;
+  int32_t position_bits;         /* 32 or 64 */
+  int64_t position_strides[2];   /* elements, (B,M); 0: shared */
+  float eps;
+} fcr_rope;
+
+int fcr_qk_norm_rope(const fcr_rope* problem, const void* q, const void* k, const void* positions,
+                     const float* inv_freq, const void* q_weight, const void* k_weight, void* q_out,
+                     void* k_out, void* stream);
+
+/*
+ * A KV cache: K and V of shape (B,H,N,D), N the capacity, innermost stride 1.
+ * FCR_KV_16BIT holds values of `dtype`.  FCR_KV_FP8 (e4m3) and FCR_KV_INT8 hold
+ * a code per value and, per row, one scale 2^e as an E8M0 byte (e + 127) in an
+ * array of shape (B,H,N): e is the least exponent, at least -127, for which the
+ * row's largest magnitude is at most 448 * 2^e or 127 * 2^e, and the codes are
+ * x * 2^-e rounded to nearest even.  Magnitudes that code * 2^e could not hold
+ * finitely in the written type are clamped to the largest that it can.  A row
+ * with a NaN or an infinity gets scale byte 255 and reads back as NaN.  Reading
+ * in the type a row was written from is exact.
+ */
+typedef enum fcr_kv_format { FCR_KV_16BIT = 0, FCR_KV_FP8 = 1, FCR_KV_INT8 = 2 } fcr_kv_format;
+
+typedef struct fcr_kv_cache {
+  int32_t B, H, N, D;            /* D <= 256 */
+  int32_t format;                /* fcr_kv_format */
+  int32_t dtype;                 /* FCR_F16 or FCR_BF16: type of the values written and read */
+  int64_t k_strides[4];          /* elements, (B,H,N,D) */
+  int64_t v_strides[4];
+  int64_t k_scale_strides[3];    /* elements (bytes), (B,H,N); ignored for FCR_KV_16BIT */
+  int64_t v_scale_strides[3];
+} fcr_kv_cache;
+
+/*
+ * Writes token m < M of sequence b (key, value: (B,H,M,D) of the cache's dtype,
+ * innermost stride 1) at position lengths[b] + m of the cache.  With `counts`
+ * only the tokens m < counts[b] are written.  Tokens of a negative length or at
+ * positions >= N are left out.  lengths and counts (B): int32 or int64
+ * (index_bits).  Positions not written keep what they held.
+ */
+int fcr_kv_append(const fcr_kv_cache* cache, void* k_cache, void* v_cache, void* k_scales, void* v_scales,
+                  const void* key, const int64_t key_strides[4], const void* value,
+                  const int64_t value_strides[4], int32_t M, const void* lengths, const void* counts,
+                  int32_t index_bits, void* stream);
+
+/*
+ * Reads positions 0 .. n-1 of every head, or with `positions` (contiguous
+ * (B,H,n), int32 or int64: index_bits) the ones it names, e.g. those fcr_topk
+ * selected, into contiguous (B,H,n,D) arrays of the cache's dtype.  A position
+ * outside 0 .. N-1 reads as zeros.
+ */
+int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_cache, const void* k_scales,
+                const void* v_scales, const void* positions, int32_t index_bits, int32_t n, void* k_out,
+                void* v_out, void* stream);
+
+/*
+ * Attention of M drafted tokens per sequence (q: (B,Hq,M,D), innermost stride
+ * 1; Hq a multiple of the cache's H, query head h reads cache head h / (Hq / H))
+ * over a cache.  Every token of sequence b attends positions 0 .. lengths[b]-1
+ * and, of the drafted tokens, which lie at lengths[b] .. lengths[b]+M-1
+ * (fcr_kv_append puts them there), those j with mask[b,m,j] != 0; a null mask
+ * is a chain (j <= m), which with M = 1 is plain decoding.  Positions >= N do
+ * not exist; a negative length counts as 0.
+ * out: contiguous (B,Hq,M,D) of the cache's dtype; lse (may be null): fp32
+ * (B,Hq,M), natural logarithm of the sum of exponentials.  A row that attends
+ * nothing has out 0 and lse -inf.  What masked and unwritten positions hold
+ * does not matter, NaN and infinities included.
+ */
+typedef struct fcr_tree {
+  int32_t Hq, M;                 /* M <= 256 */
+  int64_t q_strides[4];
+  int32_t index_bits;            /* of lengths: 32 or 64 */
+  int64_t mask_strides[2];       /* bytes, (B,M); the innermost stride is 1; 0 for a mask that sequences share */
+  float scale;
+} fcr_tree;
+
+size_t fcr_tree_workspace_bytes(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t num_sms);
+int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const void* q, const void* k_cache,
+                       const void* v_cache, const void* k_scales, const void* v_scales, const void* lengths,
+                       const void* mask, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif
