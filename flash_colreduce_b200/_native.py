@@ -54,6 +54,7 @@ EXPORTS = (
     "fcr_kv_read",
     "fcr_tree_workspace_bytes",
     "fcr_tree_attention",
+    "fcr_tree_segment",
 )
 
 
@@ -227,6 +228,9 @@ def _load() -> C.CDLL:
     lib.fcr_kv_read.restype = C.c_int
     lib.fcr_tree_workspace_bytes.argtypes = [C.POINTER(KvCache), C.POINTER(Tree), C.c_int32]
     lib.fcr_tree_workspace_bytes.restype = C.c_size_t
+    lib.fcr_tree_segment.argtypes = [C.POINTER(KvCache), C.POINTER(Tree), C.c_int32, C.POINTER(C.c_int64), C.c_int32, C.c_int32,
+                                     C.POINTER(C.c_int32)]
+    lib.fcr_tree_segment.restype = C.c_int
     lib.fcr_tree_attention.argtypes = [C.POINTER(KvCache), C.POINTER(Tree)] + [C.c_void_p] * 10 + [C.c_size_t, C.c_void_p]
     lib.fcr_tree_attention.restype = C.c_int
     return lib

@@ -99,7 +99,14 @@ enum {
   ST_WAIT_MERGE_EMPTY = 37,
 };
 
-struct PassParams : PassGeom {
+// Where a kernel reports a bounded wait that expired, and the bound.
+struct WaitParams {
+  int* status;
+  int* host_status;       // the device's status mailbox in mapped host memory (null: none)
+  long long wait_limit;   // bound of a device-side wait, in clock64 cycles (wait_bar: once to three times)
+};
+
+struct PassParams : PassGeom, WaitParams {
   int m_pad, n_pad;
   float scale2;    // |scale| * log2(e)
   uint32_t idesc;  // tcgen05 instruction descriptor
@@ -115,9 +122,6 @@ struct PassParams : PassGeom {
   int out_dtype;
   int mean_mode;   // 0: none, 1: divide by div_M, 2: causal rule
   int div_M, div_N, div_c;
-  int* status;
-  int* host_status;       // the device's status mailbox in mapped host memory (null: none)
-  long long wait_limit;   // bound of a device-side wait, in clock64 cycles (wait_bar: once to three times)
   int skip_ring_load;     // self-test: CTA 0's TMA warp leaves out this ring load (-1: none)
   int* sched_counter;  // zero at launch; hands out work items beyond the first gridDim.x (null: round-robin)
   int clear_status;    // 1: this kernel clears status words 0-3 itself (no memset ran before it)
@@ -127,7 +131,7 @@ struct PassParams : PassGeom {
 
 // First failure wins: the code goes to status word 0 of the workspace and, when the device has
 // one, to the mailbox in mapped host memory, where the host sees it without a synchronisation.
-__device__ __noinline__ void report_status(const PassParams& p, int code, int detail) {
+__device__ __noinline__ void report_status(const WaitParams& p, int code, int detail) {
   if (atomicCAS(p.status, 0, code) == 0) {
     p.status[1] = (int)blockIdx.x;
     p.status[2] = (int)threadIdx.x;
@@ -186,11 +190,11 @@ struct SmemLayout {
 // hint), so a waiting warp polls.  Letting the waiting warps sleep between polls was measured
 // (100 ns to 1 us for the TMA and MMA warps, 50 and 200 ns for the fold warps): no timing changed by
 // more than the run-to-run noise, so they simply poll.
-// `bounds` is the wait's limit in units of PassParams::wait_limit: 1 for a wait on loads or products, which is where a
+// `bounds` is the wait's limit in units of WaitParams::wait_limit: 1 for a wait on loads or products, which is where a
 // failure shows first; 2 or 3 for a wait on warps or blocks that themselves wait (the TMA warp's, for slots that its
 // consumers give back), so that it expires later and the status names the wait at the root.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                         const PassParams& p, int code, int bounds) {
+                                         const WaitParams& p, int code, int bounds) {
   if (ptx::mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   uint32_t spins = 0;
@@ -212,7 +216,7 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
 #define WAIT_BEHIND(bar, par, code) wait_bar_warp(bar, par, abort_flag, p, code, 2)
 #define WAIT_BEHIND_PEERS(bar, par, code) wait_bar_warp(bar, par, abort_flag, p, code, 3)
 __device__ __forceinline__ bool wait_bar_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                              const PassParams& p, int code, int bounds) {
+                                              const WaitParams& p, int code, int bounds) {
   const bool ok = wait_bar(bar, parity, abort_flag, p, code, bounds);
   return __all_sync(0xffffffffu, ok);
 }

@@ -99,6 +99,74 @@ FCR_HD T hd_min(T a, T b) { return a < b ? a : b; }
 template <typename T>
 FCR_HD T hd_max(T a, T b) { return a > b ? a : b; }
 
+// ------------------------------------------------------------ attention of drafted tokens
+// The key tiles of all (sequence, key head, row tile) groups are one line, cut into one piece of equal length per CTA,
+// whatever the sequences' lengths are: lengths live on the device, so every CTA finds its piece itself.
+constexpr int kTreeTile = 128;  // keys per tile
+
+// Cached positions in front of the drafted tokens, and 128-key tiles up to the last one of them.
+FCR_HD int tree_have(long long length, int N) { return (int)(length < 0 ? 0 : length > N ? N : length); }
+FCR_HD int tree_end(int have, int M, int N) { return N - have < M ? N : have + M; }
+FCR_HD int tree_tiles(int have, int M, int N) { return (tree_end(have, M, N) + kTreeTile - 1) / kTreeTile; }
+
+// One CTA's walk over its piece: segments are runs of tiles of one group.
+struct TreeSegment {
+  int b, group;          // sequence; key head * row tiles + row tile
+  int lo, hi, tiles;     // tiles [lo, hi) of the group's `tiles`
+  int have, end;         // cached positions, end of the drafted tokens' positions
+  FCR_HD bool whole() const { return lo == 0 && hi == tiles; }
+  FCR_HD int slot() const { return lo == 0 ? 1 : 0; }  // which of its CTA's two partial results it leaves, when not whole
+};
+template <typename Lengths>  // long long operator()(int b)
+struct TreeWalk {
+  Lengths lengths;
+  int B, groups, M, N;
+  int b, group, t, tiles, have;
+  long long left;
+  FCR_HD void start(int first_b, long long offset, long long n) {
+    b = first_b;
+    left = n;
+    group = 0;
+    t = 0;
+    if (n <= 0) return;
+    sequence();
+    group = (int)(offset / tiles);
+    t = (int)(offset - (long long)group * tiles);
+  }
+  FCR_HD void sequence() {
+    have = tree_have(lengths(b), N);
+    tiles = tree_tiles(have, M, N);
+  }
+  FCR_HD bool next(TreeSegment& s) {
+    if (left <= 0) return false;
+    s.b = b;
+    s.group = group;
+    s.lo = t;
+    s.tiles = tiles;
+    s.hi = left < tiles - t ? t + (int)left : tiles;
+    s.have = have;
+    s.end = tree_end(have, M, N);
+    left -= s.hi - s.lo;
+    t = 0;
+    if (left > 0 && ++group == groups) {
+      group = 0;
+      ++b;
+      sequence();
+    }
+    return true;
+  }
+};
+// CTAs that get a piece: every one of these gets a tile at least, so that a group's partial results lie without gaps.
+FCR_HD int tree_ctas(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
+// Piece [lo, hi) of CTA c < tree_ctas, and the CTA that owns tile `tile` of `total`.
+FCR_HD long long tree_piece(long long total, int ctas, int c) { return total * c / ctas; }
+FCR_HD int tree_owner(long long total, int ctas, long long tile) {
+  int c = (int)((tile * ctas) / total);
+  while (c + 1 < ctas && tree_piece(total, ctas, c + 1) <= tile) ++c;
+  while (c > 0 && tree_piece(total, ctas, c) > tile) --c;
+  return c;
+}
+
 // Maps a linear work-item index to its head, stationary block and split, and
 // derives the streamed tile range of each stationary sub-tile.  The rows pass
 // keeps Q tiles stationary and streams the K tiles a tile's rows may attend;

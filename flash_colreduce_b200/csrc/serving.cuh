@@ -81,15 +81,6 @@ static cudaError_t launch_read_f(int format, const KvReadParams& p, bool vec, un
   return launch_read<T, FCR_KV_16BIT>(p, vec, blocks, stream);
 }
 
-template <typename T>
-static cudaError_t launch_tree(int format, const TreeParams& p, cudaStream_t stream) {
-  const long long rows = (long long)p.B * p.Hq * p.M;
-  const dim3 grid((unsigned)((rows + 3) / 4)), block(128);
-  if (format == FCR_KV_FP8) return launch_kernel(tree_rows_kernel<T, FCR_KV_FP8>, grid, block, 0, stream, false, p);
-  if (format == FCR_KV_INT8) return launch_kernel(tree_rows_kernel<T, FCR_KV_INT8>, grid, block, 0, stream, false, p);
-  return launch_kernel(tree_rows_kernel<T, FCR_KV_16BIT>, grid, block, 0, stream, false, p);
-}
-
 static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
   if (c.B <= 0 || c.H <= 0 || c.N <= 0 || c.D <= 0 || t.Hq <= 0 || t.M <= 0)
     return fail(FCR_ERR_BAD_ARG, "attention sizes must be positive");
@@ -108,6 +99,72 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
         return fail(FCR_ERR_UNSUPPORTED, "strides of the cache must be positive multiples of 16 bytes");
   }
   return FCR_OK;
+}
+
+struct HostLengths {
+  const int64_t* p;
+  FCR_HD long long operator()(int b) const { return (long long)p[b]; }
+};
+
+// What the host decides of an attention call: the kernel's variant and the workspace.
+struct TreePlan {
+  int rows, copies, part_rows, row_tiles, ctas, words, mask_rows;
+  bool pair;
+  int d_pad;
+  size_t off_mask, off_ml, off_o, bytes;
+};
+static TreePlan plan_tree(const fcr_kv_cache& c, const fcr_tree& t, int sms) {
+  TreePlan pl;
+  pl.rows = t.Hq / c.H * t.M;
+  pl.pair = pl.rows > 128;
+  pl.row_tiles = pl.pair ? (pl.rows + 255) / 256 : 1;
+  pl.copies = pl.rows <= 32 ? 4 : pl.rows <= 64 ? 2 : 1;
+  pl.part_rows = pl.pair ? 256 : 128 / pl.copies;
+  pl.d_pad = c.D <= 64 ? 64 : 128;
+  const long long most = (long long)c.B * c.H * pl.row_tiles * ((c.N + kTreeTile - 1) / kTreeTile);
+  pl.ctas = (int)std::min<long long>(most, sms);
+  pl.words = (t.M + 31) / 32;
+  pl.mask_rows = t.mask_strides[0] == 0 ? 1 : c.B;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  pl.off_mask = kStatusWords * 4;
+  pl.off_ml = up(pl.off_mask + (size_t)pl.mask_rows * t.M * pl.words * 4);
+  pl.off_o = up(pl.off_ml + (size_t)pl.ctas * 2 * pl.part_rows * 8);
+  pl.bytes = up(pl.off_o + (size_t)pl.ctas * 2 * pl.part_rows * pl.d_pad * 4);
+  return pl;
+}
+
+template <typename T, int DPAD, bool PAIR, bool QUANT>
+static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
+  auto kern = tree_attention_kernel<T, DPAD, PAIR, QUANT>;
+  constexpr int smem = TreeSmem<DPAD, PAIR>::kDynamicBytes;
+  static std::atomic<unsigned long long> opted_in{0};
+  cudaError_t e = cudaSuccess;
+  const unsigned long long bit = 1ULL << (t_device & 63);
+  if (!(opted_in.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    opted_in.fetch_or(bit, std::memory_order_release);
+  }
+  e = launch_kernel(kern, dim3(pl.ctas), dim3(tree_threads<QUANT>()), smem, stream, true, map_k, map_v, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
+  if (p.N > kTreeTile && pl.ctas > 1) {  // a group of one tile is never shared
+    const int rows_per_tile = std::min(p.rows, 256), blocks_per_group = (rows_per_tile + 7) / 8;
+    const long long blocks = (long long)p.B * p.groups * blocks_per_group;
+    if (blocks > 0x7fffffffLL) return fail(FCR_ERR_UNSUPPORTED, "too many rows");
+    e = launch_kernel(tree_combine_kernel<T, DPAD>, dim3((unsigned)blocks), dim3(256), 0, stream, true, p, pl.ctas, rows_per_tile,
+                      blocks_per_group);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "tree combine launch");
+  }
+  return FCR_OK;
+}
+template <typename T, int DPAD>
+static int launch_tree_d(bool quant, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
+                         cudaStream_t stream) {
+  if (pl.pair)
+    return quant ? launch_tree<T, DPAD, true, true>(map_k, map_v, p, pl, stream) : launch_tree<T, DPAD, true, false>(map_k, map_v, p, pl, stream);
+  return quant ? launch_tree<T, DPAD, false, true>(map_k, map_v, p, pl, stream) : launch_tree<T, DPAD, false, false>(map_k, map_v, p, pl, stream);
 }
 
 }  // namespace fcr
@@ -265,8 +322,43 @@ size_t fcr_tree_workspace_bytes(const fcr_kv_cache* cache, const fcr_tree* tree,
     return 0;
   }
   if (check_tree(*cache, *tree) != FCR_OK) return 0;
-  (void)num_sms;
-  return 256;
+  int sms = num_sms;
+  if (sms <= 0 && device_sm_count(&sms) != FCR_OK) return 0;
+  return plan_tree(*cache, *tree, sms).bytes;
+}
+
+int fcr_tree_segment(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t num_sms, const int64_t* lengths, int32_t cta,
+                     int32_t index, int32_t* out) {
+  if (!cache || !tree || !lengths || !out || num_sms <= 0) return fail(FCR_ERR_BAD_ARG, "null argument");
+  const int rc = check_tree(*cache, *tree);
+  if (rc != FCR_OK) return rc;
+  const fcr_kv_cache& c = *cache;
+  const TreePlan pl = plan_tree(c, *tree, num_sms);
+  if (cta < 0 || cta >= pl.ctas || index < 0) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
+  const int groups = c.H * pl.row_tiles;
+  long long total = 0;
+  for (int b = 0; b < c.B; ++b) total += (long long)tree_tiles(tree_have(lengths[b], c.N), tree->M, c.N) * groups;
+  const int ctas = tree_ctas(total, pl.ctas);
+  if (cta >= ctas) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
+  const long long lo = tree_piece(total, ctas, cta), hi = tree_piece(total, ctas, cta + 1);
+  long long before = 0;
+  int first = 0;
+  for (; first < c.B; ++first) {
+    const long long mine = (long long)tree_tiles(tree_have(lengths[first], c.N), tree->M, c.N) * groups;
+    if (lo < before + mine) break;
+    before += mine;
+  }
+  TreeWalk<HostLengths> walk{{lengths}, c.B, groups, tree->M, c.N};
+  walk.start(first, lo - before, hi - lo);
+  TreeSegment s;
+  for (int i = 0; i <= index; ++i)
+    if (!walk.next(s)) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
+  long long group_first = (long long)s.group * s.tiles;
+  for (int b = 0; b < s.b; ++b) group_first += (long long)tree_tiles(tree_have(lengths[b], c.N), tree->M, c.N) * groups;
+  const int v[10] = {s.b, s.group / pl.row_tiles, s.group % pl.row_tiles, s.lo, s.hi, s.tiles, s.whole() ? -1 : s.slot(),
+                     tree_owner(total, ctas, group_first), tree_owner(total, ctas, group_first + s.tiles - 1), ctas};
+  for (int i = 0; i < 10; ++i) out[i] = v[i];
+  return FCR_OK;
 }
 
 int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const void* q, const void* k_cache,
@@ -282,17 +374,35 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   if (rc != FCR_OK) return rc;
   if (reinterpret_cast<uintptr_t>(k_cache) % 16 || reinterpret_cast<uintptr_t>(v_cache) % 16)
     return fail(FCR_ERR_UNSUPPORTED, "cache base address must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(out) % 16) return fail(FCR_ERR_UNSUPPORTED, "output must be 16-byte aligned");
+  const DeviceInfo* dev = nullptr;
+  rc = device_info(&dev, true);
+  if (rc != FCR_OK) return rc;
+  rc = check_mailbox(*dev, nullptr);  // a wait that expired in an earlier call is reported here
+  if (rc != FCR_OK) return rc;
+  t_device = dev->index;
+  const TreePlan pl = plan_tree(c, t, dev->sms);
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < pl.bytes)
+    return fail(FCR_ERR_WORKSPACE, "workspace missing, misaligned or smaller than " + std::to_string(pl.bytes) + " bytes");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
+  const bool quant = c.format != FCR_KV_16BIT;
   TreeParams p;
   memset(&p, 0, sizeof(p));
+  p.status = reinterpret_cast<int*>(ws);
+  p.host_status = dev->mailbox_dev;
+  p.wait_limit = g_wait_limit_override > 0 ? g_wait_limit_override : kWaitLimitCycles;
+  p.skip_ring_load = g_skip_ring_load;
   p.q = q;
   p.cache[0] = k_cache;
   p.cache[1] = v_cache;
   p.scales[0] = static_cast<const unsigned char*>(k_scales);
   p.scales[1] = static_cast<const unsigned char*>(v_scales);
   p.lengths = lengths;
-  p.mask = static_cast<const unsigned char*>(mask);
   p.out = out;
   p.lse = lse;
+  p.part_ml = reinterpret_cast<float2*>(ws + pl.off_ml);
+  p.part_o = reinterpret_cast<float*>(ws + pl.off_o);
   p.qb = t.q_strides[0];
   p.qh = t.q_strides[1];
   p.qm = t.q_strides[2];
@@ -306,8 +416,6 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
     p.sh[i] = ss[i][1];
     p.sn[i] = ss[i][2];
   }
-  p.mask_b = t.mask_strides[0];
-  p.mask_m = t.mask_strides[1];
   p.B = c.B;
   p.Hq = t.Hq;
   p.Hk = c.H;
@@ -315,16 +423,49 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.N = c.N;
   p.D = c.D;
   p.G = t.Hq / c.H;
+  p.rows = pl.rows;
+  p.row_tiles = pl.row_tiles;
+  p.groups = c.H * pl.row_tiles;
+  p.copies = pl.copies;
+  p.part_rows = pl.part_rows;
+  p.words = pl.words;
+  p.mask_shared = t.mask_strides[0] == 0;
   p.index_bits = t.index_bits;
-  p.scale2 = t.scale * 1.4426950408889634f;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  if (!workspace || workspace_bytes < 256) return fail(FCR_ERR_WORKSPACE, "workspace missing or too small");
-  cudaError_t e = cudaMemsetAsync(workspace, 0, 256, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync");
-  e = c.dtype == FCR_F16 ? launch_tree<__half>(c.format, p, stream) : launch_tree<__nv_bfloat16>(c.format, p, stream);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
-  return FCR_OK;
+  p.format = c.format;
+  const int32_t q_sizes[3] = {c.B, t.Hq, t.M};
+  p.q_vec = kv_aligned(q, t.q_strides, q_sizes, 3, 2, 16);
+  float s2 = fabsf(t.scale) * 1.4426950408889634f;
+  if (!(s2 >= 1e-30f)) s2 = 1e-30f;  // scale 0: every score becomes (numerically) zero
+  p.scale2 = s2;
+  p.idesc_s = instr_desc(c.dtype, t.scale < 0.f);
+  // P V: the second operand is MN-major (bit 16), N = the padded head dimension
+  p.idesc_o = (instr_desc(c.dtype, false) & ~(63u << 17)) | (1u << 16) | ((uint32_t)(pl.d_pad >> 3) << 17);
+  p.k_steps = (c.D + 15) / 16;
+  CUtensorMap map_k, map_v;
+  memset(&map_k, 0, sizeof(map_k));
+  memset(&map_v, 0, sizeof(map_v));
+  if (!quant) {
+    rc = make_tensor_map(&map_k, k_cache, c.dtype, c.D, c.N, c.H, c.B, c.k_strides);
+    if (rc != FCR_OK) return rc;
+    rc = make_tensor_map(&map_v, v_cache, c.dtype, c.D, c.N, c.H, c.B, c.v_strides);
+    if (rc != FCR_OK) return rc;
+  }
+  if (mask) {
+    const long long n_words = (long long)pl.mask_rows * t.M * pl.words;
+    if (n_words > 0x7fffffffLL) return fail(FCR_ERR_UNSUPPORTED, "mask too large");
+    uint32_t* packed = reinterpret_cast<uint32_t*>(ws + pl.off_mask);
+    p.mask = packed;
+    cudaError_t e = launch_kernel(tree_pack_mask_kernel, dim3((unsigned)((n_words + 7) / 8)), dim3(256), 0, stream, true,
+                                  static_cast<const unsigned char*>(mask), (long long)t.mask_strides[0], (long long)t.mask_strides[1],
+                                  (int)t.M, pl.words, (int)n_words, packed);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "mask packing launch");
+  }
+  if (c.dtype == FCR_F16)
+    return pl.d_pad == 64 ? launch_tree_d<__half, 64>(quant, map_k, map_v, p, pl, stream)
+                          : launch_tree_d<__half, 128>(quant, map_k, map_v, p, pl, stream);
+  return pl.d_pad == 64 ? launch_tree_d<__nv_bfloat16, 64>(quant, map_k, map_v, p, pl, stream)
+                        : launch_tree_d<__nv_bfloat16, 128>(quant, map_k, map_v, p, pl, stream);
 }
 
 }  // extern "C"

@@ -6,89 +6,925 @@
 //
 // A row that attends nothing has out = 0 and lse = -inf.
 //
+// The G query heads of a key head and their M tokens are G * M rows that read the same keys.  One CTA runs a row tile
+// of them against a run of 128-key tiles:
+//
+//   S = Q K^T    tcgen05, 128 rows x 128 keys, fp32 in tensor memory
+//   P = 2^(S * scale * log2 e - m)   one thread per row, 16 bits, back to tensor memory over S
+//   O += P V     tcgen05, A = P from tensor memory, B = V as it lies in the cache (rows are the K dimension)
+//
+// with m a reference that follows the running maximum only when that has grown by more than 2^8: O is then rescaled in
+// tensor memory, otherwise the loop carries no correction.  Two warpgroups take turns, so that the exponentials of one
+// tile run under the products of the other.  With more than 128 rows (PAIR) they are two row tiles over the same keys;
+// with fewer, two runs of keys (every other tile) whose results are merged.  With at most 64 (32) rows the rows lie 2 (4)
+// times in the 128 lanes and each copy folds its half (quarter) of a tile's keys, P being zero elsewhere: no lane idles.
+//
+// The key tiles of all rows of all sequences are one line that the CTAs share equally (plan.h), so ragged lengths cost
+// nothing and a single long sequence uses every SM.  A piece that covers a group's keys only in part leaves its
+// (m, l, O) in the workspace and tree_combine_kernel joins them, in the order of the keys.
+//
+// A cache in 8 bits goes through registers: eight warps load the codes, turn code * 2^e into 16 bits (exactly) and
+// write the swizzled tile that TMA writes for a 16-bit cache.
+//
+// Masked scores are selected away, so NaN in masked keys is harmless; a masked value is not, being multiplied by zero,
+// so values behind the last drafted token are zeroed and non-finite ones among the drafted tokens too; a row that does attend such
+// a token gets it back in the epilogue.
+//
 // Included by colreduce_sm100.cu after kvcache_sm100.cuh.
 #pragma once
 
 namespace fcr {
 
-struct TreeParams {
-  const void* q;
-  const void* cache[2];    // K, V
-  const unsigned char* scales[2];
-  const void* lengths;
-  const unsigned char* mask;
-  void* out;
-  float* lse;
-  long long qb, qh, qm;
-  long long cb[2], ch[2], cn[2];
-  long long sb[2], sh[2], sn[2];
-  long long mask_b, mask_m;
-  int B, Hq, Hk, M, N, D, G;
-  int index_bits;
-  float scale2;            // scale * log2(e)
+constexpr int kTreeMaxM = 256;
+constexpr int kTreeSoftmaxWarps = 8;  // two warpgroups
+constexpr int kTreeMmaWarp = 8;
+constexpr int kTreeQWarp = 9;         // two warps that bring the queries
+constexpr int kTreeQWarps = 2;
+constexpr int kTreeLoadWarp = 11;     // one TMA warp, or the warps that convert codes
+constexpr int kTreeConvertWarps = 8;
+template <bool QUANT>
+constexpr int tree_threads() { return 32 * (kTreeLoadWarp + (QUANT ? kTreeConvertWarps : 1)); }
+
+enum {
+  ST_TR_WAIT_Q_EMPTY = 71,
+  ST_TR_WAIT_K_EMPTY = 72,
+  ST_TR_WAIT_V_EMPTY = 73,
+  ST_TR_WAIT_Q_FULL = 74,
+  ST_TR_WAIT_K_FULL = 75,
+  ST_TR_WAIT_V_FULL = 76,
+  ST_TR_WAIT_P = 77,
+  ST_TR_WAIT_S = 78,
+  ST_TR_WAIT_O = 79,
+  ST_TR_WAIT_MERGE = 80,
+  ST_TR_WAIT_V_FULL_SM = 81,
+  ST_TR_WAIT_DRAIN = 82,
 };
 
-template <typename T, int FORMAT>
-__device__ __forceinline__ float tree_load(const TreeParams& p, int which, int b, int h, long long n, int d) {
-  const long long at = b * p.cb[which] + h * p.ch[which] + n * p.cn[which] + d;
-  if (FORMAT == FCR_KV_16BIT) return to_f32(reinterpret_cast<const T*>(p.cache[which])[at]);
-  const uint32_t byte = reinterpret_cast<const unsigned char*>(p.cache[which])[at];
-  float v[4];
-  unpack_codes4<FORMAT>(byte, v);
-  return v[0] * kv_scale(p.scales[which][b * p.sb[which] + h * p.sh[which] + n * p.sn[which]]);
+struct TreeParams : WaitParams {
+  const void* q;
+  const void* cache[2];             // K, V
+  const unsigned char* scales[2];
+  const void* lengths;
+  const uint32_t* mask;             // packed (mask_rows, M, words); null: a chain
+  void* out;
+  float* lse;
+  float* part_o;                    // [ctas][2][part_rows][DPAD]
+  float2* part_ml;                  // [ctas][2][part_rows]
+  long long qb, qh, qm;
+  long long cb[2], ch[2], cn[2];    // 8-bit cache: byte strides
+  long long sb[2], sh[2], sn[2];
+  int B, Hq, Hk, M, N, D, G, rows;  // rows = G * M
+  int row_tiles, groups;            // groups = Hk * row_tiles
+  int copies;                       // 1, 2 or 4 copies of the rows in the lanes
+  int part_rows;
+  int words, mask_shared;
+  int index_bits, format, q_vec;
+  float scale2;                     // |scale| * log2(e)
+  uint32_t idesc_s, idesc_o;
+  int k_steps;                      // 32-byte steps of a key row that hold data
+  int skip_ring_load;
+};
+
+struct TreeLengths {
+  const void* p;
+  int bits;
+  FCR_HD long long operator()(int b) const {
+    return bits == 64 ? reinterpret_cast<const long long*>(p)[b] : (long long)reinterpret_cast<const int*>(p)[b];
+  }
+};
+
+template <int DPAD, bool PAIR>
+struct TreeSmem {
+  static constexpr int kTileBytes = 128 * DPAD * 2;
+  static constexpr int kSlabBytes = 128 * 128;
+  static constexpr int kQBuffers = PAIR ? 1 : 2;
+  // a query buffer doubles as the space in which the two warpgroups merge: 256 lanes x 32 columns of fp32
+  static constexpr int kQBytes = PAIR ? 2 * kTileBytes : 32768;
+  static constexpr int KS = DPAD == 64 ? 5 : 3, VS = DPAD == 64 ? 4 : 2;  // key and value tiles in flight
+  static constexpr int off_q = 0;
+  static constexpr int off_k = off_q + kQBuffers * kQBytes;
+  static constexpr int off_v = off_k + KS * kTileBytes;
+  static constexpr int off_stat = off_v + VS * kTileBytes;  // float2 [256]
+  static constexpr int off_bars = off_stat + 2048;
+  static constexpr int kNumBars = 4 + 2 * KS + 2 * VS + 2 + 2 + 2 + 1;
+  static constexpr int off_misc = off_bars + 8 * kNumBars;
+  static constexpr int kDynamicBytes = off_misc + 48;
+  static_assert(kDynamicBytes <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
+};
+
+// Bits of the keys n0 .. n0 + 31 that row m attends.
+__device__ __forceinline__ uint32_t tree_bits(const TreeParams& p, const uint32_t* words, int m, int n0, int have, int end) {
+  if (n0 + 32 <= have) return 0xffffffffu;
+  if (n0 >= end) return 0u;
+  const int j0 = n0 - have;  // place of the first key among the drafted tokens, negative: cached positions come first
+  uint32_t bits;
+  if (words == nullptr) {
+    const int last = m - j0;  // attended: bit <= last
+    bits = last < 0 ? 0u : last >= 31 ? 0xffffffffu : (2u << last) - 1u;
+  } else {
+    const int first = max(j0, 0), w = first >> 5;
+    const uint32_t lo = words[w], hi = w + 1 < p.words ? words[w + 1] : 0u;
+    bits = __funnelshift_r(lo, hi, first & 31);
+    if (j0 < 0) bits = bits << -j0 | ((1u << -j0) - 1u);
+  }
+  if (n0 + 32 > end) bits &= (1u << (end - n0)) - 1u;
+  return bits;
 }
 
-// One warp per query row.
-template <typename T, int FORMAT>
-__global__ void __launch_bounds__(128)
-tree_rows_kernel(const TreeParams p) {
+template <typename T>
+__device__ __forceinline__ bool non_finite16(uint32_t h) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (h & kExp) == kExp;
+}
+
+// The values of a drafted token that the product left out because they are not finite; 0 for a finite one.
+template <typename T, bool QUANT>
+__device__ __forceinline__ float tree_non_finite(const TreeParams& p, int b, int h, int n, int d) {
+  const long long at = b * p.cb[1] + h * p.ch[1] + n * p.cn[1] + d;
+  float v;
+  if (QUANT) {
+    float c[4];
+    const uint32_t byte = reinterpret_cast<const unsigned char*>(p.cache[1])[at];
+    if (p.format == FCR_KV_FP8) unpack_codes4<FCR_KV_FP8>(byte, c); else unpack_codes4<FCR_KV_INT8>(byte, c);
+    v = c[0] * kv_scale(p.scales[1][b * p.sb[1] + h * p.sh[1] + n * p.sn[1]]);
+  } else {
+    v = to_f32(reinterpret_cast<const T*>(p.cache[1])[at]);
+  }
+  return fabsf(v) < INFINITY ? 0.f : v;
+}
+template <typename T, bool QUANT>
+__device__ __noinline__ void tree_add_non_finite(const TreeParams& p, const TreeSegment& s, const uint32_t* words, int m, int d0, int nd,
+                                                 float* o) {
+  const int h = s.group / p.row_tiles;
+  const int hi = min(s.end, s.hi * kTreeTile);
+  for (int n = max(s.have, s.lo * kTreeTile); n < hi; ++n) {
+    const int j = n - s.have;
+    if (words ? !(words[j >> 5] >> (j & 31) & 1u) : j > m) continue;
+    for (int d = 0; d < nd && d0 + d < p.D; ++d) o[d] += tree_non_finite<T, QUANT>(p, s.b, h, n, d0 + d);
+  }
+}
+
+// Packs a bool mask (mask_b, M, M) into words of 32 tokens; a warp per word.
+__global__ void __launch_bounds__(256)
+tree_pack_mask_kernel(const unsigned char* __restrict__ mask, long long stride_b, long long stride_m, int M, int words, int n_words,
+                      uint32_t* __restrict__ out) {
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
   const int lane = threadIdx.x & 31;
-  const long long rows = (long long)p.B * p.Hq * p.M;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (r >= rows) return;
-  const int m = (int)(r % p.M);
-  const int h = (int)(r / p.M % p.Hq), b = (int)(r / p.M / p.Hq);
-  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + h * p.qh + m * p.qm;
-  float qv[4], o[4], mx = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = lane + 32 * j;
-    qv[j] = d < p.D ? to_f32(q[d]) * p.scale2 : 0.f;
-    o[j] = 0.f;
+  const int i = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (i >= n_words) return;
+  const int w = i % words, m = i / words % M, b = i / words / M;
+  const int j = 32 * w + lane;
+  const bool on = j < M && mask[b * stride_b + m * stride_m + j] != 0;
+  const uint32_t bits = __ballot_sync(0xffffffffu, on);
+  if (lane == 0) out[i] = bits;
+}
+
+template <typename T, int DPAD, bool PAIR, bool QUANT>
+__global__ void __launch_bounds__(tree_threads<QUANT>(), 1)
+tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                      const __grid_constant__ TreeParams p) {
+  using L = TreeSmem<DPAD, PAIR>;
+  constexpr int KS = L::KS, VS = L::VS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = ptx::smem_u32(smem);
+  if ((base & 1023u) != 0) {
+    if (threadIdx.x == 0) report_status(p, ST_SMEM_MISALIGNED, (int)base);
+    return;
   }
-  const long long have = max(0LL, min(load_index(p.lengths, p.index_bits, b), (long long)p.N));
-  const long long end = min(have + p.M, (long long)p.N);
-  for (long long n = 0; n < end; ++n) {
-    if (n >= have) {
-      const int j = (int)(n - have);
-      if (p.mask ? !p.mask[b * p.mask_b + m * p.mask_m + j] : j > m) continue;
+  const uint32_t bar0 = base + L::off_bars;
+  auto bar_q_full = [&](uint32_t i) { return bar0 + 8u * i; };
+  auto bar_q_empty = [&](uint32_t i) { return bar0 + 8u * (2 + i); };
+  auto bar_k_full = [&](uint32_t i) { return bar0 + 8u * (4 + i); };
+  auto bar_k_empty = [&](uint32_t i) { return bar0 + 8u * (4 + KS + i); };
+  auto bar_v_full = [&](uint32_t i) { return bar0 + 8u * (4 + 2 * KS + i); };
+  auto bar_v_empty = [&](uint32_t i) { return bar0 + 8u * (4 + 2 * KS + VS + i); };
+  auto bar_s = [&](uint32_t w) { return bar0 + 8u * (4 + 2 * KS + 2 * VS + w); };
+  auto bar_p = [&](uint32_t w) { return bar0 + 8u * (6 + 2 * KS + 2 * VS + w); };
+  auto bar_o = [&](uint32_t w) { return bar0 + 8u * (8 + 2 * KS + 2 * VS + w); };
+  const uint32_t bar_merge = bar0 + 8u * (10 + 2 * KS + 2 * VS);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::off_misc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 4);
+  volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 8);  // a drafted value was not finite
+  volatile int* start_b = reinterpret_cast<volatile int*>(smem + L::off_misc + 12);
+  volatile long long* start_off = reinterpret_cast<volatile long long*>(smem + L::off_misc + 16);
+  volatile long long* start_n = reinterpret_cast<volatile long long*>(smem + L::off_misc + 24);
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // warp-uniform for the compiler
+  const int lane = (int)(threadIdx.x & 31);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kQBuffers; ++i) {
+      ptx::mbar_init(bar_q_full(i), kTreeQWarps);
+      ptx::mbar_init(bar_q_empty(i), PAIR ? 1 : kTreeSoftmaxWarps);
     }
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = lane + 32 * j;
-      if (d < p.D) s = fmaf(qv[j], tree_load<T, FORMAT>(p, 0, b, h / p.G, n, d), s);
+    for (int i = 0; i < KS; ++i) {
+      ptx::mbar_init(bar_k_full(i), QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_k_empty(i), 1);
     }
+    for (int i = 0; i < VS; ++i) {
+      ptx::mbar_init(bar_v_full(i), QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_v_empty(i), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      ptx::mbar_init(bar_s(w), 1);
+      ptx::mbar_init(bar_p(w), 4);
+      ptx::mbar_init(bar_o(w), 1);
+    }
+    ptx::mbar_init(bar_merge, kTreeSoftmaxWarps);
+    *abort_flag = 0;
+    *bad_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == kTreeMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  if (!QUANT && warp == kTreeLoadWarp && lane == 0) {
+    ptx::prefetch_tensormap(&tmap_k);
+    ptx::prefetch_tensormap(&tmap_v);
+  }
+  if (threadIdx.x == 0) ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();  // the kernel before this one may have written lengths, cache or queries
+  if (blockIdx.x == 0 && threadIdx.x < 4) p.status[threadIdx.x] = 0;
+  const TreeLengths lengths{p.lengths, p.index_bits};
+  if (warp == kTreeQWarp) {
+    // this CTA's piece of the line of tiles: the total, then the sequence in which the piece begins
+    long long total = 0;
+    for (int b = lane; b < p.B; b += 32) total += tree_tiles(tree_have(lengths(b), p.N), p.M, p.N);
 #pragma unroll
-    for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    const float m_new = fmaxf(mx, s);
-    const float at = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = exp2f(mx - at), w = exp2f(s - at);
-    l = l * alpha + w;
-    mx = m_new;
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= p.groups;
+    const int ctas = tree_ctas(total, gridDim.x), c = min((int)blockIdx.x, ctas);
+    const long long lo = tree_piece(total, ctas, c), hi = c < ctas ? tree_piece(total, ctas, c + 1) : lo;
+    long long before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane;
+      const long long mine = b < p.B ? (long long)tree_tiles(tree_have(lengths(b), p.N), p.M, p.N) * p.groups : 0;
+      long long incl = mine;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = lane + 32 * j;
-      if (d < p.D) o[j] = o[j] * alpha + w * tree_load<T, FORMAT>(p, 1, b, h / p.G, n, d);
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      if (mine > 0 && before + incl - mine <= lo && lo < before + incl) {
+        *start_b = b;
+        *start_off = lo - (before + incl - mine);
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      if (before > lo) break;
+    }
+    if (lane == 0) *start_n = hi - lo;
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  TreeWalk<TreeLengths> walk{lengths, p.B, p.groups, p.M, p.N};
+  const long long n_tiles = *start_n;
+  walk.start(n_tiles > 0 ? *start_b : 0, *start_off, n_tiles);
+  TreeSegment seg{};
+
+  if (warp >= kTreeQWarp && warp < kTreeQWarp + kTreeQWarps) {
+    // ----------------------------------------------------- queries of the next segment
+    const int tid = threadIdx.x - 32 * kTreeQWarp;
+    const int rows_here = PAIR ? 256 : 128 / p.copies;
+    uint32_t seq = 0;
+    while (walk.next(seg)) {
+      const uint32_t buf = seq % L::kQBuffers, ph = (seq / L::kQBuffers) & 1u;
+      if (!WAIT_BEHIND(bar_q_empty(buf), ph ^ 1u, ST_TR_WAIT_Q_EMPTY)) break;
+      ++seq;
+      const int kh = seg.group / p.row_tiles, r0 = (seg.group - kh * p.row_tiles) * 256;
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)kh * p.G * p.qh;
+      const uint32_t dst0 = base + L::off_q + buf * L::kQBytes;
+      constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
+      constexpr int kAhead = 8;
+      const int pieces = rows_here * kChunks;
+      for (int i0 = tid; i0 < pieces; i0 += 32 * kTreeQWarps * kAhead) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = i0 + u * 32 * kTreeQWarps;
+          const int row = i / kChunks, d0 = (i % kChunks) * 8, r = r0 + row;
+          v[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (i < pieces && r < p.rows && d0 < p.D) {
+            const int g = r / p.M, m = r - g * p.M;
+            const unsigned short* src = q + g * p.qh + m * p.qm + d0;
+            if (p.q_vec) {
+              v[u] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              unsigned short* e = reinterpret_cast<unsigned short*>(&v[u]);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = src[j];
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int i = i0 + u * 32 * kTreeQWarps;
+          if (i < pieces) {
+            const int row = i / kChunks, c = i % kChunks;
+            for (int k = 0; k < (PAIR ? 1 : p.copies); ++k) {
+              const int at = row + k * rows_here;
+              const uint32_t tile = dst0 + (uint32_t)(at >> 7) * L::kTileBytes, in = (uint32_t)(at & 127);
+              ptx::sts128(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u, v[u]);
+            }
+          }
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_q_full(buf));
+    }
+  } else if (warp == kTreeMmaWarp) {
+    // ------------------------------------------------------------------- products
+    // Step j: tile j (PAIR: tile j / 2) for warpgroup j mod 2.  S runs two steps ahead of P V, which also orders
+    // the buffers: S of step j + 2 overwrites the P that the products of step j have read.
+    TreeWalk<TreeLengths> ahead = walk;
+    TreeSegment sa;
+    int s_left = 0, o_left = 0, s_done = 0;     // tiles left in the segment that S / P V is in
+    uint32_t s_tile = 0, o_tile = 0, q_seq = 0; // tiles so far
+    int o_done = 0;
+    bool ok = true;
+    const int per_tile = PAIR ? 2 : 1;
+    const long long steps = n_tiles * per_tile;
+    auto issue_s = [&](uint32_t w) {
+      const bool opens = !PAIR || w == 0, closes = !PAIR || w == 1;
+      if (opens) {
+        if (s_left == 0) {
+          ahead.next(sa);
+          s_left = sa.hi - sa.lo;
+          s_done = 0;
+          ok = WAIT(bar_q_full(q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
+          if (!ok) return;
+        }
+        ok = WAIT(bar_k_full(s_tile % KS), (s_tile / KS) & 1u, ST_TR_WAIT_K_FULL);
+        if (!ok) return;
+      }
+      ptx::tc_fence_after_sync();
+      if (ptx::elect_one()) {
+        const uint32_t a_lo = ptx::smem_desc_lo(base + L::off_q + (q_seq % L::kQBuffers) * L::kQBytes + (PAIR ? w * L::kTileBytes : 0));
+        const uint32_t b_lo = ptx::smem_desc_lo(base + L::off_k + (s_tile % KS) * L::kTileBytes);
+        const uint32_t d = tmem_base + 2 * DPAD + w * 128;
+#pragma unroll
+        for (int kk = 0; kk < DPAD / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk >> 2) * (L::kSlabBytes >> 4) + (uint32_t)(kk & 3) * 2u;
+          if (kk < p.k_steps) ptx::umma_step<false>(d, a_lo + off, b_lo + off, p.idesc_s, kk == 0);
+        }
+        ptx::umma_commit(bar_s(w));
+        if (closes) {
+          ptx::umma_commit(bar_k_empty(s_tile % KS));
+          if (PAIR && s_left == 1) ptx::umma_commit(bar_q_empty(q_seq % L::kQBuffers));
+        }
+      }
+      __syncwarp();
+      if (closes) {
+        ++s_tile;
+        ++s_done;
+        if (--s_left == 0) ++q_seq;
+      }
+    };
+    if (steps > 0) issue_s(0);
+    if (ok && steps > 1) issue_s(1);
+    for (long long j = 0; ok && j < steps; ++j) {
+      const uint32_t w = (uint32_t)j & 1u;
+      const bool opens = !PAIR || w == 0, closes = !PAIR || w == 1;
+      if (opens && o_left == 0) {
+        walk.next(seg);
+        o_left = seg.hi - seg.lo;
+        o_done = 0;
+      }
+      if (opens) {
+        ok = WAIT(bar_v_full(o_tile % VS), (o_tile / VS) & 1u, ST_TR_WAIT_V_FULL);
+        if (!ok) break;
+      }
+      ok = WAIT_BEHIND(bar_p(w), (uint32_t)(j >> 1) & 1u, ST_TR_WAIT_P);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      if (ptx::elect_one()) {
+        const uint32_t b_lo = ptx::smem_desc_lo_mn(base + L::off_v + (o_tile % VS) * L::kTileBytes, L::kSlabBytes);
+        const uint32_t a = tmem_base + 2 * DPAD + w * 128, d = tmem_base + w * DPAD;
+        const bool first = o_done < (PAIR ? 1 : 2);  // this warpgroup's first tile of the segment
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) ptx::umma_f16_ts(d, a + 8 * kk, b_lo + kk * (2048u >> 4), p.idesc_o, !(first && kk == 0));
+        if (closes) ptx::umma_commit(bar_v_empty(o_tile % VS));
+        if (o_left <= (PAIR ? 1 : 2)) ptx::umma_commit(bar_o(w));  // ... and its last one
+      }
+      __syncwarp();
+      if (closes) {
+        ++o_tile;
+        ++o_done;
+        --o_left;
+      }
+      if (j + 2 < steps) issue_s(w);
+    }
+  } else if (warp >= kTreeLoadWarp) {
+    // -------------------------------------------------------- key and value tiles
+    uint32_t seq = 0;  // tiles so far
+    bool ok = true;
+    if constexpr (!QUANT) {
+      auto load = [&](auto is_v, int t) {
+        constexpr int kv = decltype(is_v)::value;
+        constexpr uint32_t kSlots = kv ? VS : KS;
+        const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
+        const uint32_t full = kv ? bar_v_full(slot) : bar_k_full(slot);
+        ok = WAIT_BEHIND(kv ? bar_v_empty(slot) : bar_k_empty(slot), ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+        if (!ok) return;
+        const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
+        if (lane == 0 && !left_out) {
+          const uint32_t dst = base + (kv ? L::off_v : L::off_k) + slot * L::kTileBytes;
+          ptx::mbar_arrive_expect_tx(full, L::kTileBytes);
+#pragma unroll
+          for (int sl = 0; sl < DPAD / 64; ++sl)
+            ptx::tma_load_4d(dst + sl * L::kSlabBytes, kv ? &tmap_v : &tmap_k, full, sl * 64, t * kTreeTile, seg.group / p.row_tiles, seg.b);
+        }
+        __syncwarp();
+      };
+      while (ok && walk.next(seg)) {
+        for (int t = seg.lo; t < seg.hi; ++t) {
+          load(std::integral_constant<int, 0>{}, t);
+          if (!ok) break;
+          load(std::integral_constant<int, 1>{}, t);
+          if (!ok) break;
+          ++seq;
+        }
+      }
+    } else {
+      constexpr int kPerRow = DPAD / 16;                            // 16-code pieces of a row
+      constexpr int kRows = 32 * kTreeConvertWarps / kPerRow;       // rows the warps take at a time
+      constexpr int kPasses = 128 / kRows;
+      const int tid = threadIdx.x - 32 * kTreeLoadWarp;
+      const int piece = tid % kPerRow, row0 = tid / kPerRow;
+      const bool on = piece * 16 < p.D;
+      struct Batch {
+        uint4 codes[kPasses];
+        uint32_t scale[kPasses];
+      };
+      // where the tile to load next lies, and what the tile to store next needs of its own
+      int t_load = 0;
+      const unsigned char* src[2];
+      const unsigned char* sc[2];
+      auto advance = [&]() {
+        if (++t_load < seg.hi && t_load > 0) return;
+        if (!walk.next(seg)) return;
+        t_load = seg.lo;
+        const int h = seg.group / p.row_tiles;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          src[kv] = reinterpret_cast<const unsigned char*>(p.cache[kv]) + seg.b * p.cb[kv] + h * p.ch[kv] + piece * 16;
+          sc[kv] = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
+        }
+      };
+      auto load = [&](auto is_v, Batch& x) {
+        constexpr int kv = decltype(is_v)::value;
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int n = t_load * kTreeTile + row0 + k * kRows;
+          x.codes[k] = make_uint4(0u, 0u, 0u, 0u);
+          x.scale[k] = 127u;
+          if (n < seg.end && on) {
+            x.codes[k] = *reinterpret_cast<const uint4*>(src[kv] + n * p.cn[kv]);
+            x.scale[k] = sc[kv][n * p.sn[kv]];
+          }
+        }
+      };
+      auto store = [&](auto is_v, Batch& x, int drafted) {  // drafted: the tile's first row that is a drafted token's
+        constexpr int kv = decltype(is_v)::value;
+        constexpr uint32_t kSlots = kv ? VS : KS;
+        const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
+        ok = WAIT_BEHIND(kv ? bar_v_empty(slot) : bar_k_empty(slot), ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+        if (!ok) return;
+        const uint32_t dst = base + (kv ? L::off_v : L::off_k) + slot * L::kTileBytes;
+#pragma unroll
+        for (int k = 0; k < kPasses; ++k) {
+          const int row = row0 + k * kRows;
+          const float scale = kv_scale(x.scale[k]);
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(&x.codes[k]);
+          uint32_t o[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[4];
+            if (p.format == FCR_KV_FP8) unpack_codes4<FCR_KV_FP8>(w[q], v); else unpack_codes4<FCR_KV_INT8>(w[q], v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= scale;
+            if (kv == 1 && row >= drafted) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (!(fabsf(v[e]) < INFINITY)) {
+                  v[e] = 0.f;
+                  *bad_flag = 1;
+                }
+              }
+            }
+            o[2 * q] = pack2(v[0], v[1], T());
+            o[2 * q + 1] = pack2(v[2], v[3], T());
+          }
+          // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
+          const uint32_t at_row = dst + (uint32_t)(piece >> 2) * L::kSlabBytes + (uint32_t)row * 128u;
+          const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
+          const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
+          ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
+          ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
+        if (lane == 0 && !left_out) ptx::mbar_arrive(kv ? bar_v_full(slot) : bar_k_full(slot));
+      };
+      // the codes of the next tile are under way while one is converted
+      Batch kb, vb;
+      const std::integral_constant<int, 0> is_k{};
+      const std::integral_constant<int, 1> is_v{};
+      t_load = -1;
+      if (n_tiles > 0) {
+        advance();
+        load(is_k, kb);
+      }
+      for (long long i = 0; ok && i < n_tiles; ++i) {
+        const int drafted = seg.have - t_load * kTreeTile;
+        load(is_v, vb);
+        store(is_k, kb, drafted);
+        if (!ok) break;
+        if (i + 1 < n_tiles) {
+          advance();
+          load(is_k, kb);
+        }
+        store(is_v, vb, drafted);
+        if (!ok) break;
+        ++seq;
+      }
+    }
+    // no arrival may be outstanding when the CTA retires: wait until the products have given back every slot
+    for (uint32_t i = 0; ok && i < KS && i < seq; ++i) {
+      const uint32_t last = seq - 1 - i;
+      ok = WAIT_BEHIND(bar_k_empty(last % KS), (last / KS) & 1u, ST_TR_WAIT_DRAIN);
+      if (ok && i < VS) ok = WAIT_BEHIND(bar_v_empty(last % VS), (last / VS) & 1u, ST_TR_WAIT_DRAIN);
+    }
+  } else {
+    // -------------------------------------------------------------- softmax warps
+    const int w = warp >> 2;
+    const int lane_row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem_base + lanes + 2 * DPAD + w * 128, o_addr = tmem_base + lanes + w * DPAD;
+    const int rows_here = PAIR ? 128 : 128 / p.copies;
+    const int copy = (warp & 3) * 32 / rows_here, local = lane_row - copy * rows_here;  // copy: the same for a warp
+    const int c_lo = PAIR ? 0 : copy * (4 / p.copies), c_hi = PAIR ? 4 : c_lo + 4 / p.copies;
+    uint32_t tile_seq = 0;   // tiles of this CTA so far
+    uint32_t s_use = 0, o_use = 0, merge_use = 0, q_seq = 0;
+    bool ok = true;
+    auto sync_all = [&]() {  // a bounded barrier over the eight warps
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar_merge);
+      ok = WAIT_BEHIND(bar_merge, merge_use & 1u, ST_TR_WAIT_MERGE);
+      ++merge_use;
+      return ok;
+    };
+    while (ok && walk.next(seg)) {
+      const int kh = seg.group / p.row_tiles;
+      const int row = (seg.group - kh * p.row_tiles) * 256 + (PAIR ? w * 128 : 0) + local;  // of the G * M
+      const bool real = row < p.rows;
+      const int m = real ? row % p.M : 0;
+      const uint32_t* words = p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + m) * p.words : nullptr;
+      float m_ref = -INFINITY, l = 0.f;
+      int mine = 0;  // tiles this warpgroup has taken
+      for (int t = seg.lo; t < seg.hi; ++t, ++tile_seq) {
+        if (!PAIR && (int)(tile_seq & 1u) != w) continue;
+        ok = WAIT(bar_s(w), s_use & 1u, ST_TR_WAIT_S);
+        if (!ok) break;
+        ++s_use;
+        ptx::tc_fence_after_sync();
+        const bool edge = (t + 1) * kTreeTile > seg.have;
+        uint32_t ra[32];
+        float top = -INFINITY;
+        for (int c = c_lo; c < c_hi; ++c) {
+          ptx::tmem_ld<32>(s_addr + 32 * c, ra);
+          ptx::tmem_ld_wait<32>(ra);
+          if (edge) {
+            const uint32_t bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ra[e] = (bits >> e) & 1u ? ra[e] : 0xff800000u;
+          }
+          float t0 = __uint_as_float(ra[0]), t1 = __uint_as_float(ra[1]);
+#pragma unroll
+          for (int e = 2; e < 32; e += 4) {
+            t0 = ptx::max3(t0, __uint_as_float(ra[e]), __uint_as_float(ra[e + 1]));
+            if (e + 3 < 32) t1 = ptx::max3(t1, __uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3]));
+          }
+          top = ptx::max3(top, t0, t1);
+        }
+        top *= p.scale2;
+        // the reference moves when the maximum has grown by more than 2^8: P stays below that, far from any type's limits
+        const bool grow = real && top > m_ref + 8.f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? top : m_ref;
+          const float alpha = m_new == m_ref ? 1.f : ptx::ex2(m_ref - m_new);
+          m_ref = m_new;
+          l *= alpha;
+          if (mine > 0) {
+            for (int c = 0; c < DPAD / 32; ++c) {
+              ptx::tmem_ld<32>(o_addr + 32 * c, ra);
+              ptx::tmem_ld_wait<32>(ra);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) ra[e] = __float_as_uint(__uint_as_float(ra[e]) * alpha);
+              ptx::tmem_st32(o_addr + 32 * c, ra);
+            }
+          }
+        }
+        const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+        float2 s01 = make_float2(0.f, 0.f), s23 = make_float2(0.f, 0.f);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+          if (c >= c_lo && c < c_hi) {
+            ptx::tmem_ld<32>(s_addr + 32 * c, ra);
+            ptx::tmem_ld_wait<32>(ra);
+            uint32_t bits = 0xffffffffu;
+            if (edge) bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              float2 a = __ffma2_rn(make_float2(__uint_as_float(ra[e]), __uint_as_float(ra[e + 1])), make_float2(p.scale2, p.scale2),
+                                    make_float2(nm, nm));
+              float2 b = __ffma2_rn(make_float2(__uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3])), make_float2(p.scale2, p.scale2),
+                                    make_float2(nm, nm));
+              a.x = ptx::ex2(a.x);
+              a.y = ptx::ex2(a.y);
+              b.x = ptx::ex2(b.x);
+              b.y = ptx::ex2(b.y);
+              if (edge) {
+                a.x = (bits >> e) & 1u ? a.x : 0.f;
+                a.y = (bits >> (e + 1)) & 1u ? a.y : 0.f;
+                b.x = (bits >> (e + 2)) & 1u ? b.x : 0.f;
+                b.y = (bits >> (e + 3)) & 1u ? b.y : 0.f;
+              }
+              s01 = __fadd2_rn(s01, a);
+              s23 = __fadd2_rn(s23, b);
+              pk[e / 2] = pack2(a.x, a.y, T());
+              pk[e / 2 + 1] = pack2(b.x, b.y, T());
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+          }
+          // P chunk c covers columns 16 c .. 16 c + 15: scores that this thread has read, or does not need
+          ptx::tmem_st16(s_addr + 16 * c, pk);
+        }
+        l += (s01.x + s01.y) + (s23.x + s23.y);
+        ptx::tmem_st_wait();
+        ++mine;
+        if (!QUANT && edge) {
+          // values behind the last drafted token become zeros, and non-finite ones of the drafted tokens
+          const uint32_t slot = tile_seq % VS;
+          ok = WAIT(bar_v_full(slot), (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
+          if (!ok) break;
+          const int key = t * kTreeTile + lane_row;
+          if (key >= seg.have) {
+            constexpr int kHalf = DPAD / 16;  // PAIR: each warpgroup takes half of the 16-byte pieces
+            for (int c = PAIR ? w * kHalf : 0; c < (PAIR ? (w + 1) * kHalf : 2 * kHalf); ++c) {
+              const uint32_t a = base + L::off_v + slot * L::kTileBytes + (uint32_t)(c >> 3) * L::kSlabBytes + (uint32_t)lane_row * 128u +
+                                 (((uint32_t)c & 7u) ^ ((uint32_t)lane_row & 7u)) * 16u;
+              if (key >= seg.end) {
+                ptx::sts128(a, make_uint4(0u, 0u, 0u, 0u));
+              } else {
+                uint4 v = ptx::lds128(a);
+                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if (non_finite16<T>(e[i] & 0xffffu)) {
+                    e[i] &= 0xffff0000u;
+                    bad = true;
+                  }
+                  if (non_finite16<T>(e[i] >> 16)) {
+                    e[i] &= 0xffffu;
+                    bad = true;
+                  }
+                }
+                if (bad) {
+                  ptx::sts128(a, v);
+                  *bad_flag = 1;
+                }
+              }
+            }
+          }
+          ptx::fence_proxy_async_smem();
+          if (PAIR && !sync_all()) break;  // both warpgroups' halves are done before either's product
+        }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar_p(w));
+      }
+      if (!ok) break;
+      // ------------------------------------------------ the segment's results
+      if (mine > 0) {
+        ok = WAIT(bar_o(w), o_use & 1u, ST_TR_WAIT_O);
+        if (!ok) break;
+        ++o_use;
+        ptx::tc_fence_after_sync();
+      }
+      const bool whole = seg.whole();
+      const size_t part = ((size_t)blockIdx.x * 2 + seg.slot()) * p.part_rows;
+      const size_t out_row0 = (size_t)(seg.b * p.Hk + kh) * p.rows;
+      if constexpr (PAIR) {
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const int in_part = w * 128 + local;
+        for (int c = 0; c < DPAD / 32; ++c) {
+          uint32_t ra[32];
+          ptx::tmem_ld<32>(o_addr + 32 * c, ra);
+          ptx::tmem_ld_wait<32>(ra);
+          if (!real || 32 * c >= p.D) continue;
+          float o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : __uint_as_float(ra[e]) * inv;
+          if (*bad_flag) {
+            float fix[32];
+            for (int e = 0; e < 32; ++e) fix[e] = o[e];
+            tree_add_non_finite<T, QUANT>(p, seg, words, m, 32 * c, 32, fix);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = fix[e];
+          }
+          if (whole) {
+            T* dst = reinterpret_cast<T*>(p.out) + (out_row0 + row) * p.D + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              if (32 * c + e < p.D)
+                *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack2(o[e], o[e + 1], T()), pack2(o[e + 2], o[e + 3], T()),
+                                                                pack2(o[e + 4], o[e + 5], T()), pack2(o[e + 6], o[e + 7], T()));
+            }
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (part + in_part) * DPAD + 32 * c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (real) {
+          if (!whole)
+            p.part_ml[part + in_part] = make_float2(m_ref, l);
+          else if (p.lse)
+            p.lse[out_row0 + row] = l == 0.f ? -INFINITY : (m_ref + log2f(l)) * 0.69314718055994531f;
+        }
+      } else {
+        // merge the two warpgroups and the copies of a row: 2 * copies states
+        float2* stat = reinterpret_cast<float2*>(smem + L::off_stat);
+        float* buf = reinterpret_cast<float*>(smem + L::off_q + (q_seq % L::kQBuffers) * L::kQBytes);
+        const int tid = (int)threadIdx.x;
+        stat[tid] = make_float2(m_ref, l);
+        if (!sync_all()) break;
+        const int states = 2 * p.copies;  // state s of row r: lane (s mod copies) * rows_here + r of warpgroup s / copies
+        float m_all = -INFINITY, l_all = 0.f;
+        for (int s = 0; s < states; ++s) m_all = fmaxf(m_all, stat[(s / p.copies) * 128 + (s % p.copies) * rows_here + local].x);
+        const float m_use = m_all == -INFINITY ? 0.f : m_all;
+        for (int s = 0; s < states; ++s) {
+          const float2 v = stat[(s / p.copies) * 128 + (s % p.copies) * rows_here + local];
+          l_all += v.y * ptx::ex2(v.x - m_use);
+        }
+        float f = ptx::ex2(m_ref - m_use);
+        if (whole) f *= l_all == 0.f ? 0.f : 1.f / l_all;
+        const bool none = mine == 0 || l == 0.f;  // nothing summed here: the accumulator may hold anything
+        if (w == 0 && copy == 0 && real) {
+          if (!whole)
+            p.part_ml[part + local] = make_float2(m_all, l_all);
+          else if (p.lse)
+            p.lse[out_row0 + row] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * 0.69314718055994531f;
+        }
+        for (int c = 0; ok && 32 * c < p.D; ++c) {
+          uint32_t ra[32];
+          if (mine > 0) {
+            ptx::tmem_ld<32>(o_addr + 32 * c, ra);
+            ptx::tmem_ld_wait<32>(ra);
+          }
+          float4* dst = reinterpret_cast<float4*>(buf) + tid * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float4 v = make_float4(__uint_as_float(ra[4 * e]) * f, __uint_as_float(ra[4 * e + 1]) * f, __uint_as_float(ra[4 * e + 2]) * f,
+                                   __uint_as_float(ra[4 * e + 3]) * f);
+            if (none) v = make_float4(0.f, 0.f, 0.f, 0.f);
+            dst[e ^ (tid & 7)] = v;  // 16-byte pieces in another order per row: no bank is asked for twice
+          }
+          if (!sync_all()) break;
+          for (int i = tid; i < rows_here * 8; i += 256) {
+            const int r = i >> 3, piece = i & 7;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int s = 0; s < states; ++s) {
+              const int at = (s / p.copies) * 128 + (s % p.copies) * rows_here + r;
+              const float4 v = reinterpret_cast<const float4*>(buf)[at * 8 + (piece ^ (at & 7))];
+              sum.x += v.x;
+              sum.y += v.y;
+              sum.z += v.z;
+              sum.w += v.w;
+            }
+            const int d = 32 * c + 4 * piece;
+            if (r < p.rows && d < p.D) {
+              if (*bad_flag) {
+                float o[4] = {sum.x, sum.y, sum.z, sum.w};
+                const int rm = r % p.M;
+                tree_add_non_finite<T, QUANT>(p, seg, p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + rm) * p.words : nullptr,
+                                              rm, d, 4, o);
+                sum = make_float4(o[0], o[1], o[2], o[3]);
+              }
+              if (whole)
+                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (out_row0 + r) * p.D + d) =
+                    make_uint2(pack2(sum.x, sum.y, T()), pack2(sum.z, sum.w, T()));
+              else
+                *reinterpret_cast<float4*>(p.part_o + (part + r) * DPAD + d) = sum;
+            }
+          }
+          if (!sync_all()) break;
+        }
+        if (!ok) break;
+        if (lane == 0) ptx::mbar_arrive(bar_q_empty(q_seq % L::kQBuffers));
+        ++q_seq;
+      }
     }
   }
-  T* out = reinterpret_cast<T*>(p.out) + r * p.D;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d = lane + 32 * j;
-    if (d < p.D) out[d] = from_f32<T>(l == 0.f ? 0.f : o[j] / l);
+
+  // ------------------------------------------------------------- teardown
+  __syncwarp();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {
+    // A wait expired somewhere: give loads that may still be in flight time to
+    // land in this CTA's shared memory before it is released.
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    __syncthreads();
   }
-  if (p.lse && lane == 0) p.lse[r] = l == 0.f ? -INFINITY : (mx + log2f(l)) * 0.69314718055994531f;
+  if (warp == kTreeMmaWarp) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// Joins the partial results of groups whose keys more than one CTA took, in the order of the keys.  A block per group and
+// eight rows of it; a warp per row.
+template <typename T, int DPAD>
+__global__ void __launch_bounds__(256)
+tree_combine_kernel(const __grid_constant__ TreeParams p, int ctas, int rows_per_tile, int blocks_per_group) {
+  __shared__ long long warp_sum[2][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  const int item = blockIdx.x / blocks_per_group;  // sequence * groups + group
+  const int b = item / p.groups, group = item - b * p.groups;
+  const TreeLengths lengths{p.lengths, p.index_bits};
+  long long before = 0, total = 0;
+  for (int i = threadIdx.x; i < p.B; i += 256) {
+    const int t = tree_tiles(tree_have(lengths(i), p.N), p.M, p.N);
+    total += t;
+    if (i < b) before += t;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) {
+    warp_sum[0][warp] = total;
+    warp_sum[1][warp] = before;
+  }
+  __syncthreads();
+  total = before = 0;
+  for (int i = 0; i < 8; ++i) {
+    total += warp_sum[0][i];
+    before += warp_sum[1][i];
+  }
+  total *= p.groups;
+  ctas = tree_ctas(total, ctas);
+  const int tiles = tree_tiles(tree_have(lengths(b), p.N), p.M, p.N);
+  const long long first = before * p.groups + (long long)group * tiles;
+  const int c0 = tree_owner(total, ctas, first), c1 = tree_owner(total, ctas, first + tiles - 1);
+  if (c0 == c1) return;  // one CTA took all of it and has written the result
+  const int kh = group / p.row_tiles, r0 = (group - kh * p.row_tiles) * 256;
+  const int local = (blockIdx.x - item * blocks_per_group) * 8 + warp;
+  const int row = r0 + local;
+  if (local >= rows_per_tile || row >= p.rows) return;
+  // the first CTA's part starts the group (its second slot), the others' continue it (their first slot)
+  auto slot_row = [&](int c) { return ((size_t)c * 2 + (c == c0 ? 1 : 0)) * p.part_rows + local; };
+  float m_all = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m_all = fmaxf(m_all, p.part_ml[slot_row(c)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+  const float m_use = m_all == -INFINITY ? 0.f : m_all;
+  float l_all = 0.f;
+  constexpr int kVec = DPAD / 32;  // columns per lane
+  float acc[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
+  for (int c = c0; c <= c1; ++c) {
+    const float2 ml = p.part_ml[slot_row(c)];
+    const float f = ptx::ex2(ml.x - m_use);
+    l_all += ml.y * f;
+    if (ml.y != 0.f && lane * kVec < p.D) {
+      const float* o = p.part_o + slot_row(c) * DPAD + lane * kVec;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) acc[e] += o[e] * f;
+    }
+  }
+  const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+  const size_t out_row = (size_t)(b * p.Hk + kh) * p.rows + row;
+  if (lane * kVec < p.D) {
+    T* dst = reinterpret_cast<T*>(p.out) + out_row * p.D + lane * kVec;
+#pragma unroll
+    for (int e = 0; e < kVec; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack2(acc[e] * inv, acc[e + 1] * inv, T());
+  }
+  if (p.lse && lane == 0) p.lse[out_row] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * 0.69314718055994531f;
 }
 
 }  // namespace fcr

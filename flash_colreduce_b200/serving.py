@@ -299,7 +299,7 @@ def tree_attention(
             of ``query``'s type with D a multiple of 8, or float8_e4m3fn / int8 with D a multiple of 16.  Base addresses
             and strides are multiples of 16 bytes.
         lengths: (B,) int32 or int64, on the GPU: a captured graph may be replayed with other values.
-        tree_mask: (M, M) or (B, M, M) bool, or None.
+        tree_mask: (M, M), (1, M, M) or (B, M, M) bool, or None.
         scale: softmax scale, default ``1 / sqrt(D)``.
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
 
@@ -315,7 +315,7 @@ def tree_attention(
     hq, m = query.shape[1], query.shape[2]
     if m > 256:
         raise ValueError(f"{m} drafted tokens exceed 256.")
-    if tree_mask is not None and (tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((m, m), (b, m, m))):
+    if tree_mask is not None and (tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((m, m), (1, m, m), (b, m, m))):
         raise ValueError(f"tree_mask must be bool of shape ({m}, {m}) or ({b}, {m}, {m}); got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
     lengths = _lengths("lengths", lengths, b)
     scale = 1 / math.sqrt(d) if scale is None else float(scale)
@@ -330,7 +330,7 @@ def tree_attention(
     tree = nat.Tree(hq, m, (*query.stride()[:3], 1), _INDEX_BITS[lengths.dtype], (0, 0), scale)
     if tree_mask is not None:
         tree_mask = _rows(tree_mask)
-        tree.mask_strides[:] = (tree_mask.stride(0) if tree_mask.dim() == 3 else 0, tree_mask.stride(-2))
+        tree.mask_strides[:] = (tree_mask.stride(0) if tree_mask.dim() == 3 and tree_mask.shape[0] > 1 else 0, tree_mask.stride(-2))
     index = query.device.index
     with _on_device(index):
         ws_bytes = nat.lib.fcr_tree_workspace_bytes(C.byref(problem), C.byref(tree), 0)

@@ -478,11 +478,22 @@ typedef struct fcr_tree {
   float scale;
 } fcr_tree;
 
+/* Bytes of workspace (256-byte aligned, any contents) for a device with num_sms SMs (0: the current device); 0 on error. */
 size_t fcr_tree_workspace_bytes(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t num_sms);
 int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const void* q, const void* k_cache,
                        const void* v_cache, const void* k_scales, const void* v_scales, const void* lengths,
                        const void* mask, void* out, float* lse, void* workspace, size_t workspace_bytes,
                        void* stream);
+
+/*
+ * Pure host function: segment `index` of what CTA `cta` of the attention kernel runs on a device with num_sms
+ * SMs, by the routine that the kernel runs; `lengths` is a host array here.  The 128-key tiles of all (sequence,
+ * cache head, row tile) groups are one line, cut into pieces of equal length.  out[10] receives {sequence, cache
+ * head, row tile, first tile, last tile + 1, tiles of the group, partial slot (-1: the whole group), CTA of the
+ * group's first tile, CTA of its last, CTAs}.  FCR_ERR_BAD_ARG when there is no such segment.
+ */
+int fcr_tree_segment(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t num_sms, const int64_t* lengths,
+                     int32_t cta, int32_t index, int32_t* out);
 
 #ifdef __cplusplus
 }

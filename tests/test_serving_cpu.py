@@ -226,3 +226,43 @@ def test_attention_oracle_on_closed_forms():
         assert torch.allclose(lse[0, :, m].exp(), torch.tensor(5.0 + m).double())
     out, lse, _ = attention(q, k, k, torch.tensor([0]), mask=torch.zeros(3, 3, dtype=torch.bool))
     assert (out == 0).all() and (lse == -float("inf")).all()
+
+
+# ---------------------------------------------------------------------------------------- the attention's work items
+@pytest.mark.parametrize("sms", [1, 7, 148])
+@pytest.mark.parametrize("b,h,hq,m,n,lens", [
+    (1, 1, 1, 1, 1, [0]), (3, 1, 8, 1, 400, [0, 1, 399]), (2, 2, 8, 64, 5000, [4000, 17]), (1, 2, 4, 200, 3000, [2900]), (5, 3, 3, 7, 1000, [990, -4, 2000, 0, 128]),
+    (40, 8, 32, 1, 900, [(37 * i) % 900 for i in range(40)]), (1, 8, 32, 1, 131072, [131071]),
+])
+def test_every_tile_belongs_to_one_cta_and_partial_results_have_no_gaps(sms, b, h, hq, m, n, lens):
+    cache = nat.KvCache(b, h, n, 128, nat.FCR_KV_16BIT, nat.FCR_BF16, (h * n * 128, n * 128, 128, 1), (h * n * 128, n * 128, 128, 1), (0, 0, 0), (0, 0, 0))
+    tree = nat.Tree(hq, m, (hq * m * 128, m * 128, 128, 1), 32, (0, 0), 0.1)
+    rows = hq // h * m
+    row_tiles = 1 if rows <= 128 else -(-rows // 256)
+    buf, host = (C.c_int32 * 10)(), (C.c_int64 * b)(*lens)
+    seen, loads, parts = {}, {}, {}
+    for cta in range(min(sms, b * h * row_tiles * -(-n // 128))):
+        i = 0
+        while nat.lib.fcr_tree_segment(C.byref(cache), C.byref(tree), sms, host, cta, i, buf) == nat.FCR_OK:
+            seq, head, rt, lo, hi, tiles, slot, first, last, ctas = buf
+            have = min(max(lens[seq], 0), n)
+            assert tiles == -(-min(have + m, n) // 128) and 0 <= lo < hi <= tiles and rt < row_tiles
+            assert (slot == -1) == (lo == 0 and hi == tiles) == (first == last)
+            if slot >= 0:
+                assert slot == (1 if lo == 0 else 0) and (cta, slot) not in parts
+                parts[cta, slot] = (seq, head, rt)
+                # what the joining kernel reads: slot 1 of the group's first CTA, slot 0 of the others
+                assert first <= cta <= last and (slot == 1) == (cta == first)
+            for t in range(lo, hi):
+                assert (seq, head, rt, t) not in seen
+                seen[seq, head, rt, t] = cta
+            loads[cta] = loads.get(cta, 0) + hi - lo
+            i += 1
+            assert ctas <= sms
+    want = sum(-(-min(min(max(x, 0), n) + m, n) // 128) for x in lens) * h * row_tiles
+    assert len(seen) == want and max(loads.values()) - min(loads.values()) <= 1
+    groups = {}
+    for (seq, head, rt, t), cta in seen.items():
+        groups.setdefault((seq, head, rt), set()).add(cta)
+    for key, owners in groups.items():
+        assert owners == set(range(min(owners), max(owners) + 1))
