@@ -346,6 +346,6 @@ def tree_attention(
             raise ValueError(nat.last_error())
         if rc:
             nat.check(rc, "fcr_tree_attention")
-        if _debug_sync():
+        if _debug_sync() and not torch.cuda.is_current_stream_capturing():
             nat.check(nat.lib.fcr_read_device_status(ws.data_ptr(), stream, None), "fcr_tree_attention (device)")
     return (out, lse) if return_lse else out
