@@ -1769,4 +1769,5 @@ int fcr_select_above(const void* scores, int32_t dtype, int32_t rows, int32_t n,
 #include "rope_sm100.cuh"
 #include "kvcache_sm100.cuh"
 #include "treeattn_sm100.cuh"
+#include "treedecode_sm100.cuh"
 #include "serving.cuh"

@@ -108,7 +108,7 @@ struct HostLengths {
 
 // What the host decides of an attention call: the kernel's variant and the workspace.
 struct TreePlan {
-  int rows, copies, part_rows, row_tiles, ctas, words, mask_rows;
+  int rows, decode_rows, part_rows, row_tiles, ctas, words, mask_rows;
   bool pair;
   int d_pad;
   size_t off_mask, off_ml, off_o, bytes;
@@ -118,8 +118,8 @@ static TreePlan plan_tree(const fcr_kv_cache& c, const fcr_tree& t, int sms) {
   pl.rows = t.Hq / c.H * t.M;
   pl.pair = pl.rows > 128;
   pl.row_tiles = pl.pair ? (pl.rows + 255) / 256 : 1;
-  pl.copies = pl.rows <= 32 ? 4 : pl.rows <= 64 ? 2 : 1;
-  pl.part_rows = pl.pair ? 256 : 128 / pl.copies;
+  pl.decode_rows = pl.rows > 64 ? 0 : pl.rows <= 16 ? 16 : pl.rows <= 32 ? 32 : 64;
+  pl.part_rows = pl.pair ? 256 : pl.decode_rows ? pl.decode_rows : 128;
   pl.d_pad = c.D <= 64 ? 64 : 128;
   const long long most = (long long)c.B * c.H * pl.row_tiles * ((c.N + kTreeTile - 1) / kTreeTile);
   pl.ctas = (int)std::min<long long>(most, sms);
@@ -133,11 +133,10 @@ static TreePlan plan_tree(const fcr_kv_cache& c, const fcr_tree& t, int sms) {
   return pl;
 }
 
-template <typename T, int DPAD, bool PAIR, bool QUANT>
-static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
-  auto kern = tree_attention_kernel<T, DPAD, PAIR, QUANT>;
-  constexpr int smem = TreeSmem<DPAD, PAIR>::kDynamicBytes;
-  static std::atomic<unsigned long long> opted_in{0};
+template <typename T, int DPAD>
+static int launch_tree_kernel(void (*kern)(const CUtensorMap, const CUtensorMap, const TreeParams), int smem, int threads,
+                              std::atomic<unsigned long long>& opted_in, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                              const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   const unsigned long long bit = 1ULL << (t_device & 63);
   if (!(opted_in.load(std::memory_order_acquire) & bit)) {
@@ -145,7 +144,7 @@ static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     opted_in.fetch_or(bit, std::memory_order_release);
   }
-  e = launch_kernel(kern, dim3(pl.ctas), dim3(tree_threads<QUANT>()), smem, stream, true, map_k, map_v, p);
+  e = launch_kernel(kern, dim3(pl.ctas), dim3(threads), smem, stream, true, map_k, map_v, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "tree attention launch");
   if (p.N > kTreeTile && pl.ctas > 1) {  // a group of one tile is never shared
@@ -159,12 +158,31 @@ static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const
   }
   return FCR_OK;
 }
-template <typename T, int DPAD>
-static int launch_tree_d(bool quant, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
+template <typename T, int DPAD, bool PAIR, bool QUANT>
+static int launch_tree_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
+  static std::atomic<unsigned long long> opted_in{0};
+  return launch_tree_kernel<T, DPAD>(tree_attention_kernel<T, DPAD, PAIR, QUANT>, TreeSmem<DPAD, PAIR>::kDynamicBytes, tree_threads<QUANT>(),
+                                     opted_in, map_k, map_v, p, pl, stream);
+}
+template <typename T, int DPAD, int NR, bool QUANT>
+static int launch_tree_keys(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
+  static std::atomic<unsigned long long> opted_in{0};
+  return launch_tree_kernel<T, DPAD>(tree_decode_kernel<T, DPAD, NR, QUANT>, DecodeSmem<DPAD, NR>::kDynamicBytes, decode_threads<QUANT>(), opted_in,
+                                     map_k, map_v, p, pl, stream);
+}
+template <typename T, int DPAD, bool QUANT>
+static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
+  if (pl.pair) return launch_tree_rows<T, DPAD, true, QUANT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 0) return launch_tree_rows<T, DPAD, false, QUANT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 16) return launch_tree_keys<T, DPAD, 16, QUANT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 32) return launch_tree_keys<T, DPAD, 32, QUANT>(map_k, map_v, p, pl, stream);
+  return launch_tree_keys<T, DPAD, 64, QUANT>(map_k, map_v, p, pl, stream);
+}
+template <typename T>
+static int launch_tree_d(int d_pad, bool quant, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
                          cudaStream_t stream) {
-  if (pl.pair)
-    return quant ? launch_tree<T, DPAD, true, true>(map_k, map_v, p, pl, stream) : launch_tree<T, DPAD, true, false>(map_k, map_v, p, pl, stream);
-  return quant ? launch_tree<T, DPAD, false, true>(map_k, map_v, p, pl, stream) : launch_tree<T, DPAD, false, false>(map_k, map_v, p, pl, stream);
+  if (d_pad == 64) return quant ? launch_tree<T, 64, true>(map_k, map_v, p, pl, stream) : launch_tree<T, 64, false>(map_k, map_v, p, pl, stream);
+  return quant ? launch_tree<T, 128, true>(map_k, map_v, p, pl, stream) : launch_tree<T, 128, false>(map_k, map_v, p, pl, stream);
 }
 
 }  // namespace fcr
@@ -426,7 +444,6 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.rows = pl.rows;
   p.row_tiles = pl.row_tiles;
   p.groups = c.H * pl.row_tiles;
-  p.copies = pl.copies;
   p.part_rows = pl.part_rows;
   p.words = pl.words;
   p.mask_shared = t.mask_strides[0] == 0;
@@ -438,8 +455,14 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   if (!(s2 >= 1e-30f)) s2 = 1e-30f;  // scale 0: every score becomes (numerically) zero
   p.scale2 = s2;
   p.idesc_s = instr_desc(c.dtype, t.scale < 0.f);
-  // P V: the second operand is MN-major (bit 16), N = the padded head dimension
-  p.idesc_o = (instr_desc(c.dtype, false) & ~(63u << 17)) | (1u << 16) | ((uint32_t)(pl.d_pad >> 3) << 17);
+  p.idesc_o = instr_desc(c.dtype, false);
+  const uint32_t n_field = 63u << 17;
+  if (pl.decode_rows) {  // N = the rows; in V^T P^T the first operand is MN-major (bit 15)
+    p.idesc_s = (p.idesc_s & ~n_field) | ((uint32_t)(pl.decode_rows >> 3) << 17);
+    p.idesc_o = (p.idesc_o & ~n_field) | (1u << 15) | ((uint32_t)(pl.decode_rows >> 3) << 17);
+  } else {  // P V: the second operand is MN-major (bit 16), N = the padded head dimension
+    p.idesc_o = (p.idesc_o & ~n_field) | (1u << 16) | ((uint32_t)(pl.d_pad >> 3) << 17);
+  }
   p.k_steps = (c.D + 15) / 16;
   CUtensorMap map_k, map_v;
   memset(&map_k, 0, sizeof(map_k));
@@ -461,11 +484,8 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "mask packing launch");
   }
-  if (c.dtype == FCR_F16)
-    return pl.d_pad == 64 ? launch_tree_d<__half, 64>(quant, map_k, map_v, p, pl, stream)
-                          : launch_tree_d<__half, 128>(quant, map_k, map_v, p, pl, stream);
-  return pl.d_pad == 64 ? launch_tree_d<__nv_bfloat16, 64>(quant, map_k, map_v, p, pl, stream)
-                        : launch_tree_d<__nv_bfloat16, 128>(quant, map_k, map_v, p, pl, stream);
+  return c.dtype == FCR_F16 ? launch_tree_d<__half>(pl.d_pad, quant, map_k, map_v, p, pl, stream)
+                            : launch_tree_d<__nv_bfloat16>(pl.d_pad, quant, map_k, map_v, p, pl, stream);
 }
 
 }  // extern "C"

@@ -16,8 +16,7 @@
 // with m a reference that follows the running maximum only when that has grown by more than 2^8: O is then rescaled in
 // tensor memory, otherwise the loop carries no correction.  Two warpgroups take turns, so that the exponentials of one
 // tile run under the products of the other.  With more than 128 rows (PAIR) they are two row tiles over the same keys;
-// with fewer, two runs of keys (every other tile) whose results are merged.  With at most 64 (32) rows the rows lie 2 (4)
-// times in the 128 lanes and each copy folds its half (quarter) of a tile's keys, P being zero elsewhere: no lane idles.
+// with 65 to 128, two runs of keys (every other tile) whose results are merged.  Up to 64 rows treedecode_sm100.cuh takes.
 //
 // The key tiles of all rows of all sequences are one line that the CTAs share equally (plan.h), so ragged lengths cost
 // nothing and a single long sequence uses every SM.  A piece that covers a group's keys only in part leaves its
@@ -75,7 +74,6 @@ struct TreeParams : WaitParams {
   long long sb[2], sh[2], sn[2];
   int B, Hq, Hk, M, N, D, G, rows;  // rows = G * M
   int row_tiles, groups;            // groups = Hk * row_tiles
-  int copies;                       // 1, 2 or 4 copies of the rows in the lanes
   int part_rows;
   int words, mask_shared;
   int index_bits, format, q_vec;
@@ -137,6 +135,62 @@ __device__ __forceinline__ bool non_finite16(uint32_t h) {
   return (h & kExp) == kExp;
 }
 
+// Sixteen codes times 2^(byte - 127), exactly, as eight words of two 16-bit values.  The short forms hold for the
+// scales of ordinary keys and values, the caller says whether all of a warp's are such.  Instructions per four codes: fp16 4
+// (e4m3) or 5 (int8), bf16 10 or 9; the general form takes 11 to 13.
+__device__ __forceinline__ bool tree_short_scale(uint32_t byte) { return byte >= 103u && byte <= 132u; }  // 2^-24 .. 2^5
+template <typename T, int FORMAT>
+__device__ __forceinline__ void tree_convert16(const uint4& codes, uint32_t byte, bool short_scale, uint32_t (&o)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes);
+  const float s = kv_scale(byte);
+  if (short_scale && std::is_same<T, __half>::value) {
+    const __half2 s2 = __float2half2_rn(s);  // 2^-24 is fp16's least subnormal
+    if (FORMAT == FCR_KV_FP8) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const __half2 v = __hmul2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[q >> 1] >> (16 * (q & 1))), __NV_E4M3)), s2);
+        o[q] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    } else {
+      // byte + 128 under the exponent of 1024 is the fp16 value 1152 + code; one multiplication-addition takes 1152 * s away
+      const __half2 off = __hmul2(s2, __float2half2_rn(-1152.f));
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t u = __byte_perm(w[q >> 1] ^ 0x80808080u, 0x64646464u, (q & 1) ? 0x4342 : 0x4140);
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&u), s2, off);
+        o[q] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+    }
+    return;
+  }
+  const float2 s2 = make_float2(s, s);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float2 a, b;
+    if (FORMAT == FCR_KV_FP8) {
+      a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[q], __NV_E4M3)));
+      b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[q] >> 16), __NV_E4M3)));
+      a = __fmul2_rn(a, s2);
+      b = __fmul2_rn(b, s2);
+    } else {
+      const uint32_t u = w[q] ^ 0x80808080u;
+      a = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)));
+      b = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)));
+      if (short_scale) {
+        const float2 off = make_float2(-8388736.f * s, -8388736.f * s);
+        a = __ffma2_rn(a, s2, off);
+        b = __ffma2_rn(b, s2, off);
+      } else {  // the offset times a large scale would pass fp32's range
+        const float2 off = make_float2(-8388736.f, -8388736.f);
+        a = __fmul2_rn(__fadd2_rn(a, off), s2);
+        b = __fmul2_rn(__fadd2_rn(b, off), s2);
+      }
+    }
+    o[2 * q] = pack2(a.x, a.y, T());
+    o[2 * q + 1] = pack2(b.x, b.y, T());
+  }
+}
+
 // The values of a drafted token that the product left out because they are not finite; 0 for a finite one.
 template <typename T, bool QUANT>
 __device__ __forceinline__ float tree_non_finite(const TreeParams& p, int b, int h, int n, int d) {
@@ -150,6 +204,7 @@ __device__ __forceinline__ float tree_non_finite(const TreeParams& p, int b, int
   } else {
     v = to_f32(reinterpret_cast<const T*>(p.cache[1])[at]);
   }
+  v = to_f32(from_f32<T>(v));  // as the product would have had it
   return fabsf(v) < INFINITY ? 0.f : v;
 }
 template <typename T, bool QUANT>
@@ -178,6 +233,230 @@ tree_pack_mask_kernel(const unsigned char* __restrict__ mask, long long stride_b
   const bool on = j < M && mask[b * stride_b + m * stride_m + j] != 0;
   const uint32_t bits = __ballot_sync(0xffffffffu, on);
   if (lane == 0) out[i] = bits;
+}
+
+// ------------------------------------------------------------------ what both kernels share
+// Pieces c0 .. c1 - 1 of row `row` (key n) of a value tile: zeros behind the last drafted token, and in place of what is not
+// finite in a drafted token's values.
+template <typename T, int DPAD>
+__device__ __forceinline__ void tree_clean_values(uint32_t tile, int row, int n, const TreeSegment& s, int c0, int c1, volatile int* bad_flag) {
+  if (n < s.have) return;
+  for (int c = c0; c < c1; ++c) {
+    const uint32_t a = tile + (uint32_t)(c >> 3) * (128u * 128u) + (uint32_t)row * 128u + (((uint32_t)c & 7u) ^ ((uint32_t)row & 7u)) * 16u;
+    if (n >= s.end) {
+      ptx::sts128(a, make_uint4(0u, 0u, 0u, 0u));
+      continue;
+    }
+    uint4 v = ptx::lds128(a);
+    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool lo = non_finite16<T>(e[i] & 0xffffu), hi = non_finite16<T>(e[i] >> 16);
+      if (lo) e[i] &= 0xffff0000u;
+      if (hi) e[i] &= 0xffffu;
+      bad = bad || lo || hi;
+    }
+    if (bad) {
+      ptx::sts128(a, v);
+      *bad_flag = 1;
+    }
+  }
+}
+
+// The rings of key and value tiles in shared memory (swizzled 16-bit tiles of 128 keys) and their barriers.
+struct TreeRing {
+  uint32_t k, v;
+  uint32_t bar_k_full, bar_k_empty, bar_v_full, bar_v_empty;
+};
+
+// No arrival may be outstanding when the CTA retires: wait until the products have given back every slot.
+template <int KS, int VS>
+__device__ __forceinline__ void tree_drain(const TreeParams& p, const TreeRing& r, uint32_t seq, bool ok, volatile int* abort_flag) {
+  for (uint32_t i = 0; ok && i < (KS > VS ? KS : VS) && i < seq; ++i) {
+    const uint32_t last = seq - 1 - i;
+    if (i < KS) ok = WAIT_BEHIND(r.bar_k_empty + 8u * (last % KS), (last / KS) & 1u, ST_TR_WAIT_DRAIN);
+    if (ok && i < VS) ok = WAIT_BEHIND(r.bar_v_empty + 8u * (last % VS), (last / VS) & 1u, ST_TR_WAIT_DRAIN);
+  }
+}
+
+// One warp: the tiles of a 16-bit cache by TMA.
+template <int DPAD, int KS, int VS>
+__device__ __forceinline__ void tree_tma_tiles(const TreeParams& p, const TreeRing& r, const CUtensorMap* tmap_k, const CUtensorMap* tmap_v,
+                                               TreeWalk<TreeLengths> walk, int lane, volatile int* abort_flag) {
+  constexpr uint32_t kTileBytes = 128 * DPAD * 2, kSlabBytes = 128 * 128;
+  uint32_t seq = 0;
+  bool ok = true;
+  TreeSegment seg{};
+  auto load = [&](auto is_v, int t, int h) {
+    constexpr bool kv = decltype(is_v)::value;
+    constexpr uint32_t kSlots = kv ? VS : KS;
+    const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
+    const uint32_t full = (kv ? r.bar_v_full : r.bar_k_full) + 8u * slot;
+    ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+    if (!ok) return;
+    const bool left_out = blockIdx.x == 0 && !kv && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
+    if (lane == 0 && !left_out) {
+      const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes;
+      ptx::mbar_arrive_expect_tx(full, kTileBytes);
+#pragma unroll
+      for (int sl = 0; sl < DPAD / 64; ++sl)
+        ptx::tma_load_4d(dst + sl * kSlabBytes, kv ? tmap_v : tmap_k, full, sl * 64, t * kTreeTile, h, seg.b);
+    }
+    __syncwarp();
+  };
+  while (ok && walk.next(seg)) {
+    const int h = seg.group / p.row_tiles;
+    for (int t = seg.lo; ok && t < seg.hi; ++t) {
+      load(std::false_type{}, t, h);
+      if (!ok) break;
+      load(std::true_type{}, t, h);
+      ++seq;
+    }
+  }
+  tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
+}
+
+// kTreeConvertWarps warps: the tiles of an 8-bit cache, codes times scale in 16 bits.  `tid` counts these warps' threads.
+template <typename T, int DPAD, int KS, int VS>
+__device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, long long n_tiles, int tid,
+                                                   volatile int* abort_flag, volatile int* bad_flag) {
+  constexpr uint32_t kTileBytes = 128 * DPAD * 2, kSlabBytes = 128 * 128;
+  const int lane = tid & 31;
+  uint32_t seq = 0;  // tiles so far
+  bool ok = true;
+  TreeSegment seg{};
+  constexpr int kPerRow = DPAD / 16;                            // 16-code pieces of a row
+  constexpr int kRows = 32 * kTreeConvertWarps / kPerRow;       // rows the warps take at a time
+  constexpr int kPasses = 128 / kRows;
+  const int piece = tid % kPerRow, row0 = tid / kPerRow;
+  const bool on = piece * 16 < p.D;
+  struct Batch {
+    uint4 codes[kPasses];
+    uint32_t scale[kPasses];
+  };
+  // where the tile to load next lies, and what the tile to store next needs of its own
+  int t_load = 0;
+  const unsigned char* src[2];
+  const unsigned char* sc[2];
+  auto advance = [&]() {
+    if (++t_load < seg.hi && t_load > 0) return;
+    if (!walk.next(seg)) return;
+    t_load = seg.lo;
+    const int h = seg.group / p.row_tiles;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      src[kv] = reinterpret_cast<const unsigned char*>(p.cache[kv]) + seg.b * p.cb[kv] + h * p.ch[kv] + piece * 16;
+      sc[kv] = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
+    }
+  };
+  auto load = [&](int kv, Batch& x) {
+    const unsigned char* from = kv ? src[1] : src[0];
+    const unsigned char* from_sc = kv ? sc[1] : sc[0];
+    const long long stride = p.cn[kv], stride_sc = p.sn[kv];
+#pragma unroll
+    for (int k = 0; k < kPasses; ++k) {
+      const int n = t_load * kTreeTile + row0 + k * kRows;
+      x.codes[k] = make_uint4(0u, 0u, 0u, 0u);
+      x.scale[k] = 127u;
+      if (n < seg.end && on) {
+        x.codes[k] = *reinterpret_cast<const uint4*>(from + n * stride);
+        x.scale[k] = from_sc[n * stride_sc];
+      }
+    }
+  };
+  auto store = [&](int kv, Batch& x, int drafted) {  // drafted: the tile's first row that is a drafted token's
+    const uint32_t kSlots = kv ? VS : KS;
+    const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
+    ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+    if (!ok) return;
+    const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes;
+    bool short_scale = true;
+#pragma unroll
+    for (int k = 0; k < kPasses; ++k) short_scale = short_scale && tree_short_scale(x.scale[k]);
+    short_scale = __all_sync(0xffffffffu, short_scale);
+    const bool check = kv == 1 && drafted < kTreeTile;
+    auto convert = [&](auto format) {
+#pragma unroll
+      for (int k = 0; k < kPasses; ++k) {
+        const int row = row0 + k * kRows;
+        uint32_t o[8];
+        tree_convert16<T, decltype(format)::value>(x.codes[k], x.scale[k], short_scale, o);
+        if (check && row >= drafted) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (non_finite16<T>(o[e] & 0xffffu) || non_finite16<T>(o[e] >> 16)) {
+              if (non_finite16<T>(o[e] & 0xffffu)) o[e] &= 0xffff0000u;
+              if (non_finite16<T>(o[e] >> 16)) o[e] &= 0xffffu;
+              *bad_flag = 1;
+            }
+          }
+        }
+        // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
+        const uint32_t at_row = dst + (uint32_t)(piece >> 2) * kSlabBytes + (uint32_t)row * 128u;
+        const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
+        const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
+        ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
+        ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
+      }
+    };
+    if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
+    if (lane == 0 && !left_out) ptx::mbar_arrive((kv ? r.bar_v_full : r.bar_k_full) + 8u * slot);
+  };
+  // the codes of the next tile are under way while one is converted
+  Batch kb, vb;
+  t_load = -1;
+  if (n_tiles > 0) {
+    advance();
+    load(0, kb);
+  }
+  for (long long i = 0; ok && i < n_tiles; ++i) {
+    const int drafted = seg.have - t_load * kTreeTile;
+    load(1, vb);
+    store(0, kb, drafted);
+    if (!ok) break;
+    if (i + 1 < n_tiles) {
+      advance();
+      load(0, kb);
+    }
+    store(1, vb, drafted);
+    if (!ok) break;
+    ++seq;
+  }
+  tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
+}
+
+// One warp: this CTA's piece of the line of tiles, as the sequence it begins in, the tile there and its length.
+__device__ __forceinline__ void tree_find_piece(const TreeParams& p, const TreeLengths& lengths, int lane, volatile int* start_b,
+                                                volatile long long* start_off, volatile long long* start_n) {
+  auto tiles_of = [&](int b) { return b < p.B ? tree_tiles(tree_have(lengths(b), p.N), p.M, p.N) : 0; };
+  const int mine0 = tiles_of(lane);
+  long long total = mine0;
+  for (int b = lane + 32; b < p.B; b += 32) total += tiles_of(b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= p.groups;
+  const int ctas = tree_ctas(total, gridDim.x), c = min((int)blockIdx.x, ctas);
+  const long long lo = tree_piece(total, ctas, c), hi = c < ctas ? tree_piece(total, ctas, c + 1) : lo;
+  long long before = 0;
+  for (int b0 = 0; b0 < p.B && before <= lo; b0 += 32) {
+    const long long mine = (long long)(b0 == 0 ? mine0 : tiles_of(b0 + lane)) * p.groups;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (mine > 0 && before + incl - mine <= lo && lo < before + incl) {
+      *start_b = b0 + lane;
+      *start_off = lo - (before + incl - mine);
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) *start_n = hi - lo;
 }
 
 template <typename T, int DPAD, bool PAIR, bool QUANT>
@@ -249,32 +528,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if (blockIdx.x == 0 && threadIdx.x < 4) p.status[threadIdx.x] = 0;
   const TreeLengths lengths{p.lengths, p.index_bits};
   if (warp == kTreeQWarp) {
-    // this CTA's piece of the line of tiles: the total, then the sequence in which the piece begins
-    long long total = 0;
-    for (int b = lane; b < p.B; b += 32) total += tree_tiles(tree_have(lengths(b), p.N), p.M, p.N);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= p.groups;
-    const int ctas = tree_ctas(total, gridDim.x), c = min((int)blockIdx.x, ctas);
-    const long long lo = tree_piece(total, ctas, c), hi = c < ctas ? tree_piece(total, ctas, c + 1) : lo;
-    long long before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-      const int b = b0 + lane;
-      const long long mine = b < p.B ? (long long)tree_tiles(tree_have(lengths(b), p.N), p.M, p.N) * p.groups : 0;
-      long long incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      if (mine > 0 && before + incl - mine <= lo && lo < before + incl) {
-        *start_b = b;
-        *start_off = lo - (before + incl - mine);
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
-      if (before > lo) break;
-    }
-    if (lane == 0) *start_n = hi - lo;
+    tree_find_piece(p, lengths, lane, start_b, start_off, start_n);
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
@@ -288,7 +542,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if (warp >= kTreeQWarp && warp < kTreeQWarp + kTreeQWarps) {
     // ----------------------------------------------------- queries of the next segment
     const int tid = threadIdx.x - 32 * kTreeQWarp;
-    const int rows_here = PAIR ? 256 : 128 / p.copies;
+    constexpr int kRowsHere = PAIR ? 256 : 128;
     uint32_t seq = 0;
     while (walk.next(seg)) {
       const uint32_t buf = seq % L::kQBuffers, ph = (seq / L::kQBuffers) & 1u;
@@ -299,7 +553,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const uint32_t dst0 = base + L::off_q + buf * L::kQBytes;
       constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
       constexpr int kAhead = 8;
-      const int pieces = rows_here * kChunks;
+      constexpr int pieces = kRowsHere * kChunks;
       for (int i0 = tid; i0 < pieces; i0 += 32 * kTreeQWarps * kAhead) {
         uint4 v[kAhead];
 #pragma unroll
@@ -324,11 +578,8 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           const int i = i0 + u * 32 * kTreeQWarps;
           if (i < pieces) {
             const int row = i / kChunks, c = i % kChunks;
-            for (int k = 0; k < (PAIR ? 1 : p.copies); ++k) {
-              const int at = row + k * rows_here;
-              const uint32_t tile = dst0 + (uint32_t)(at >> 7) * L::kTileBytes, in = (uint32_t)(at & 127);
-              ptx::sts128(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u, v[u]);
-            }
+            const uint32_t tile = dst0 + (uint32_t)(row >> 7) * L::kTileBytes, in = (uint32_t)(row & 127);
+            ptx::sts128(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u, v[u]);
           }
         }
       }
@@ -420,155 +671,17 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   } else if (warp >= kTreeLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    uint32_t seq = 0;  // tiles so far
-    bool ok = true;
-    if constexpr (!QUANT) {
-      auto load = [&](auto is_v, int t) {
-        constexpr int kv = decltype(is_v)::value;
-        constexpr uint32_t kSlots = kv ? VS : KS;
-        const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
-        const uint32_t full = kv ? bar_v_full(slot) : bar_k_full(slot);
-        ok = WAIT_BEHIND(kv ? bar_v_empty(slot) : bar_k_empty(slot), ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
-        if (!ok) return;
-        const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
-        if (lane == 0 && !left_out) {
-          const uint32_t dst = base + (kv ? L::off_v : L::off_k) + slot * L::kTileBytes;
-          ptx::mbar_arrive_expect_tx(full, L::kTileBytes);
-#pragma unroll
-          for (int sl = 0; sl < DPAD / 64; ++sl)
-            ptx::tma_load_4d(dst + sl * L::kSlabBytes, kv ? &tmap_v : &tmap_k, full, sl * 64, t * kTreeTile, seg.group / p.row_tiles, seg.b);
-        }
-        __syncwarp();
-      };
-      while (ok && walk.next(seg)) {
-        for (int t = seg.lo; t < seg.hi; ++t) {
-          load(std::integral_constant<int, 0>{}, t);
-          if (!ok) break;
-          load(std::integral_constant<int, 1>{}, t);
-          if (!ok) break;
-          ++seq;
-        }
-      }
-    } else {
-      constexpr int kPerRow = DPAD / 16;                            // 16-code pieces of a row
-      constexpr int kRows = 32 * kTreeConvertWarps / kPerRow;       // rows the warps take at a time
-      constexpr int kPasses = 128 / kRows;
-      const int tid = threadIdx.x - 32 * kTreeLoadWarp;
-      const int piece = tid % kPerRow, row0 = tid / kPerRow;
-      const bool on = piece * 16 < p.D;
-      struct Batch {
-        uint4 codes[kPasses];
-        uint32_t scale[kPasses];
-      };
-      // where the tile to load next lies, and what the tile to store next needs of its own
-      int t_load = 0;
-      const unsigned char* src[2];
-      const unsigned char* sc[2];
-      auto advance = [&]() {
-        if (++t_load < seg.hi && t_load > 0) return;
-        if (!walk.next(seg)) return;
-        t_load = seg.lo;
-        const int h = seg.group / p.row_tiles;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          src[kv] = reinterpret_cast<const unsigned char*>(p.cache[kv]) + seg.b * p.cb[kv] + h * p.ch[kv] + piece * 16;
-          sc[kv] = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
-        }
-      };
-      auto load = [&](auto is_v, Batch& x) {
-        constexpr int kv = decltype(is_v)::value;
-#pragma unroll
-        for (int k = 0; k < kPasses; ++k) {
-          const int n = t_load * kTreeTile + row0 + k * kRows;
-          x.codes[k] = make_uint4(0u, 0u, 0u, 0u);
-          x.scale[k] = 127u;
-          if (n < seg.end && on) {
-            x.codes[k] = *reinterpret_cast<const uint4*>(src[kv] + n * p.cn[kv]);
-            x.scale[k] = sc[kv][n * p.sn[kv]];
-          }
-        }
-      };
-      auto store = [&](auto is_v, Batch& x, int drafted) {  // drafted: the tile's first row that is a drafted token's
-        constexpr int kv = decltype(is_v)::value;
-        constexpr uint32_t kSlots = kv ? VS : KS;
-        const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
-        ok = WAIT_BEHIND(kv ? bar_v_empty(slot) : bar_k_empty(slot), ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
-        if (!ok) return;
-        const uint32_t dst = base + (kv ? L::off_v : L::off_k) + slot * L::kTileBytes;
-#pragma unroll
-        for (int k = 0; k < kPasses; ++k) {
-          const int row = row0 + k * kRows;
-          const float scale = kv_scale(x.scale[k]);
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&x.codes[k]);
-          uint32_t o[8];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float v[4];
-            if (p.format == FCR_KV_FP8) unpack_codes4<FCR_KV_FP8>(w[q], v); else unpack_codes4<FCR_KV_INT8>(w[q], v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= scale;
-            if (kv == 1 && row >= drafted) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (!(fabsf(v[e]) < INFINITY)) {
-                  v[e] = 0.f;
-                  *bad_flag = 1;
-                }
-              }
-            }
-            o[2 * q] = pack2(v[0], v[1], T());
-            o[2 * q + 1] = pack2(v[2], v[3], T());
-          }
-          // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
-          const uint32_t at_row = dst + (uint32_t)(piece >> 2) * L::kSlabBytes + (uint32_t)row * 128u;
-          const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
-          const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
-          ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
-          ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
-        }
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
-        if (lane == 0 && !left_out) ptx::mbar_arrive(kv ? bar_v_full(slot) : bar_k_full(slot));
-      };
-      // the codes of the next tile are under way while one is converted
-      Batch kb, vb;
-      const std::integral_constant<int, 0> is_k{};
-      const std::integral_constant<int, 1> is_v{};
-      t_load = -1;
-      if (n_tiles > 0) {
-        advance();
-        load(is_k, kb);
-      }
-      for (long long i = 0; ok && i < n_tiles; ++i) {
-        const int drafted = seg.have - t_load * kTreeTile;
-        load(is_v, vb);
-        store(is_k, kb, drafted);
-        if (!ok) break;
-        if (i + 1 < n_tiles) {
-          advance();
-          load(is_k, kb);
-        }
-        store(is_v, vb, drafted);
-        if (!ok) break;
-        ++seq;
-      }
-    }
-    // no arrival may be outstanding when the CTA retires: wait until the products have given back every slot
-    for (uint32_t i = 0; ok && i < KS && i < seq; ++i) {
-      const uint32_t last = seq - 1 - i;
-      ok = WAIT_BEHIND(bar_k_empty(last % KS), (last / KS) & 1u, ST_TR_WAIT_DRAIN);
-      if (ok && i < VS) ok = WAIT_BEHIND(bar_v_empty(last % VS), (last / VS) & 1u, ST_TR_WAIT_DRAIN);
-    }
+    const TreeRing ring{base + L::off_k, base + L::off_v, bar_k_full(0), bar_k_empty(0), bar_v_full(0), bar_v_empty(0)};
+    if constexpr (QUANT)
+      tree_convert_tiles<T, DPAD, KS, VS>(p, ring, walk, n_tiles, threadIdx.x - 32 * kTreeLoadWarp, abort_flag, bad_flag);
+    else
+      tree_tma_tiles<DPAD, KS, VS>(p, ring, &tmap_k, &tmap_v, walk, lane, abort_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int w = warp >> 2;
     const int lane_row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem_base + lanes + 2 * DPAD + w * 128, o_addr = tmem_base + lanes + w * DPAD;
-    const int rows_here = PAIR ? 128 : 128 / p.copies;
-    const int copy = (warp & 3) * 32 / rows_here, local = lane_row - copy * rows_here;  // copy: the same for a warp
-    const int c_lo = PAIR ? 0 : copy * (4 / p.copies), c_hi = PAIR ? 4 : c_lo + 4 / p.copies;
     uint32_t tile_seq = 0;   // tiles of this CTA so far
     uint32_t s_use = 0, o_use = 0, merge_use = 0, q_seq = 0;
     bool ok = true;
@@ -581,7 +694,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     };
     while (ok && walk.next(seg)) {
       const int kh = seg.group / p.row_tiles;
-      const int row = (seg.group - kh * p.row_tiles) * 256 + (PAIR ? w * 128 : 0) + local;  // of the G * M
+      const int row = (seg.group - kh * p.row_tiles) * 256 + (PAIR ? w * 128 : 0) + lane_row;  // of the G * M
       const bool real = row < p.rows;
       const int m = real ? row % p.M : 0;
       const uint32_t* words = p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + m) * p.words : nullptr;
@@ -596,7 +709,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         const bool edge = (t + 1) * kTreeTile > seg.have;
         uint32_t ra[32];
         float top = -INFINITY;
-        for (int c = c_lo; c < c_hi; ++c) {
+        for (int c = 0; c < 4; ++c) {
           ptx::tmem_ld<32>(s_addr + 32 * c, ra);
           ptx::tmem_ld_wait<32>(ra);
           if (edge) {
@@ -634,37 +747,32 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         float2 s01 = make_float2(0.f, 0.f), s23 = make_float2(0.f, 0.f);
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
-          if (c >= c_lo && c < c_hi) {
-            ptx::tmem_ld<32>(s_addr + 32 * c, ra);
-            ptx::tmem_ld_wait<32>(ra);
-            uint32_t bits = 0xffffffffu;
-            if (edge) bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+          ptx::tmem_ld<32>(s_addr + 32 * c, ra);
+          ptx::tmem_ld_wait<32>(ra);
+          uint32_t bits = 0xffffffffu;
+          if (edge) bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float2 a = __ffma2_rn(make_float2(__uint_as_float(ra[e]), __uint_as_float(ra[e + 1])), make_float2(p.scale2, p.scale2),
-                                    make_float2(nm, nm));
-              float2 b = __ffma2_rn(make_float2(__uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3])), make_float2(p.scale2, p.scale2),
-                                    make_float2(nm, nm));
-              a.x = ptx::ex2(a.x);
-              a.y = ptx::ex2(a.y);
-              b.x = ptx::ex2(b.x);
-              b.y = ptx::ex2(b.y);
-              if (edge) {
-                a.x = (bits >> e) & 1u ? a.x : 0.f;
-                a.y = (bits >> (e + 1)) & 1u ? a.y : 0.f;
-                b.x = (bits >> (e + 2)) & 1u ? b.x : 0.f;
-                b.y = (bits >> (e + 3)) & 1u ? b.y : 0.f;
-              }
-              s01 = __fadd2_rn(s01, a);
-              s23 = __fadd2_rn(s23, b);
-              pk[e / 2] = pack2(a.x, a.y, T());
-              pk[e / 2 + 1] = pack2(b.x, b.y, T());
+          for (int e = 0; e < 32; e += 4) {
+            float2 a = __ffma2_rn(make_float2(__uint_as_float(ra[e]), __uint_as_float(ra[e + 1])), make_float2(p.scale2, p.scale2),
+                                  make_float2(nm, nm));
+            float2 b = __ffma2_rn(make_float2(__uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3])), make_float2(p.scale2, p.scale2),
+                                  make_float2(nm, nm));
+            a.x = ptx::ex2(a.x);
+            a.y = ptx::ex2(a.y);
+            b.x = ptx::ex2(b.x);
+            b.y = ptx::ex2(b.y);
+            if (edge) {
+              a.x = (bits >> e) & 1u ? a.x : 0.f;
+              a.y = (bits >> (e + 1)) & 1u ? a.y : 0.f;
+              b.x = (bits >> (e + 2)) & 1u ? b.x : 0.f;
+              b.y = (bits >> (e + 3)) & 1u ? b.y : 0.f;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+            s01 = __fadd2_rn(s01, a);
+            s23 = __fadd2_rn(s23, b);
+            pk[e / 2] = pack2(a.x, a.y, T());
+            pk[e / 2 + 1] = pack2(b.x, b.y, T());
           }
-          // P chunk c covers columns 16 c .. 16 c + 15: scores that this thread has read, or does not need
+          // P chunk c covers columns 16 c .. 16 c + 15: scores that this thread has read
           ptx::tmem_st16(s_addr + 16 * c, pk);
         }
         l += (s01.x + s01.y) + (s23.x + s23.y);
@@ -675,36 +783,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           const uint32_t slot = tile_seq % VS;
           ok = WAIT(bar_v_full(slot), (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
           if (!ok) break;
-          const int key = t * kTreeTile + lane_row;
-          if (key >= seg.have) {
-            constexpr int kHalf = DPAD / 16;  // PAIR: each warpgroup takes half of the 16-byte pieces
-            for (int c = PAIR ? w * kHalf : 0; c < (PAIR ? (w + 1) * kHalf : 2 * kHalf); ++c) {
-              const uint32_t a = base + L::off_v + slot * L::kTileBytes + (uint32_t)(c >> 3) * L::kSlabBytes + (uint32_t)lane_row * 128u +
-                                 (((uint32_t)c & 7u) ^ ((uint32_t)lane_row & 7u)) * 16u;
-              if (key >= seg.end) {
-                ptx::sts128(a, make_uint4(0u, 0u, 0u, 0u));
-              } else {
-                uint4 v = ptx::lds128(a);
-                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-                bool bad = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if (non_finite16<T>(e[i] & 0xffffu)) {
-                    e[i] &= 0xffff0000u;
-                    bad = true;
-                  }
-                  if (non_finite16<T>(e[i] >> 16)) {
-                    e[i] &= 0xffffu;
-                    bad = true;
-                  }
-                }
-                if (bad) {
-                  ptx::sts128(a, v);
-                  *bad_flag = 1;
-                }
-              }
-            }
-          }
+          // (PAIR: each warpgroup takes half of the 16-byte pieces)
+          constexpr int kPieces = PAIR ? DPAD / 16 : DPAD / 8;
+          tree_clean_values<T, DPAD>(base + L::off_v + slot * L::kTileBytes, lane_row, t * kTreeTile + lane_row, seg, PAIR ? w * kPieces : 0,
+                                     PAIR ? (w + 1) * kPieces : kPieces, bad_flag);
           ptx::fence_proxy_async_smem();
           if (PAIR && !sync_all()) break;  // both warpgroups' halves are done before either's product
         }
@@ -725,7 +807,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const size_t out_row0 = (size_t)(seg.b * p.Hk + kh) * p.rows;
       if constexpr (PAIR) {
         const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        const int in_part = w * 128 + local;
+        const int in_part = w * 128 + lane_row;
         for (int c = 0; c < DPAD / 32; ++c) {
           uint32_t ra[32];
           ptx::tmem_ld<32>(o_addr + 32 * c, ra);
@@ -762,26 +844,22 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             p.lse[out_row0 + row] = l == 0.f ? -INFINITY : (m_ref + log2f(l)) * 0.69314718055994531f;
         }
       } else {
-        // merge the two warpgroups and the copies of a row: 2 * copies states
+        // merge the two warpgroups: lane_row is the same row in both
         float2* stat = reinterpret_cast<float2*>(smem + L::off_stat);
         float* buf = reinterpret_cast<float*>(smem + L::off_q + (q_seq % L::kQBuffers) * L::kQBytes);
         const int tid = (int)threadIdx.x;
         stat[tid] = make_float2(m_ref, l);
         if (!sync_all()) break;
-        const int states = 2 * p.copies;  // state s of row r: lane (s mod copies) * rows_here + r of warpgroup s / copies
-        float m_all = -INFINITY, l_all = 0.f;
-        for (int s = 0; s < states; ++s) m_all = fmaxf(m_all, stat[(s / p.copies) * 128 + (s % p.copies) * rows_here + local].x);
-        const float m_use = m_all == -INFINITY ? 0.f : m_all;
-        for (int s = 0; s < states; ++s) {
-          const float2 v = stat[(s / p.copies) * 128 + (s % p.copies) * rows_here + local];
-          l_all += v.y * ptx::ex2(v.x - m_use);
-        }
+        const float2 other = stat[tid ^ 128];
+        const float m_all = fmaxf(m_ref, other.x), m_use = m_all == -INFINITY ? 0.f : m_all;
         float f = ptx::ex2(m_ref - m_use);
+        // (in warpgroup order, so that both find the same sum)
+        const float a0 = l * f, a1 = other.y * ptx::ex2(other.x - m_use), l_all = w == 0 ? a0 + a1 : a1 + a0;
         if (whole) f *= l_all == 0.f ? 0.f : 1.f / l_all;
         const bool none = mine == 0 || l == 0.f;  // nothing summed here: the accumulator may hold anything
-        if (w == 0 && copy == 0 && real) {
+        if (w == 0 && real) {
           if (!whole)
-            p.part_ml[part + local] = make_float2(m_all, l_all);
+            p.part_ml[part + lane_row] = make_float2(m_all, l_all);
           else if (p.lse)
             p.lse[out_row0 + row] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * 0.69314718055994531f;
         }
@@ -800,17 +878,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             dst[e ^ (tid & 7)] = v;  // 16-byte pieces in another order per row: no bank is asked for twice
           }
           if (!sync_all()) break;
-          for (int i = tid; i < rows_here * 8; i += 256) {
+          for (int i = tid; i < 128 * 8; i += 256) {
             const int r = i >> 3, piece = i & 7;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int s = 0; s < states; ++s) {
-              const int at = (s / p.copies) * 128 + (s % p.copies) * rows_here + r;
-              const float4 v = reinterpret_cast<const float4*>(buf)[at * 8 + (piece ^ (at & 7))];
-              sum.x += v.x;
-              sum.y += v.y;
-              sum.z += v.z;
-              sum.w += v.w;
-            }
+            const float4* src = reinterpret_cast<const float4*>(buf) + r * 8 + (piece ^ (r & 7));
+            const float4 v0 = src[0], v1 = src[128 * 8];
+            float4 sum = make_float4(v0.x + v1.x, v0.y + v1.y, v0.z + v1.z, v0.w + v1.w);
             const int d = 32 * c + 4 * piece;
             if (r < p.rows && d < p.D) {
               if (*bad_flag) {
@@ -907,14 +979,44 @@ tree_combine_kernel(const __grid_constant__ TreeParams p, int ctas, int rows_per
   float acc[kVec];
 #pragma unroll
   for (int e = 0; e < kVec; ++e) acc[e] = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const float2 ml = p.part_ml[slot_row(c)];
-    const float f = ptx::ex2(ml.x - m_use);
-    l_all += ml.y * f;
-    if (ml.y != 0.f && lane * kVec < p.D) {
-      const float* o = p.part_o + slot_row(c) * DPAD + lane * kVec;
+  for (int cb = c0; cb <= c1; cb += 32) {
+    // a lane per part for the statistics, then all lanes over the parts' values, several loads under way at a time
+    float f_mine = 0.f, l_mine = 0.f;
+    if (cb + lane <= c1) {
+      const float2 ml = p.part_ml[slot_row(cb + lane)];
+      f_mine = ptx::ex2(ml.x - m_use);
+      l_mine = ml.y;
+    }
+    const int n = min(32, c1 - cb + 1);
+    constexpr int kAhead = 4;
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+      float v[kAhead][kVec];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) acc[e] += o[e] * f;
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = min(i0 + u, n - 1);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[u][e] = 0.f;
+        if (lane * kVec < p.D) {
+          const float* o = p.part_o + slot_row(cb + i) * DPAD + lane * kVec;
+          if constexpr (kVec == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(o);
+            v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
+          } else {
+            const float2 q = *reinterpret_cast<const float2*>(o);
+            v[u][0] = q.x, v[u][1] = q.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = (i0 + u) & 31;
+        const float f = __shfl_sync(0xffffffffu, f_mine, i), l = __shfl_sync(0xffffffffu, l_mine, i);
+        if (i0 + u < n && l != 0.f) {  // a part that saw nothing may hold anything
+          l_all += l * f;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) acc[e] += v[u][e] * f;
+        }
+      }
     }
   }
   const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
