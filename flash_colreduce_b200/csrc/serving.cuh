@@ -101,6 +101,23 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
   return FCR_OK;
 }
 
+// Tensor map over an 8-bit cache's codes: a box is 128 rows of d_pad codes of one head, as they lie; codes beyond D or
+// beyond the capacity read as zero.
+static int make_code_map(CUtensorMap* map, const void* ptr, const fcr_kv_cache& c, const int64_t* strides, int d_pad) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return fail(FCR_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  auto stride = [&](int64_t s) -> cuuint64_t { return s > 0 && s % 16 == 0 ? (cuuint64_t)s : 256u; };  // of a dimension of one: never used
+  cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.N, (cuuint64_t)c.H, (cuuint64_t)c.B};
+  cuuint64_t gstr[3] = {stride(strides[2]), stride(strides[1]), stride(strides[0])};
+  cuuint32_t box[4] = {(cuuint32_t)d_pad, (cuuint32_t)kTreeTile, 1u, 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FCR_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
+  return FCR_OK;
+}
+
 struct HostLengths {
   const int64_t* p;
   FCR_HD long long operator()(int b) const { return (long long)p[b]; }
@@ -161,13 +178,14 @@ static int launch_tree_kernel(void (*kern)(const CUtensorMap, const CUtensorMap,
 template <typename T, int DPAD, bool PAIR, bool QUANT>
 static int launch_tree_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
-  return launch_tree_kernel<T, DPAD>(tree_attention_kernel<T, DPAD, PAIR, QUANT>, TreeSmem<DPAD, PAIR>::kDynamicBytes, tree_threads<QUANT>(),
+  return launch_tree_kernel<T, DPAD>(tree_attention_kernel<T, DPAD, PAIR, QUANT>, TreeSmem<DPAD, PAIR, QUANT>::kDynamicBytes, tree_threads<QUANT>(),
                                      opted_in, map_k, map_v, p, pl, stream);
 }
 template <typename T, int DPAD, int NR, bool QUANT>
 static int launch_tree_keys(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
-  return launch_tree_kernel<T, DPAD>(tree_decode_kernel<T, DPAD, NR, QUANT>, DecodeSmem<DPAD, NR>::kDynamicBytes, decode_threads<QUANT>(), opted_in,
+  return launch_tree_kernel<T, DPAD>(tree_decode_kernel<T, DPAD, NR, QUANT>, DecodeSmem<DPAD, NR, QUANT>::kDynamicBytes, decode_threads<NR, QUANT>(),
+                                     opted_in,
                                      map_k, map_v, p, pl, stream);
 }
 template <typename T, int DPAD, bool QUANT>
@@ -457,9 +475,9 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.idesc_s = instr_desc(c.dtype, t.scale < 0.f);
   p.idesc_o = instr_desc(c.dtype, false);
   const uint32_t n_field = 63u << 17;
-  if (pl.decode_rows) {  // N = the rows; in V^T P^T the first operand is MN-major (bit 15)
+  if (pl.decode_rows) {  // N = the rows; in V^T P^T both operands are MN-major (bits 15 and 16)
     p.idesc_s = (p.idesc_s & ~n_field) | ((uint32_t)(pl.decode_rows >> 3) << 17);
-    p.idesc_o = (p.idesc_o & ~n_field) | (1u << 15) | ((uint32_t)(pl.decode_rows >> 3) << 17);
+    p.idesc_o = (p.idesc_o & ~n_field) | (3u << 15) | ((uint32_t)(pl.decode_rows >> 3) << 17);
   } else {  // P V: the second operand is MN-major (bit 16), N = the padded head dimension
     p.idesc_o = (p.idesc_o & ~n_field) | (1u << 16) | ((uint32_t)(pl.d_pad >> 3) << 17);
   }
@@ -467,7 +485,11 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   CUtensorMap map_k, map_v;
   memset(&map_k, 0, sizeof(map_k));
   memset(&map_v, 0, sizeof(map_v));
-  if (!quant) {
+  if (quant) {
+    rc = make_code_map(&map_k, k_cache, c, c.k_strides, pl.d_pad);
+    if (rc == FCR_OK) rc = make_code_map(&map_v, v_cache, c, c.v_strides, pl.d_pad);
+    if (rc != FCR_OK) return rc;
+  } else {
     rc = make_tensor_map(&map_k, k_cache, c.dtype, c.D, c.N, c.H, c.B, c.k_strides);
     if (rc != FCR_OK) return rc;
     rc = make_tensor_map(&map_v, v_cache, c.dtype, c.D, c.N, c.H, c.B, c.v_strides);

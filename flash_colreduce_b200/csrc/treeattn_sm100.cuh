@@ -39,10 +39,10 @@ constexpr int kTreeSoftmaxWarps = 8;  // two warpgroups
 constexpr int kTreeMmaWarp = 8;
 constexpr int kTreeQWarp = 9;         // two warps that bring the queries
 constexpr int kTreeQWarps = 2;
-constexpr int kTreeLoadWarp = 11;     // one TMA warp, or the warps that convert codes
+constexpr int kTreeLoadWarp = 11;     // TMA; for an 8-bit cache then a warp for the scales and those that convert codes
 constexpr int kTreeConvertWarps = 8;
 template <bool QUANT>
-constexpr int tree_threads() { return 32 * (kTreeLoadWarp + (QUANT ? kTreeConvertWarps : 1)); }
+constexpr int tree_threads() { return 32 * (kTreeLoadWarp + 1 + (QUANT ? 1 + kTreeConvertWarps : 0)); }
 
 enum {
   ST_TR_WAIT_Q_EMPTY = 71,
@@ -57,6 +57,10 @@ enum {
   ST_TR_WAIT_MERGE = 80,
   ST_TR_WAIT_V_FULL_SM = 81,
   ST_TR_WAIT_DRAIN = 82,
+  ST_TR_WAIT_C_EMPTY = 83,
+  ST_TR_WAIT_C_FULL = 84,
+  ST_TR_WAIT_SC_EMPTY = 85,
+  ST_TR_WAIT_SC_FULL = 86,
 };
 
 struct TreeParams : WaitParams {
@@ -91,20 +95,24 @@ struct TreeLengths {
   }
 };
 
-template <int DPAD, bool PAIR>
+template <int DPAD, bool PAIR, bool QUANT>
 struct TreeSmem {
   static constexpr int kTileBytes = 128 * DPAD * 2;
   static constexpr int kSlabBytes = 128 * 128;
   static constexpr int kQBuffers = PAIR ? 1 : 2;
   // a query buffer doubles as the space in which the two warpgroups merge: 256 lanes x 32 columns of fp32
   static constexpr int kQBytes = PAIR ? 2 * kTileBytes : 32768;
-  static constexpr int KS = DPAD == 64 ? 5 : 3, VS = DPAD == 64 ? 4 : 2;  // key and value tiles in flight
+  static constexpr int KS = DPAD == 64 ? (QUANT ? 3 : 5) : (QUANT ? 2 : 3);  // key and value tiles in flight
+  static constexpr int VS = DPAD == 64 ? (QUANT ? 3 : 4) : 2;
+  static constexpr int SS = QUANT ? (DPAD == 64 ? 5 : 2) : 0;               // tiles of codes in flight
   static constexpr int off_q = 0;
   static constexpr int off_k = off_q + kQBuffers * kQBytes;
   static constexpr int off_v = off_k + KS * kTileBytes;
-  static constexpr int off_stat = off_v + VS * kTileBytes;  // float2 [256]
-  static constexpr int off_bars = off_stat + 2048;
-  static constexpr int kNumBars = 4 + 2 * KS + 2 * VS + 2 + 2 + 2 + 1;
+  static constexpr int off_codes = off_v + VS * kTileBytes;
+  static constexpr int off_stat = off_codes + SS * 128 * DPAD;  // float2 [256]; PAIR keeps none, scale bytes then lie there
+  static constexpr int off_scales = PAIR ? off_stat : off_stat + 2048;
+  static constexpr int off_bars = off_stat + 2048 + (PAIR || !QUANT ? 0 : 512);
+  static constexpr int kNumBars = 4 + 2 * KS + 2 * VS + 2 + 2 + 2 + 1 + (QUANT ? 2 * SS + 4 : 0);
   static constexpr int off_misc = off_bars + 8 * kNumBars;
   static constexpr int kDynamicBytes = off_misc + 48;
   static_assert(kDynamicBytes <= 232448, "exceeds the 227 KB shared memory of an sm_100 CTA");
@@ -264,10 +272,14 @@ __device__ __forceinline__ void tree_clean_values(uint32_t tile, int row, int n,
   }
 }
 
-// The rings of key and value tiles in shared memory (swizzled 16-bit tiles of 128 keys) and their barriers.
+// The rings of key and value tiles in shared memory (swizzled 16-bit tiles of 128 keys) and their barriers; for an 8-bit cache
+// also the rings of codes (key and value tiles in turn, rows of DPAD bytes) and of scale bytes (two batches of two tiles: 128
+// keys, then 128 values, per tile) that the tiles are made from.
 struct TreeRing {
   uint32_t k, v;
   uint32_t bar_k_full, bar_k_empty, bar_v_full, bar_v_empty;
+  uint32_t codes, scales;
+  uint32_t bar_c_full, bar_c_empty, bar_sc_full, bar_sc_empty;
 };
 
 // No arrival may be outstanding when the CTA retires: wait until the products have given back every slot.
@@ -317,116 +329,179 @@ __device__ __forceinline__ void tree_tma_tiles(const TreeParams& p, const TreeRi
   tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
 }
 
-// kTreeConvertWarps warps: the tiles of an 8-bit cache, codes times scale in 16 bits.  `tid` counts these warps' threads.
-template <typename T, int DPAD, int KS, int VS>
-__device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, long long n_tiles, int tid,
-                                                   volatile int* abort_flag, volatile int* bad_flag) {
-  constexpr uint32_t kTileBytes = 128 * DPAD * 2, kSlabBytes = 128 * 128;
-  const int lane = tid & 31;
-  uint32_t seq = 0;  // tiles so far
+// An 8-bit cache takes three roles.  One warp: the codes by TMA, SS tiles of them under way.
+template <int DPAD, int SS>
+__device__ __forceinline__ void tree_tma_codes(const TreeParams& p, const TreeRing& r, const CUtensorMap* tmap_k, const CUtensorMap* tmap_v,
+                                               TreeWalk<TreeLengths> walk, int lane, volatile int* abort_flag) {
+  uint32_t seq = 0;
   bool ok = true;
   TreeSegment seg{};
+  while (ok && walk.next(seg)) {
+    const int h = seg.group / p.row_tiles;
+    for (int t2 = 2 * seg.lo; t2 < 2 * seg.hi; ++t2, ++seq) {
+      const uint32_t slot = seq % SS, full = r.bar_c_full + 8u * slot;
+      ok = WAIT_BEHIND(r.bar_c_empty + 8u * slot, ((seq / SS) & 1u) ^ 1u, ST_TR_WAIT_C_EMPTY);
+      if (!ok) break;
+      const bool left_out = blockIdx.x == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
+      if (lane == 0 && !left_out) {
+        ptx::mbar_arrive_expect_tx(full, 128 * DPAD);
+        ptx::tma_load_4d(r.codes + slot * (128 * DPAD), (t2 & 1) ? tmap_v : tmap_k, full, 0, (t2 >> 1) * kTreeTile, h, seg.b);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// One warp: the scale bytes, two tiles at a time so that their loads' latencies overlap.  They may lie anywhere, at any
+// stride, so plain loads bring them.
+__device__ __forceinline__ void tree_load_scales(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int lane,
+                                                 volatile int* abort_flag) {
+  TreeSegment seg{};
+  int t = 0;
+  bool more = walk.next(seg);
+  if (more) t = seg.lo;
+  for (uint32_t batch = 0; more; ++batch) {
+    uint32_t byte[2][8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int h = more ? seg.group / p.row_tiles : 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const unsigned char* src = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const long long n = t * kTreeTile + k * 32 + lane;
+          byte[i][4 * kv + k] = more && n < seg.end ? src[n * p.sn[kv]] : 127u;
+        }
+      }
+      if (more && ++t == seg.hi) {
+        more = walk.next(seg);
+        if (more) t = seg.lo;
+      }
+    }
+    const uint32_t buf = batch & 1u;
+    if (!WAIT_BEHIND(r.bar_sc_empty + 8u * buf, ((batch >> 1) & 1u) ^ 1u, ST_TR_WAIT_SC_EMPTY)) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ptx::sts8(r.scales + buf * 512u + i * 256u + k * 32u + lane, byte[i][k]);
+    }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(r.bar_sc_full + 8u * buf);
+  }
+}
+
+// kTreeConvertWarps warps: codes times scale in 16 bits.  `tid` counts these warps' threads.  (Loading the codes straight
+// into registers was built first: a warp's waits for a load include the younger loads behind it, so that there was
+// never more than one tile under way, and a pair of tiles took 5800 cycles.)
+template <typename T, int DPAD, int KS, int VS, int SS>
+__device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int tid,
+                                                   volatile int* abort_flag, volatile int* bad_flag) {
+  constexpr uint32_t kTileBytes = 128 * DPAD * 2, kSlabBytes = 128 * 128;
   constexpr int kPerRow = DPAD / 16;                            // 16-code pieces of a row
   constexpr int kRows = 32 * kTreeConvertWarps / kPerRow;       // rows the warps take at a time
   constexpr int kPasses = 128 / kRows;
+  const int lane = tid & 31;
   const int piece = tid % kPerRow, row0 = tid / kPerRow;
-  const bool on = piece * 16 < p.D;
-  struct Batch {
-    uint4 codes[kPasses];
-    uint32_t scale[kPasses];
-  };
-  // where the tile to load next lies, and what the tile to store next needs of its own
-  int t_load = 0;
-  const unsigned char* src[2];
-  const unsigned char* sc[2];
-  auto advance = [&]() {
-    if (++t_load < seg.hi && t_load > 0) return;
-    if (!walk.next(seg)) return;
-    t_load = seg.lo;
-    const int h = seg.group / p.row_tiles;
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-      src[kv] = reinterpret_cast<const unsigned char*>(p.cache[kv]) + seg.b * p.cb[kv] + h * p.ch[kv] + piece * 16;
-      sc[kv] = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
-    }
-  };
-  auto load = [&](int kv, Batch& x) {
-    const unsigned char* from = kv ? src[1] : src[0];
-    const unsigned char* from_sc = kv ? sc[1] : sc[0];
-    const long long stride = p.cn[kv], stride_sc = p.sn[kv];
-#pragma unroll
-    for (int k = 0; k < kPasses; ++k) {
-      const int n = t_load * kTreeTile + row0 + k * kRows;
-      x.codes[k] = make_uint4(0u, 0u, 0u, 0u);
-      x.scale[k] = 127u;
-      if (n < seg.end && on) {
-        x.codes[k] = *reinterpret_cast<const uint4*>(from + n * stride);
-        x.scale[k] = from_sc[n * stride_sc];
+  uint32_t seq = 0;  // tiles so far
+  bool ok = true;
+  TreeSegment seg{};
+  while (ok && walk.next(seg)) {
+    for (int t = seg.lo; ok && t < seg.hi; ++t) {
+      // rows from `drafted` on are drafted tokens', rows from `end` on nobody's
+      const int drafted = seg.have - t * kTreeTile, end = seg.end - t * kTreeTile;
+      if ((seq & 1u) == 0) {
+        ok = WAIT(r.bar_sc_full + 8u * ((seq >> 1) & 1u), (seq >> 2) & 1u, ST_TR_WAIT_SC_FULL);
+        if (!ok) break;
       }
-    }
-  };
-  auto store = [&](int kv, Batch& x, int drafted) {  // drafted: the tile's first row that is a drafted token's
-    const uint32_t kSlots = kv ? VS : KS;
-    const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
-    ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
-    if (!ok) return;
-    const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes;
-    bool short_scale = true;
+      const uint32_t scales = r.scales + (seq & 3u) * 256u;
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t from = 2u * seq + kv, c_slot = from % SS;
+        ok = WAIT(r.bar_c_full + 8u * c_slot, (from / SS) & 1u, ST_TR_WAIT_C_FULL);
+        if (!ok) break;
+        uint4 codes[kPasses];
+        uint32_t scale[kPasses];
+        bool short_scale = true;
 #pragma unroll
-    for (int k = 0; k < kPasses; ++k) short_scale = short_scale && tree_short_scale(x.scale[k]);
-    short_scale = __all_sync(0xffffffffu, short_scale);
-    const bool check = kv == 1 && drafted < kTreeTile;
-    auto convert = [&](auto format) {
-#pragma unroll
-      for (int k = 0; k < kPasses; ++k) {
-        const int row = row0 + k * kRows;
-        uint32_t o[8];
-        tree_convert16<T, decltype(format)::value>(x.codes[k], x.scale[k], short_scale, o);
-        if (check && row >= drafted) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (non_finite16<T>(o[e] & 0xffffu) || non_finite16<T>(o[e] >> 16)) {
-              if (non_finite16<T>(o[e] & 0xffffu)) o[e] &= 0xffff0000u;
-              if (non_finite16<T>(o[e] >> 16)) o[e] &= 0xffffu;
-              *bad_flag = 1;
-            }
-          }
+        for (int k = 0; k < kPasses; ++k) {
+          const int row = row0 + k * kRows;
+          codes[k] = ptx::lds128(r.codes + c_slot * (128 * DPAD) + row * DPAD + piece * 16);
+          scale[k] = ptx::lds8(scales + kv * 128u + row);
+          if (row >= end) codes[k] = make_uint4(0u, 0u, 0u, 0u);
+          short_scale = short_scale && tree_short_scale(scale[k]);
         }
-        // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
-        const uint32_t at_row = dst + (uint32_t)(piece >> 2) * kSlabBytes + (uint32_t)row * 128u;
-        const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
-        const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
-        ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
-        ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
+        short_scale = __all_sync(0xffffffffu, short_scale);  // (every lane has its codes: the slot may be filled again)
+        if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);
+        const uint32_t slots = kv ? VS : KS, slot = seq % slots;
+        ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ((seq / slots) & 1u) ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+        if (!ok) break;
+        const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes;
+        const bool check = kv == 1 && drafted < kTreeTile;
+        auto convert = [&](auto format) {
+#pragma unroll
+          for (int k = 0; k < kPasses; ++k) {
+            const int row = row0 + k * kRows;
+            uint32_t o[8];
+            tree_convert16<T, decltype(format)::value>(codes[k], scale[k], short_scale, o);
+            if (check && row >= drafted) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const bool lo = non_finite16<T>(o[e] & 0xffffu), hi = non_finite16<T>(o[e] >> 16);
+                if (lo) o[e] &= 0xffff0000u;
+                if (hi) o[e] &= 0xffffu;
+                if (lo || hi) *bad_flag = 1;
+              }
+            }
+            // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
+            const uint32_t at_row = dst + (uint32_t)(piece >> 2) * kSlabBytes + (uint32_t)row * 128u;
+            const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
+            const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
+            ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
+            ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
+          }
+        };
+        if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive((kv ? r.bar_v_full : r.bar_k_full) + 8u * slot);
+          if (kv == 1 && (seq & 1u)) ptx::mbar_arrive(r.bar_sc_empty + 8u * ((seq >> 1) & 1u));
+        }
       }
-    };
-    if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
-    ptx::fence_proxy_async_smem();
-    __syncwarp();
-    const bool left_out = blockIdx.x == 0 && kv == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
-    if (lane == 0 && !left_out) ptx::mbar_arrive((kv ? r.bar_v_full : r.bar_k_full) + 8u * slot);
-  };
-  // the codes of the next tile are under way while one is converted
-  Batch kb, vb;
-  t_load = -1;
-  if (n_tiles > 0) {
-    advance();
-    load(0, kb);
-  }
-  for (long long i = 0; ok && i < n_tiles; ++i) {
-    const int drafted = seg.have - t_load * kTreeTile;
-    load(1, vb);
-    store(0, kb, drafted);
-    if (!ok) break;
-    if (i + 1 < n_tiles) {
-      advance();
-      load(0, kb);
+      if (ok) ++seq;
     }
-    store(1, vb, drafted);
-    if (!ok) break;
-    ++seq;
   }
   tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
+}
+
+template <int SS>
+__device__ __forceinline__ void tree_init_code_bars(const TreeRing& r) {
+  for (int i = 0; i < SS; ++i) {
+    ptx::mbar_init(r.bar_c_full + 8u * i, 1);
+    ptx::mbar_init(r.bar_c_empty + 8u * i, kTreeConvertWarps);
+  }
+  for (int i = 0; i < 2; ++i) {
+    ptx::mbar_init(r.bar_sc_full + 8u * i, 1);
+    ptx::mbar_init(r.bar_sc_empty + 8u * i, kTreeConvertWarps);
+  }
+}
+
+// What the load warps do; `role` counts them.
+template <typename T, int DPAD, int KS, int VS, int SS, bool QUANT>
+__device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeRing& ring, const CUtensorMap* tmap_k, const CUtensorMap* tmap_v,
+                                                const TreeWalk<TreeLengths>& walk, int role, int lane, volatile int* abort_flag,
+                                                volatile int* bad_flag) {
+  if constexpr (!QUANT) {
+    tree_tma_tiles<DPAD, KS, VS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
+  } else {
+    if (role == 0)
+      tree_tma_codes<DPAD, SS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
+    else if (role == 1)
+      tree_load_scales(p, ring, walk, lane, abort_flag);
+    else
+      tree_convert_tiles<T, DPAD, KS, VS, SS>(p, ring, walk, 32 * (role - 2) + lane, abort_flag, bad_flag);
+  }
 }
 
 // One warp: this CTA's piece of the line of tiles, as the sequence it begins in, the tile there and its length.
@@ -463,7 +538,7 @@ template <typename T, int DPAD, bool PAIR, bool QUANT>
 __global__ void __launch_bounds__(tree_threads<QUANT>(), 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ TreeParams p) {
-  using L = TreeSmem<DPAD, PAIR>;
+  using L = TreeSmem<DPAD, PAIR, QUANT>;
   constexpr int KS = L::KS, VS = L::VS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = ptx::smem_u32(smem);
@@ -482,6 +557,9 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   auto bar_p = [&](uint32_t w) { return bar0 + 8u * (6 + 2 * KS + 2 * VS + w); };
   auto bar_o = [&](uint32_t w) { return bar0 + 8u * (8 + 2 * KS + 2 * VS + w); };
   const uint32_t bar_merge = bar0 + 8u * (10 + 2 * KS + 2 * VS);
+  const uint32_t bar_c = bar_merge + 8u;
+  const TreeRing ring{base + L::off_k, base + L::off_v, bar_k_full(0), bar_k_empty(0), bar_v_full(0), bar_v_empty(0), base + L::off_codes,
+                      base + L::off_scales, bar_c, bar_c + 8u * L::SS, bar_c + 16u * L::SS, bar_c + 16u * L::SS + 16u};
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::off_misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 4);
   volatile int* bad_flag = reinterpret_cast<volatile int*>(smem + L::off_misc + 8);  // a drafted value was not finite
@@ -511,6 +589,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       ptx::mbar_init(bar_o(w), 1);
     }
     ptx::mbar_init(bar_merge, kTreeSoftmaxWarps);
+    if (QUANT) tree_init_code_bars<L::SS>(ring);
     *abort_flag = 0;
     *bad_flag = 0;
     ptx::fence_mbar_init();
@@ -519,7 +598,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
     ptx::tmem_relinquish();
   }
-  if (!QUANT && warp == kTreeLoadWarp && lane == 0) {
+  if (warp == kTreeLoadWarp && lane == 0) {
     ptx::prefetch_tensormap(&tmap_k);
     ptx::prefetch_tensormap(&tmap_v);
   }
@@ -671,11 +750,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   } else if (warp >= kTreeLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    const TreeRing ring{base + L::off_k, base + L::off_v, bar_k_full(0), bar_k_empty(0), bar_v_full(0), bar_v_empty(0)};
-    if constexpr (QUANT)
-      tree_convert_tiles<T, DPAD, KS, VS>(p, ring, walk, n_tiles, threadIdx.x - 32 * kTreeLoadWarp, abort_flag, bad_flag);
-    else
-      tree_tma_tiles<DPAD, KS, VS>(p, ring, &tmap_k, &tmap_v, walk, lane, abort_flag);
+    tree_load_roles<T, DPAD, KS, VS, L::SS, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kTreeLoadWarp, lane, abort_flag, bad_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int w = warp >> 2;
