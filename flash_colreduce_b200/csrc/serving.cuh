@@ -101,15 +101,15 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
   return FCR_OK;
 }
 
-// Tensor map over an 8-bit cache's codes: a box is 128 rows of d_pad codes of one head, as they lie; codes beyond D or
+// Tensor map over an 8-bit cache's codes: a box is 128 rows of 64 codes of one head, as they lie; codes beyond D or
 // beyond the capacity read as zero.
-static int make_code_map(CUtensorMap* map, const void* ptr, const fcr_kv_cache& c, const int64_t* strides, int d_pad) {
+static int make_code_map(CUtensorMap* map, const void* ptr, const fcr_kv_cache& c, const int64_t* strides) {
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) return fail(FCR_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   auto stride = [&](int64_t s) -> cuuint64_t { return s > 0 && s % 16 == 0 ? (cuuint64_t)s : 256u; };  // of a dimension of one: never used
   cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.N, (cuuint64_t)c.H, (cuuint64_t)c.B};
   cuuint64_t gstr[3] = {stride(strides[2]), stride(strides[1]), stride(strides[0])};
-  cuuint32_t box[4] = {(cuuint32_t)d_pad, (cuuint32_t)kTreeTile, 1u, 1u};
+  cuuint32_t box[4] = {64u, (cuuint32_t)kTreeTile, 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -410,6 +410,9 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   if (rc != FCR_OK) return rc;
   if (reinterpret_cast<uintptr_t>(k_cache) % 16 || reinterpret_cast<uintptr_t>(v_cache) % 16)
     return fail(FCR_ERR_UNSUPPORTED, "cache base address must be 16-byte aligned");
+  const int32_t q_sizes[3] = {c.B, t.Hq, t.M};
+  if (!kv_aligned(q, t.q_strides, q_sizes, 3, 2, 16))
+    return fail(FCR_ERR_UNSUPPORTED, "base address and strides of the queries must be multiples of 16 bytes");
   if (reinterpret_cast<uintptr_t>(out) % 16) return fail(FCR_ERR_UNSUPPORTED, "output must be 16-byte aligned");
   const DeviceInfo* dev = nullptr;
   rc = device_info(&dev, true);
@@ -467,8 +470,6 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.mask_shared = t.mask_strides[0] == 0;
   p.index_bits = t.index_bits;
   p.format = c.format;
-  const int32_t q_sizes[3] = {c.B, t.Hq, t.M};
-  p.q_vec = kv_aligned(q, t.q_strides, q_sizes, 3, 2, 16);
   float s2 = fabsf(t.scale) * 1.4426950408889634f;
   if (!(s2 >= 1e-30f)) s2 = 1e-30f;  // scale 0: every score becomes (numerically) zero
   p.scale2 = s2;
@@ -486,8 +487,8 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   memset(&map_k, 0, sizeof(map_k));
   memset(&map_v, 0, sizeof(map_v));
   if (quant) {
-    rc = make_code_map(&map_k, k_cache, c, c.k_strides, pl.d_pad);
-    if (rc == FCR_OK) rc = make_code_map(&map_v, v_cache, c, c.v_strides, pl.d_pad);
+    rc = make_code_map(&map_k, k_cache, c, c.k_strides);
+    if (rc == FCR_OK) rc = make_code_map(&map_v, v_cache, c, c.v_strides);
     if (rc != FCR_OK) return rc;
   } else {
     rc = make_tensor_map(&map_k, k_cache, c.dtype, c.D, c.N, c.H, c.B, c.k_strides);

@@ -37,12 +37,11 @@ namespace fcr {
 constexpr int kTreeMaxM = 256;
 constexpr int kTreeSoftmaxWarps = 8;  // two warpgroups
 constexpr int kTreeMmaWarp = 8;
-constexpr int kTreeQWarp = 9;         // two warps that bring the queries
-constexpr int kTreeQWarps = 2;
-constexpr int kTreeLoadWarp = 11;     // TMA; for an 8-bit cache then a warp for the scales and those that convert codes
+constexpr int kTreeQWarp = 9;         // two warps that bring the queries; for an 8-bit cache one, and one for its scales
+constexpr int kTreeLoadWarp = 11;     // TMA; for an 8-bit cache then the warps that convert codes
 constexpr int kTreeConvertWarps = 8;
 template <bool QUANT>
-constexpr int tree_threads() { return 32 * (kTreeLoadWarp + 1 + (QUANT ? 1 + kTreeConvertWarps : 0)); }
+constexpr int tree_threads() { return 32 * (kTreeLoadWarp + 1 + (QUANT ? kTreeConvertWarps : 0)); }
 
 enum {
   ST_TR_WAIT_Q_EMPTY = 71,
@@ -80,7 +79,7 @@ struct TreeParams : WaitParams {
   int row_tiles, groups;            // groups = Hk * row_tiles
   int part_rows;
   int words, mask_shared;
-  int index_bits, format, q_vec;
+  int index_bits, format;
   float scale2;                     // |scale| * log2(e)
   uint32_t idesc_s, idesc_o;
   int k_steps;                      // 32-byte steps of a key row that hold data
@@ -143,15 +142,15 @@ __device__ __forceinline__ bool non_finite16(uint32_t h) {
   return (h & kExp) == kExp;
 }
 
-// Sixteen codes times 2^(byte - 127), exactly, as eight words of two 16-bit values.  The short forms hold for the
-// scales of ordinary keys and values, the caller says whether all of a warp's are such.  Instructions per four codes: fp16 4
-// (e4m3) or 5 (int8), bf16 10 or 9; the general form takes 11 to 13.
-__device__ __forceinline__ bool tree_short_scale(uint32_t byte) { return byte >= 103u && byte <= 132u; }  // 2^-24 .. 2^5
+// Sixteen codes times 2^(byte - 127), exactly, as eight words of two 16-bit values.  The short form holds for the scales of
+// ordinary keys and values, 2^-24 .. 2^5; the caller says whether all of a warp's are such.  Instructions per four codes:
+// fp16 4 (e4m3) or 5 (int8), bf16 10 or 9.
+__device__ __forceinline__ bool tree_short_scale(uint32_t byte) { return byte >= 103u && byte <= 132u; }
 template <typename T, int FORMAT>
-__device__ __forceinline__ void tree_convert16(const uint4& codes, uint32_t byte, bool short_scale, uint32_t (&o)[8]) {
+__device__ __forceinline__ void tree_convert16(const uint4& codes, uint32_t byte, uint32_t (&o)[8]) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&codes);
-  const float s = kv_scale(byte);
-  if (short_scale && std::is_same<T, __half>::value) {
+  const float s = __uint_as_float(byte << 23);
+  if (std::is_same<T, __half>::value) {
     const __half2 s2 = __float2half2_rn(s);  // 2^-24 is fp16's least subnormal
     if (FORMAT == FCR_KV_FP8) {
 #pragma unroll
@@ -172,31 +171,42 @@ __device__ __forceinline__ void tree_convert16(const uint4& codes, uint32_t byte
     return;
   }
   const float2 s2 = make_float2(s, s);
+  const float2 off = make_float2(-8388736.f * s, -8388736.f * s);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     float2 a, b;
     if (FORMAT == FCR_KV_FP8) {
-      a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[q], __NV_E4M3)));
-      b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[q] >> 16), __NV_E4M3)));
-      a = __fmul2_rn(a, s2);
-      b = __fmul2_rn(b, s2);
-    } else {
+      a = __fmul2_rn(__half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w[q], __NV_E4M3))), s2);
+      b = __fmul2_rn(__half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[q] >> 16), __NV_E4M3))), s2);
+    } else {  // the same with 2^23 + 128 in fp32
       const uint32_t u = w[q] ^ 0x80808080u;
-      a = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)));
-      b = make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)));
-      if (short_scale) {
-        const float2 off = make_float2(-8388736.f * s, -8388736.f * s);
-        a = __ffma2_rn(a, s2, off);
-        b = __ffma2_rn(b, s2, off);
-      } else {  // the offset times a large scale would pass fp32's range
-        const float2 off = make_float2(-8388736.f, -8388736.f);
-        a = __fmul2_rn(__fadd2_rn(a, off), s2);
-        b = __fmul2_rn(__fadd2_rn(b, off), s2);
-      }
+      a = __ffma2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441))), s2, off);
+      b = __ffma2_rn(make_float2(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)), __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443))), s2, off);
     }
     o[2 * q] = pack2(a.x, a.y, T());
     o[2 * q + 1] = pack2(b.x, b.y, T());
   }
+}
+// Any scale, NaN included.  Out of line, for the instruction cache's sake.
+template <typename T, int FORMAT>
+__device__ __noinline__ uint4 tree_convert8_any(uint2 codes, uint32_t byte) {
+  const float s = kv_scale(byte);
+  float v[8];
+  unpack_codes4<FORMAT>(codes.x, v);
+  unpack_codes4<FORMAT>(codes.y, v + 4);
+  return make_uint4(pack2(v[0] * s, v[1] * s, T()), pack2(v[2] * s, v[3] * s, T()), pack2(v[4] * s, v[5] * s, T()), pack2(v[6] * s, v[7] * s, T()));
+}
+// Zeros in place of what is not finite; whether there was any.
+template <typename T>
+__device__ __forceinline__ bool clean_words(uint32_t* e, int n) {
+  bool bad = false;
+  for (int i = 0; i < n; ++i) {
+    const bool lo = non_finite16<T>(e[i] & 0xffffu), hi = non_finite16<T>(e[i] >> 16);
+    if (lo) e[i] &= 0xffff0000u;
+    if (hi) e[i] &= 0xffffu;
+    bad = bad || lo || hi;
+  }
+  return bad;
 }
 
 // The values of a drafted token that the product left out because they are not finite; 0 for a finite one.
@@ -255,25 +265,17 @@ __device__ __forceinline__ void tree_clean_values(uint32_t tile, int row, int n,
       ptx::sts128(a, make_uint4(0u, 0u, 0u, 0u));
       continue;
     }
-    uint4 v = ptx::lds128(a);
-    uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool lo = non_finite16<T>(e[i] & 0xffffu), hi = non_finite16<T>(e[i] >> 16);
-      if (lo) e[i] &= 0xffff0000u;
-      if (hi) e[i] &= 0xffffu;
-      bad = bad || lo || hi;
-    }
-    if (bad) {
-      ptx::sts128(a, v);
+    uint32_t e[4];
+    *reinterpret_cast<uint4*>(e) = ptx::lds128(a);
+    if (clean_words<T>(e, 4)) {
+      ptx::sts128(a, make_uint4(e[0], e[1], e[2], e[3]));
       *bad_flag = 1;
     }
   }
 }
 
 // The rings of key and value tiles in shared memory (swizzled 16-bit tiles of 128 keys) and their barriers; for an 8-bit cache
-// also the rings of codes (key and value tiles in turn, rows of DPAD bytes) and of scale bytes (two batches of two tiles: 128
+// also the rings of codes (key and value tiles in turn, slabs of 64 bytes by 128 rows) and of scale bytes (two batches of two tiles: 128
 // keys, then 128 values, per tile) that the tiles are made from.
 struct TreeRing {
   uint32_t k, v;
@@ -345,7 +347,9 @@ __device__ __forceinline__ void tree_tma_codes(const TreeParams& p, const TreeRi
       const bool left_out = blockIdx.x == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
       if (lane == 0 && !left_out) {
         ptx::mbar_arrive_expect_tx(full, 128 * DPAD);
-        ptx::tma_load_4d(r.codes + slot * (128 * DPAD), (t2 & 1) ? tmap_v : tmap_k, full, 0, (t2 >> 1) * kTreeTile, h, seg.b);
+#pragma unroll
+        for (int sl = 0; sl < DPAD / 64; ++sl)  // slabs of 64 codes, like those of the tiles they become
+          ptx::tma_load_4d(r.codes + slot * (128 * DPAD) + sl * 8192, (t2 & 1) ? tmap_v : tmap_k, full, sl * 64, (t2 >> 1) * kTreeTile, h, seg.b);
       }
       __syncwarp();
     }
@@ -353,9 +357,10 @@ __device__ __forceinline__ void tree_tma_codes(const TreeParams& p, const TreeRi
 }
 
 // One warp: the scale bytes, two tiles at a time so that their loads' latencies overlap.  They may lie anywhere, at any
-// stride, so plain loads bring them.
+// stride, so plain loads bring them.  After each two tiles `also(tiles so far)` may do other work; it returns whether to go on.
+template <typename Also>
 __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int lane,
-                                                 volatile int* abort_flag) {
+                                                 volatile int* abort_flag, Also also) {
   TreeSegment seg{};
   int t = 0;
   bool more = walk.next(seg);
@@ -388,6 +393,7 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
     }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(r.bar_sc_full + 8u * buf);
+    if (!also(2LL * (batch + 1))) return;
   }
 }
 
@@ -397,13 +403,14 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
 template <typename T, int DPAD, int KS, int VS, int SS>
 __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int tid,
                                                    volatile int* abort_flag, volatile int* bad_flag) {
-  constexpr uint32_t kTileBytes = 128 * DPAD * 2, kSlabBytes = 128 * 128;
-  constexpr int kPerRow = DPAD / 16;                            // 16-code pieces of a row
-  constexpr int kRows = 32 * kTreeConvertWarps / kPerRow;       // rows the warps take at a time
-  constexpr int kPasses = 128 / kRows;
-  const int lane = tid & 31;
-  const int piece = tid % kPerRow, row0 = tid / kPerRow;
-  uint32_t seq = 0;  // tiles so far
+  constexpr uint32_t kTileBytes = 128 * DPAD * 2;
+  constexpr int kPasses = DPAD / 32;  // a warp takes 16 rows, 8 of one slab at a time
+  const int lane = tid & 31, row0 = (tid >> 5) * 16 + (lane >> 2), piece = lane & 3;
+  // Eight lanes read two rows of 64 codes and write 16-byte pieces 2 * piece (then 2 * piece + 1) of two rows of opposite
+  // parity: the swizzle puts them in eight different places, so neither access meets a bank twice.
+  const uint32_t from = r.codes + row0 * 64 + piece * 16;
+  const uint32_t to = row0 * 128u, at0 = ((2u * piece) ^ (lane >> 2)) << 4, at1 = at0 ^ 16u;
+  uint32_t seq = 0, c_seq = 0;  // tiles so far; code tiles so far
   bool ok = true;
   TreeSegment seg{};
   while (ok && walk.next(seg)) {
@@ -414,51 +421,50 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
         ok = WAIT(r.bar_sc_full + 8u * ((seq >> 1) & 1u), (seq >> 2) & 1u, ST_TR_WAIT_SC_FULL);
         if (!ok) break;
       }
-      const uint32_t scales = r.scales + (seq & 3u) * 256u;
+      const uint32_t scales = r.scales + (seq & 3u) * 256u + row0;
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv) {
-        const uint32_t from = 2u * seq + kv, c_slot = from % SS;
-        ok = WAIT(r.bar_c_full + 8u * c_slot, (from / SS) & 1u, ST_TR_WAIT_C_FULL);
+      for (int kv = 0; kv < 2; ++kv, ++c_seq) {
+        const uint32_t c_slot = c_seq % SS;
+        ok = WAIT(r.bar_c_full + 8u * c_slot, (c_seq / SS) & 1u, ST_TR_WAIT_C_FULL);
         if (!ok) break;
         uint4 codes[kPasses];
-        uint32_t scale[kPasses];
-        bool short_scale = true;
+        const uint32_t scale[2] = {ptx::lds8(scales + kv * 128u), ptx::lds8(scales + kv * 128u + 8u)};
 #pragma unroll
-        for (int k = 0; k < kPasses; ++k) {
-          const int row = row0 + k * kRows;
-          codes[k] = ptx::lds128(r.codes + c_slot * (128 * DPAD) + row * DPAD + piece * 16);
-          scale[k] = ptx::lds8(scales + kv * 128u + row);
-          if (row >= end) codes[k] = make_uint4(0u, 0u, 0u, 0u);
-          short_scale = short_scale && tree_short_scale(scale[k]);
+        for (int k = 0; k < kPasses; ++k) codes[k] = ptx::lds128(from + c_slot * (128 * DPAD) + (k >> 1) * 8192 + (k & 1) * 512);
+        if (end < kTreeTile) {
+#pragma unroll
+          for (int k = 0; k < kPasses; ++k)
+            if (row0 + (k & 1) * 8 >= end) codes[k] = make_uint4(0u, 0u, 0u, 0u);
         }
-        short_scale = __all_sync(0xffffffffu, short_scale);  // (every lane has its codes: the slot may be filled again)
-        if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);
+        const bool short_scale = __all_sync(0xffffffffu, tree_short_scale(scale[0]) && tree_short_scale(scale[1]));
+        if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);  // (every lane has its codes)
         const uint32_t slots = kv ? VS : KS, slot = seq % slots;
         ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ((seq / slots) & 1u) ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
         if (!ok) break;
-        const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes;
-        const bool check = kv == 1 && drafted < kTreeTile;
+        const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes + to;
+        const bool plain = short_scale && !(kv == 1 && drafted < kTreeTile);
         auto convert = [&](auto format) {
+          constexpr int kFormat = decltype(format)::value;
+          if (plain) {
 #pragma unroll
-          for (int k = 0; k < kPasses; ++k) {
-            const int row = row0 + k * kRows;
-            uint32_t o[8];
-            tree_convert16<T, decltype(format)::value>(codes[k], scale[k], short_scale, o);
-            if (check && row >= drafted) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const bool lo = non_finite16<T>(o[e] & 0xffffu), hi = non_finite16<T>(o[e] >> 16);
-                if (lo) o[e] &= 0xffff0000u;
-                if (hi) o[e] &= 0xffffu;
-                if (lo || hi) *bad_flag = 1;
-              }
+            for (int k = 0; k < kPasses; ++k) {
+              uint32_t o[8];
+              tree_convert16<T, kFormat>(codes[k], scale[k & 1], o);
+              const uint32_t a = dst + (k >> 1) * (128u * 128u) + (k & 1) * 1024u;
+              ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
+              ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
             }
-            // pieces of the second slab write their halves in the other order: a quarter of a warp then covers all banks
-            const uint32_t at_row = dst + (uint32_t)(piece >> 2) * kSlabBytes + (uint32_t)row * 128u;
-            const uint32_t c = (uint32_t)(piece & 3) * 2u, x7 = (uint32_t)row & 7u, odd = (uint32_t)(piece >> 2) & 1u;
-            const uint4 half0 = make_uint4(o[0], o[1], o[2], o[3]), half1 = make_uint4(o[4], o[5], o[6], o[7]);
-            ptx::sts128(at_row + (((c + odd) ^ x7) << 4), odd ? half1 : half0);
-            ptx::sts128(at_row + (((c + 1u - odd) ^ x7) << 4), odd ? half0 : half1);
+          } else {  // unusual scales, or values of drafted tokens, which must be finite
+#pragma unroll
+            for (int k = 0; k < kPasses; ++k) {
+              const uint32_t a = dst + (k >> 1) * (128u * 128u) + (k & 1) * 1024u;
+              uint32_t o[8];
+              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[k].x, codes[k].y), scale[k & 1]);
+              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[k].z, codes[k].w), scale[k & 1]);
+              if (kv == 1 && row0 + (k & 1) * 8 >= drafted && clean_words<T>(o, 8)) *bad_flag = 1;
+              ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
+              ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
+            }
           }
         };
         if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
@@ -497,10 +503,8 @@ __device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeR
   } else {
     if (role == 0)
       tree_tma_codes<DPAD, SS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
-    else if (role == 1)
-      tree_load_scales(p, ring, walk, lane, abort_flag);
     else
-      tree_convert_tiles<T, DPAD, KS, VS, SS>(p, ring, walk, 32 * (role - 2) + lane, abort_flag, bad_flag);
+      tree_convert_tiles<T, DPAD, KS, VS, SS>(p, ring, walk, 32 * (role - 1) + lane, abort_flag, bad_flag);
   }
 }
 
@@ -540,6 +544,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                       const __grid_constant__ TreeParams p) {
   using L = TreeSmem<DPAD, PAIR, QUANT>;
   constexpr int KS = L::KS, VS = L::VS;
+  constexpr int kTreeQWarps = QUANT ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = ptx::smem_u32(smem);
   if ((base & 1023u) != 0) {
@@ -631,41 +636,22 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)kh * p.G * p.qh;
       const uint32_t dst0 = base + L::off_q + buf * L::kQBytes;
       constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
-      constexpr int kAhead = 8;
-      constexpr int pieces = kRowsHere * kChunks;
-      for (int i0 = tid; i0 < pieces; i0 += 32 * kTreeQWarps * kAhead) {
-        uint4 v[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int i = i0 + u * 32 * kTreeQWarps;
-          const int row = i / kChunks, d0 = (i % kChunks) * 8, r = r0 + row;
-          v[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (i < pieces && r < p.rows && d0 < p.D) {
-            const int g = r / p.M, m = r - g * p.M;
-            const unsigned short* src = q + g * p.qh + m * p.qm + d0;
-            if (p.q_vec) {
-              v[u] = *reinterpret_cast<const uint4*>(src);
-            } else {
-              unsigned short* e = reinterpret_cast<unsigned short*>(&v[u]);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) e[j] = src[j];
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int i = i0 + u * 32 * kTreeQWarps;
-          if (i < pieces) {
-            const int row = i / kChunks, c = i % kChunks;
-            const uint32_t tile = dst0 + (uint32_t)(row >> 7) * L::kTileBytes, in = (uint32_t)(row & 127);
-            ptx::sts128(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u, v[u]);
-          }
-        }
+      // (all copies of a segment under way at once: behind the flood of key and value tiles each wait costs microseconds)
+      for (int i = tid; i < kRowsHere * kChunks; i += 32 * kTreeQWarps) {
+        const int row = i / kChunks, c = i % kChunks, d0 = c * 8, r = r0 + row;
+        const int g = r / p.M, m = r - g * p.M;
+        const bool on = r < p.rows && d0 < p.D;
+        const uint32_t tile = dst0 + (uint32_t)(row >> 7) * L::kTileBytes, in = (uint32_t)(row & 127);
+        ptx::cp_async16(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u,
+                        on ? q + g * p.qh + m * p.qm + d0 : q, on);
       }
+      ptx::cp_async_wait_all();
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_q_full(buf));
     }
+  } else if (QUANT && warp == kTreeQWarp + 1) {
+    tree_load_scales(p, ring, walk, lane, abort_flag, [](long long) { return true; });
   } else if (warp == kTreeMmaWarp) {
     // ------------------------------------------------------------------- products
     // Step j: tile j (PAIR: tile j / 2) for warpgroup j mod 2.  S runs two steps ahead of P V, which also orders

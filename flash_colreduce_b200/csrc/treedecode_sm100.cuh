@@ -20,11 +20,12 @@
 
 namespace fcr {
 
-// Warps: 4 per 32 rows for the softmax, one that issues S^T, one that issues O^T, one for the queries, then the loads'.
+// Warps: 4 per 32 rows for the softmax, one that issues S^T, one that issues O^T, one for the queries (and an 8-bit cache's
+// scales), one for TMA, and those that convert codes.
 template <int NR>
 __host__ __device__ constexpr int decode_softmax_warps() { return NR == 64 ? 8 : 4; }
 template <int NR, bool QUANT>
-__host__ __device__ constexpr int decode_threads() { return 32 * (decode_softmax_warps<NR>() + 4 + (QUANT ? 1 + kTreeConvertWarps : 0)); }
+__host__ __device__ constexpr int decode_threads() { return 32 * (decode_softmax_warps<NR>() + 4 + (QUANT ? kTreeConvertWarps : 0)); }
 
 // Minus the reference of a row that has seen no key: any finite score passes it, and a masked one (-inf) stays at weight 0.
 constexpr float kNothingSeen = 3e38f;
@@ -182,10 +183,11 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
 
   if (warp == kQWarp) {
     // ----------------------------------------------------- queries of the next segment
+    // (all copies of a segment under way at once: behind the flood of key and value tiles each wait costs microseconds)
     uint32_t seq = 0;
-    while (walk.next(seg)) {
+    auto load_queries = [&]() {
       const uint32_t buf = seq % L::kQBuffers;
-      if (!WAIT_BEHIND(bar_q_empty + 8u * buf, ((seq / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) break;
+      if (!WAIT_BEHIND(bar_q_empty + 8u * buf, ((seq / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
       ++seq;
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)seg.group * p.G * p.qh;
       const uint32_t dst = base + L::off_q + buf * L::kQBytes;
@@ -195,24 +197,33 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       int row = lane / kChunks, g = row / p.M, m = row - g * p.M;
 #pragma unroll 4
       for (int i = 0; i < NR / kRowsAtATime; ++i) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < p.rows && d0 < p.D) {
-          const unsigned short* src = q + g * p.qh + m * p.qm + d0;
-          if (p.q_vec) {
-            v = *reinterpret_cast<const uint4*>(src);
-          } else {
-            unsigned short* e = reinterpret_cast<unsigned short*>(&v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = src[j];
-          }
-        }
-        ptx::sts128(dst + (uint32_t)(c >> 3) * L::kQSlabBytes + (uint32_t)row * 128u + (((uint32_t)c & 7u) ^ ((uint32_t)row & 7u)) * 16u, v);
+        const bool on = row < p.rows && d0 < p.D;
+        ptx::cp_async16(dst + (uint32_t)(c >> 3) * L::kQSlabBytes + (uint32_t)row * 128u + (((uint32_t)c & 7u) ^ ((uint32_t)row & 7u)) * 16u,
+                        on ? q + g * p.qh + m * p.qm + d0 : q, on);
         row += kRowsAtATime;
         for (m += kRowsAtATime; m >= p.M; m -= p.M) ++g;
       }
+      ptx::cp_async_wait_all();
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_q_full + 8u * buf);
+      return true;
+    };
+    if constexpr (QUANT) {
+      // The queries of a segment follow the scales of its first tiles: those never wait for queries, which may wait for the
+      // products of the segment before.
+      TreeWalk<TreeLengths> scale_walk = walk;
+      long long next_at = 0;  // first tile of the next segment whose queries are to come
+      tree_load_scales(p, ring, scale_walk, lane, abort_flag, [&](long long tiles) {
+        while (next_at < tiles && walk.next(seg)) {
+          next_at += seg.hi - seg.lo;
+          if (!load_queries()) return false;
+        }
+        return true;
+      });
+    } else {
+      while (walk.next(seg) && load_queries()) {
+      }
     }
   } else if (warp == kSWarp) {
     // ------------------------------------------------------------------- S^T = K Q^T
@@ -318,13 +329,16 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const bool edge = (t + 1) * kTreeTile > seg.have;
-        uint32_t x[W];
-        tmem_row_ld<W>(s_addr, x);
-        if (edge) {
-          const uint32_t bits = decode_row_bits(p, seg, t * kTreeTile + key, r0, W);
+        auto load_scores = [&](uint32_t (&x)[W]) {
+          tmem_row_ld<W>(s_addr, x);
+          if (edge) {
+            const uint32_t bits = decode_row_bits(p, seg, t * kTreeTile + key, r0, W);
 #pragma unroll
-          for (int e = 0; e < W; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xff800000u;
-        }
+            for (int e = 0; e < W; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xff800000u;
+          }
+        };
+        uint32_t x[W];
+        load_scores(x);
         // exponents against the reference as it is: has one passed 8?
         float w[W];
         float most = -INFINITY;
@@ -341,6 +355,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         if (vote[buf] == (int)tile_seq) {
           // the rows' maxima over the tile's 128 keys; O^T, the sums and the reference follow where a row has grown
           float top = -INFINITY;
+          load_scores(x);  // (again: in registers they would crowd out the loop's values)
 #pragma unroll
           for (int e = 0; e < W; ++e) {
             const float largest = ptx::redux_max(__uint_as_float(x[e]));
@@ -371,6 +386,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
             tmem_row_st<W>(o_addr, o);
             ptx::tmem_st_wait();
           }
+          load_scores(x);
 #pragma unroll
           for (int e = 0; e < W; ++e) w[e] = fmaf(__uint_as_float(x[e]), p.scale2, ref_s[e]);
         }

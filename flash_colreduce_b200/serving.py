@@ -294,7 +294,7 @@ def tree_attention(
     matter, NaN and infinities included.
 
     Args:
-        query: (B, Hq, M, D) fp16 or bf16, M <= 256, D <= 128; any strides with innermost 1 (others are copied).
+        query: (B, Hq, M, D) fp16 or bf16, M <= 256, D <= 128; strides that are not multiples of 16 bytes are copied.
         key_cache, value_cache: (B, H, N, D), Hq a multiple of H (query head ``h`` reads cache head ``h // (Hq // H)``);
             of ``query``'s type with D a multiple of 8, or float8_e4m3fn / int8 with D a multiple of 16.  Base addresses
             and strides are multiples of 16 bytes.
@@ -326,7 +326,8 @@ def tree_attention(
     if out.numel() == 0 or n == 0:
         out.zero_()
         return (out, lse.fill_(-math.inf)) if return_lse else out
-    query = _rows(query)
+    if query.stride(3) != 1 or query.data_ptr() % 16 or any(query.shape[i] > 1 and query.stride(i) % 8 for i in range(3)):
+        query = query.clone(memory_format=torch.contiguous_format)  # the kernels copy queries 16 bytes at a time
     tree = nat.Tree(hq, m, (*query.stride()[:3], 1), _INDEX_BITS[lengths.dtype], (0, 0), scale)
     if tree_mask is not None:
         tree_mask = _rows(tree_mask)

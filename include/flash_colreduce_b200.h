@@ -459,7 +459,7 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
 
 /*
  * Attention of M drafted tokens per sequence (q: (B,Hq,M,D), innermost stride
- * 1; Hq a multiple of the cache's H, query head h reads cache head h / (Hq / H))
+ * 1, base and other strides multiples of 16 bytes, like the cache's; Hq a multiple of the cache's H, query head h reads cache head h / (Hq / H))
  * over a cache.  Every token of sequence b attends positions 0 .. lengths[b]-1
  * and, of the drafted tokens, which lie at lengths[b] .. lengths[b]+M-1
  * (fcr_kv_append puts them there), those j with mask[b,m,j] != 0; a null mask
