@@ -32,6 +32,7 @@ struct KvAppendParams {
   long long xb[2], xh[2], xm[2];
   int B, H, N, D, M;
   int group;               // lanes per row: the power of two that covers D in steps of 8
+  int blocks_per_head;
   const void* lengths;
   const void* counts;      // null: all M tokens
   int index_bits;
@@ -41,7 +42,7 @@ struct KvReadParams {
   KvTensor t[2];
   void* y[2];              // contiguous (B, H, n, D)
   int B, H, N, D, n;
-  int group;
+  int group, blocks_per_head;
   const void* positions;   // (B, H, n) contiguous or null: 0 .. n-1
   int index_bits;
 };
@@ -116,57 +117,75 @@ __device__ __forceinline__ float kv_largest() {
   return sizeof(T) == 2 && std::is_same<T, __half>::value ? m * 32768.f : m * 1.7014118346046923e38f;
 }
 
-// `group` lanes per row, 8 consecutive values each.  A row's K and V, tokens, heads and sequences are all one index.
+// Both kernels: a block takes kKvRows rows per lane group of one (K or V, sequence, head); `group` lanes per row, eight
+// consecutive values each.  A thread's rows are read together, so that four loads are under way (a row at a time, with the
+// row's place found by 64-bit divisions, took 2.4 times as long on 32768 tokens).
+constexpr int kKvRows = 4;
+struct KvPlace {
+  int kv, b, h, row0, step;  // first row of this thread, distance to its next
+};
+__device__ __forceinline__ KvPlace kv_place(int B, int H, int group, int blocks_per_head) {
+  const int combo = blockIdx.x / blocks_per_head, block = blockIdx.x - combo * blocks_per_head;
+  KvPlace r;
+  r.kv = combo / (B * H);
+  const int bh = combo - r.kv * (B * H);
+  r.b = bh / H;
+  r.h = bh - r.b * H;
+  r.step = (int)blockDim.x / group;
+  r.row0 = block * r.step * kKvRows + (int)threadIdx.x / group;
+  return r;
+}
+
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(256)
-kv_append_kernel(const KvAppendParams p) {
+kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   const int group = p.group;
-  const int gl = threadIdx.x & (group - 1);
-  const long long rows = 2LL * p.B * p.H * p.M;
-  const int d0 = gl * 8;
+  const int gl = threadIdx.x & (group - 1), d0 = gl * 8;
   const bool on = d0 < p.D;
-  const long long per_block = blockDim.x / group;
-  const long long stride = (long long)gridDim.x * per_block;
-  // every lane of a warp makes the same number of trips: the shuffles below need them all
-  for (long long base = (long long)blockIdx.x * per_block; base < rows; base += stride) {
-    const long long r = base + threadIdx.x / group;
-    bool live = r < rows;
-    long long rest = live ? r : 0;
-    const long long m = rest % p.M;
-    rest /= p.M;
-    const int h = (int)(rest % p.H);
-    rest /= p.H;
-    const int b = (int)(rest % p.B), kv = (int)(rest / p.B);
-    long long n = -1;
-    if (live) {
-      n = load_index(p.lengths, p.index_bits, b);
-      if (n < 0 || (p.counts && m >= load_index(p.counts, p.index_bits, b))) live = false;
-      n += m;
-      if (n >= p.N) live = false;
-    }
-    const T* x = reinterpret_cast<const T*>(p.x[kv]) + b * p.xb[kv] + h * p.xh[kv] + m * p.xm[kv] + d0;
-    const KvTensor& t = p.t[kv];
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (live && on) {
+  const KvPlace at = kv_place(p.B, p.H, group, p.blocks_per_head);
+  const KvTensor& t = p.t[at.kv];
+  const T* x = reinterpret_cast<const T*>(p.x[at.kv]) + at.b * p.xb[at.kv] + at.h * p.xh[at.kv] + d0;
+  const long long first = load_index(p.lengths, p.index_bits, at.b);
+  // tokens that are written: m < count, and their positions exist
+  long long count = p.counts ? min(load_index(p.counts, p.index_bits, at.b), (long long)p.M) : p.M;
+  count = first < 0 ? 0 : min(count, (long long)p.N - first);
+  uint4 raw[kKvRows];
+#pragma unroll
+  for (int u = 0; u < kKvRows; ++u) {
+    const int m = at.row0 + u * at.step;
+    raw[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (m < count && on) {
       if (VEC) {
-        raw = *reinterpret_cast<const uint4*>(x);
+        raw[u] = *reinterpret_cast<const uint4*>(x + m * p.xm[at.kv]);
       } else {
-        unsigned short* e = reinterpret_cast<unsigned short*>(&raw);
-        for (int j = 0; j < 8; ++j) e[j] = d0 + j < p.D ? reinterpret_cast<const unsigned short*>(x)[j] : (unsigned short)0;
+        unsigned short e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = d0 + j < p.D ? reinterpret_cast<const unsigned short*>(x + m * p.xm[at.kv])[j] : (unsigned short)0;
+        raw[u] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
       }
     }
+  }
+#pragma unroll
+  for (int u = 0; u < kKvRows; ++u) {
+    const int m = at.row0 + u * at.step;
+    const bool live = m < count;
+    const long long n = first + m;
     if (FORMAT == FCR_KV_16BIT) {
       if (live && on) {
-        T* y = reinterpret_cast<T*>(t.data) + b * t.sb + h * t.sh + n * t.sn + d0;
-        if (VEC)
-          *reinterpret_cast<uint4*>(y) = raw;
-        else
-          for (int j = 0; j < 8 && d0 + j < p.D; ++j) y[j] = reinterpret_cast<const T*>(&raw)[j];
+        unsigned short* y = reinterpret_cast<unsigned short*>(t.data) + at.b * t.sb + at.h * t.sh + n * t.sn + d0;
+        if (VEC) {
+          *reinterpret_cast<uint4*>(y) = raw[u];
+        } else {
+          const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (d0 + j < p.D) y[j] = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
+        }
       }
       continue;
     }
     float v[8];
-    unpack8(raw, v, T());
+    unpack8(raw[u], v, T());
     // the largest magnitude by its bits: a NaN or infinity is then larger than every finite value
     uint32_t top = 0;
 #pragma unroll
@@ -194,65 +213,94 @@ kv_append_kernel(const KvAppendParams p) {
       }
     }
     if (on) {
-      unsigned char* y = reinterpret_cast<unsigned char*>(t.data) + b * t.sb + h * t.sh + n * t.sn + d0;
-      if (VEC)
+      unsigned char* y = reinterpret_cast<unsigned char*>(t.data) + at.b * t.sb + at.h * t.sh + n * t.sn + d0;
+      if (VEC) {
         *reinterpret_cast<uint2*>(y) = make_uint2(code[0], code[1]);
-      else
-        for (int j = 0; j < 8 && d0 + j < p.D; ++j) y[j] = (unsigned char)(code[j >> 2] >> (8 * (j & 3)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (d0 + j < p.D) y[j] = (unsigned char)(code[j >> 2] >> (8 * (j & 3)));
+      }
     }
-    if (gl == 0) t.scales[b * t.ssb + h * t.ssh + n * t.ssn] = (unsigned char)(e + 127);
+    if (gl == 0) t.scales[at.b * t.ssb + at.h * t.ssh + n * t.ssn] = (unsigned char)(e + 127);
   }
 }
 
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(256)
-kv_read_kernel(const KvReadParams p) {
+kv_read_kernel(const __grid_constant__ KvReadParams p) {
   const int group = p.group;
-  const int gl = threadIdx.x & (group - 1);
-  const long long rows = 2LL * p.B * p.H * p.n;
-  const int d0 = gl * 8;
+  const int gl = threadIdx.x & (group - 1), d0 = gl * 8;
   if (d0 >= p.D) return;
-  const long long per_block = blockDim.x / group;
-  for (long long r = (long long)blockIdx.x * per_block + threadIdx.x / group; r < rows; r += (long long)gridDim.x * per_block) {
-    long long rest = r;
-    const long long i = rest % p.n;
-    rest /= p.n;
-    const int h = (int)(rest % p.H);
-    rest /= p.H;
-    const int b = (int)(rest % p.B), kv = (int)(rest / p.B);
-    const KvTensor& t = p.t[kv];
-    const long long row = ((long long)b * p.H + h) * p.n + i;
-    const long long pos = p.positions ? load_index(p.positions, p.index_bits, row) : i;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (pos >= 0 && pos < p.N) {
-      const long long at = b * t.sb + h * t.sh + pos * t.sn + d0;
-      if (FORMAT == FCR_KV_16BIT) {
-        const unsigned short* x = reinterpret_cast<const unsigned short*>(t.data) + at;
-        if (VEC)
-          raw = *reinterpret_cast<const uint4*>(x);
-        else
-          for (int j = 0; j < 8 && d0 + j < p.D; ++j) reinterpret_cast<unsigned short*>(&raw)[j] = x[j];
-      } else {
-        const unsigned char* x = reinterpret_cast<const unsigned char*>(t.data) + at;
-        uint2 c = make_uint2(0u, 0u);
-        if (VEC)
-          c = *reinterpret_cast<const uint2*>(x);
-        else
-          for (int j = 0; j < 8 && d0 + j < p.D; ++j) reinterpret_cast<unsigned char*>(&c)[j] = x[j];
-        const float s = kv_scale(t.scales[b * t.ssb + h * t.ssh + pos * t.ssn]);
-        float v[8];
-        unpack_codes4<FORMAT>(c.x, v);
-        unpack_codes4<FORMAT>(c.y, v + 4);
-        uint32_t* o = reinterpret_cast<uint32_t*>(&raw);
+  const KvPlace at = kv_place(p.B, p.H, group, p.blocks_per_head);
+  const KvTensor& t = p.t[at.kv];
+  const long long row_base = ((long long)at.b * p.H + at.h) * p.n;
+  const long long data_base = at.b * t.sb + at.h * t.sh + d0, scale_base = at.b * t.ssb + at.h * t.ssh;
+  constexpr int kWords = FORMAT == FCR_KV_16BIT ? 4 : 2;
+  long long pos[kKvRows];
+  uint32_t raw[kKvRows][kWords];
+  uint32_t byte[kKvRows];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = pack2(v[2 * j] * s, v[2 * j + 1] * s, T());
+  for (int u = 0; u < kKvRows; ++u) {
+    const int i = at.row0 + u * at.step;
+    pos[u] = -1;
+    if (i < p.n) pos[u] = p.positions ? load_index(p.positions, p.index_bits, row_base + i) : i;
+  }
+#pragma unroll
+  for (int u = 0; u < kKvRows; ++u) {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) raw[u][j] = 0u;
+    byte[u] = 127u;
+    if (pos[u] >= 0 && pos[u] < p.N) {
+      const long long from = data_base + pos[u] * t.sn;
+      if (FORMAT == FCR_KV_16BIT) {
+        const unsigned short* x = reinterpret_cast<const unsigned short*>(t.data) + from;
+        if (VEC) {
+          const uint4 q = *reinterpret_cast<const uint4*>(x);
+          raw[u][0] = q.x, raw[u][1] = q.y, raw[u][kWords - 2] = q.z, raw[u][kWords - 1] = q.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (d0 + j < p.D) raw[u][(j >> 1) % kWords] |= (uint32_t)x[j] << (16 * (j & 1));
+        }
+      } else {
+        const unsigned char* x = reinterpret_cast<const unsigned char*>(t.data) + from;
+        if (VEC) {
+          const uint2 q = *reinterpret_cast<const uint2*>(x);
+          raw[u][0] = q.x, raw[u][1] = q.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (d0 + j < p.D) raw[u][(j >> 2) % kWords] |= (uint32_t)x[j] << (8 * (j & 3));
+        }
+        byte[u] = t.scales[scale_base + pos[u] * t.ssn];
       }
     }
-    T* y = reinterpret_cast<T*>(p.y[kv]) + row * p.D + d0;
-    if (VEC)
-      *reinterpret_cast<uint4*>(y) = raw;
-    else
-      for (int j = 0; j < 8 && d0 + j < p.D; ++j) reinterpret_cast<unsigned short*>(y)[j] = reinterpret_cast<const unsigned short*>(&raw)[j];
+  }
+#pragma unroll
+  for (int u = 0; u < kKvRows; ++u) {
+    const int i = at.row0 + u * at.step;
+    if (i >= p.n) continue;
+    uint32_t o[4];
+    if constexpr (FORMAT == FCR_KV_16BIT) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = raw[u][j];
+    } else {
+      const float s = kv_scale(byte[u]);
+      float v[8];
+      unpack_codes4<FORMAT>(raw[u][0], v);
+      unpack_codes4<FORMAT>(raw[u][1], v + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = pack2(v[2 * j] * s, v[2 * j + 1] * s, T());
+    }
+    unsigned short* y = reinterpret_cast<unsigned short*>(p.y[at.kv]) + (row_base + i) * p.D + d0;
+    if (VEC) {
+      *reinterpret_cast<uint4*>(y) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (d0 + j < p.D) y[j] = (unsigned short)(o[j >> 1] >> (16 * (j & 1)));
+    }
   }
 }
 

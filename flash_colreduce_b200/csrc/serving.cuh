@@ -12,6 +12,39 @@ static bool kv_aligned(const void* ptr, const int64_t* strides, const int32_t* s
   return true;
 }
 
+template <typename T, int LPR>
+static cudaError_t launch_rope_vector(const RopeParams& p, dim3 grid, cudaStream_t stream) {
+  return p.interleaved ? launch_kernel(rope_vector_kernel<T, LPR, true>, grid, dim3(256), 0, stream, false, p)
+                       : launch_kernel(rope_vector_kernel<T, LPR, false>, grid, dim3(256), 0, stream, false, p);
+}
+template <typename T>
+static cudaError_t launch_rope(RopeParams& p, int sms, cudaStream_t stream) {
+  const int heads = p.heads[0] + p.heads[1];
+  bool vec = p.D % 16 == 0 && p.half % 8 == 0;
+  for (int i = 0; i < 2; ++i) {
+    if (p.heads[i] == 0) continue;
+    const int64_t st[3] = {p.sb[i], p.sh[i], p.sm[i]};
+    const int32_t sizes[3] = {p.B, p.heads[i], p.M};
+    vec = vec && kv_aligned(p.x[i], st, sizes, 3, sizeof(T), 16) && reinterpret_cast<uintptr_t>(p.y[i]) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(p.weight[i]) % 16 == 0;
+  }
+  const long long tokens = (long long)p.B * p.M;
+  if (vec) {
+    const int lpr = p.D <= 64 ? 4 : p.D <= 128 ? 8 : 16, at_a_time = 32 / lpr;
+    // All heads of a token in one warp spare it angles; with few tokens the heads are spread until there are 8 warps per SM.
+    const long long want = std::max<long long>(1, (8LL * sms + tokens - 1) / tokens);
+    const int chunks = (int)std::min<long long>(want, (heads + at_a_time - 1) / at_a_time);
+    p.heads_per_warp = ((heads + chunks - 1) / chunks + at_a_time - 1) / at_a_time * at_a_time;
+    const long long blocks = (tokens + 7) / 8 * ((heads + p.heads_per_warp - 1) / p.heads_per_warp);
+    if (blocks <= 0x7fffffffLL) {
+      const dim3 grid((unsigned)blocks);
+      return lpr == 4 ? launch_rope_vector<T, 4>(p, grid, stream) : lpr == 8 ? launch_rope_vector<T, 8>(p, grid, stream) : launch_rope_vector<T, 16>(p, grid, stream);
+    }
+  }
+  const long long rows = tokens * heads;
+  return launch_kernel(rope_rows_kernel<T>, dim3((unsigned)std::min<long long>((rows + 7) / 8, (long long)sms * 64)), dim3(256), 0, stream, false, p);
+}
+
 static int check_cache(const fcr_kv_cache& c, const void* k, const void* v, const void* ks, const void* vs) {
   if (!k || !v) return fail(FCR_ERR_BAD_ARG, "null cache");
   if (c.B <= 0 || c.H <= 0 || c.N <= 0 || c.D <= 0) return fail(FCR_ERR_BAD_ARG, "cache sizes must be positive");
@@ -53,9 +86,12 @@ static int kv_group(int D) {
   return g;
 }
 
-static unsigned kv_blocks(long long rows, int group, int sms) {
-  const long long per_block = 256 / group;
-  return (unsigned)std::min<long long>((rows + per_block - 1) / per_block, (long long)sms * 32);
+// Blocks for `rows` rows of each of 2 * B * H (K or V, sequence, head); 0 when the grid would be too large.
+static unsigned kv_blocks(int B, int H, int rows, int group, int* blocks_per_head) {
+  const int per_block = 256 / group * kKvRows;
+  *blocks_per_head = (rows + per_block - 1) / per_block;
+  const long long blocks = 2LL * B * H * *blocks_per_head;
+  return blocks > 0x7fffffffLL ? 0u : (unsigned)blocks;
 }
 
 template <typename T, int FORMAT>
@@ -256,15 +292,13 @@ int fcr_qk_norm_rope(const fcr_rope* problem, const void* q, const void* k, cons
   const int rc = device_sm_count(&sms);
   if (rc != FCR_OK) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  const long long rows = (long long)r.B * r.M * (r.Hq + r.Hk);
-  const dim3 grid((unsigned)std::min<long long>((rows + 7) / 8, (long long)sms * 64)), block(256);
   cudaError_t e;
   if (r.dtype == FCR_F16)
-    e = launch_kernel(rope_rows_kernel<__half>, grid, block, 0, stream, false, p);
+    e = launch_rope<__half>(p, sms, stream);
   else if (r.dtype == FCR_BF16)
-    e = launch_kernel(rope_rows_kernel<__nv_bfloat16>, grid, block, 0, stream, false, p);
+    e = launch_rope<__nv_bfloat16>(p, sms, stream);
   else
-    e = launch_kernel(rope_rows_kernel<float>, grid, block, 0, stream, false, p);
+    e = launch_rope<float>(p, sms, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope launch");
   return FCR_OK;
@@ -304,11 +338,12 @@ int fcr_kv_append(const fcr_kv_cache* cache, void* k_cache, void* v_cache, void*
   const int32_t sizes[3] = {c.B, c.H, M};
   const bool vec = cache_vectors(c, k_cache, v_cache) && kv_aligned(key, key_strides, sizes, 3, 2, 16) &&
                    kv_aligned(value, value_strides, sizes, 3, 2, 16);
+  const unsigned blocks = kv_blocks(c.B, c.H, M, p.group, &p.blocks_per_head);
+  if (blocks == 0) return fail(FCR_ERR_UNSUPPORTED, "too many rows");
   int sms = 0;
-  rc = device_sm_count(&sms);
+  rc = device_sm_count(&sms);  // refuses a device that this library has no code for
   if (rc != FCR_OK) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  const unsigned blocks = kv_blocks(2LL * c.B * c.H * M, p.group, sms);
   cudaError_t e = c.dtype == FCR_F16 ? launch_append_f<__half>(c.format, p, vec, blocks, stream)
                                      : launch_append_f<__nv_bfloat16>(c.format, p, vec, blocks, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
@@ -340,11 +375,12 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
   p.index_bits = index_bits;
   const bool vec = cache_vectors(c, k_cache, v_cache) && reinterpret_cast<uintptr_t>(k_out) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_out) % 16 == 0;
+  const unsigned blocks = kv_blocks(c.B, c.H, n, p.group, &p.blocks_per_head);
+  if (blocks == 0) return fail(FCR_ERR_UNSUPPORTED, "too many rows");
   int sms = 0;
-  rc = device_sm_count(&sms);
+  rc = device_sm_count(&sms);  // refuses a device that this library has no code for
   if (rc != FCR_OK) return rc;
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_v);
-  const unsigned blocks = kv_blocks(2LL * c.B * c.H * n, p.group, sms);
   cudaError_t e = c.dtype == FCR_F16 ? launch_read_f<__half>(c.format, p, vec, blocks, stream)
                                      : launch_read_f<__nv_bfloat16>(c.format, p, vec, blocks, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
