@@ -46,8 +46,22 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 and x.is_contiguous() else x.contiguous()
 
 
-def _stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+# What a call's signature (shapes, strides, types, devices, options; no data, no addresses) comes to.  Small calls are bound
+# by the host, so that a signature is checked once.
+_ROPE_CACHE: dict = {}
+_APPEND_CACHE: dict = {}
+_READ_CACHE: dict = {}
+_TREE_CACHE: dict = {}
+
+
+def _keep(cache: dict, signature, value) -> None:
+    if len(cache) > 4096:
+        cache.clear()
+    cache[signature] = value
+
+
+def _vector_signature(x: Optional[torch.Tensor]):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
 
 
 def qk_norm_rope(
@@ -77,7 +91,34 @@ def qk_norm_rope(
     Returns:
         ``(query, key)``, new contiguous tensors of the inputs' type.
     """
-    _check_no_grad("qk_norm_rope", query, key, q_weight, k_weight, inv_freq)
+    if torch.is_grad_enabled():
+        _check_no_grad("qk_norm_rope", query, key, q_weight, k_weight, inv_freq)
+    signature = (query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype, key.get_device(), positions.shape,
+                 positions.stride(), positions.dtype, positions.get_device(), inv_freq.shape, inv_freq.is_contiguous(), inv_freq.dtype, inv_freq.get_device(),
+                 _vector_signature(q_weight), _vector_signature(k_weight), eps, interleaved)
+    problem = _ROPE_CACHE.get(signature)
+    if problem is None:
+        problem, query, key, inv_freq, q_weight, k_weight = _plan_rope(signature, query, key, positions, inv_freq, q_weight, k_weight, eps,
+                                                                       interleaved)
+    b, hq, m, d = query.shape
+    dtype, device = query.dtype, query.device
+    q_out = torch.empty((b, hq, m, d), dtype=dtype, device=device)
+    k_out = torch.empty((b, problem.Hk, m, d), dtype=dtype, device=device)
+    if problem.B * problem.M * problem.D * (problem.Hq + problem.Hk) == 0:
+        return q_out, k_out
+    index = device.index
+    with _on_device(index):
+        rc = nat.lib.fcr_qk_norm_rope(C.byref(problem), query.data_ptr(), key.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                                      None if q_weight is None else q_weight.data_ptr(),
+                                      None if k_weight is None else k_weight.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+                                      torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            nat.check(rc, "fcr_qk_norm_rope")
+    return q_out, k_out
+
+
+def _plan_rope(signature, query, key, positions, inv_freq, q_weight, k_weight, eps, interleaved):
+    """Checks a call of ``qk_norm_rope`` and describes it; the description is kept when the tensors go in as they lie."""
     if query.dim() != 4 or key.dim() != 4 or any(query.shape[i] != key.shape[i] for i in (0, 2, 3)):
         raise ValueError(f"query and key must be (B, H, M, D) with the same B, M and D; got {tuple(query.shape)} and {tuple(key.shape)}.")
     if query.dtype != key.dtype or query.dtype not in _DTYPE_CODES:
@@ -96,26 +137,16 @@ def qk_norm_rope(
             raise ValueError(f"weights must be ({d},) of {query.dtype} or fp32, both of one type; got {w.dtype} {tuple(w.shape)}.")
     _check_devices(query.device, query=query, key=key, positions=positions, inv_freq=inv_freq, q_weight=q_weight,
                    k_weight=k_weight)
-    q_out = torch.empty((b, hq, m, d), dtype=query.dtype, device=query.device)
-    k_out = torch.empty((b, hk, m, d), dtype=query.dtype, device=query.device)
-    if q_out.numel() + k_out.numel() == 0:
-        return q_out, k_out
-    query, key = _rows(query), _rows(key)
-    inv_freq = inv_freq.contiguous()
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    given = (query, key, inv_freq, q_weight, k_weight)
+    used = (_rows(query), _rows(key), inv_freq.contiguous(), *(None if w is None else w.contiguous() for w in (q_weight, k_weight)))
+    query, key, inv_freq = used[:3]
     p = nat.Rope(b, hq, hk, m, d, 2 * inv_freq.shape[0], (*query.stride()[:3], 1), (*key.stride()[:3], 1),
                  _DTYPE_CODES[query.dtype], _DTYPE_CODES[weights[0].dtype] if weights else 0, 1 if interleaved else 0,
                  _INDEX_BITS[positions.dtype], (positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1)),
                  float(eps))
-    index = query.device.index
-    with _on_device(index):
-        rc = nat.lib.fcr_qk_norm_rope(C.byref(p), query.data_ptr(), key.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
-                                      None if q_weight is None else q_weight.data_ptr(),
-                                      None if k_weight is None else k_weight.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
-                                      _stream(index))
-        if rc:
-            nat.check(rc, "fcr_qk_norm_rope")
-    return q_out, k_out
+    if all(x is y for x, y in zip(given, used)):
+        _keep(_ROPE_CACHE, signature, p)
+    return (p, *used)
 
 
 def _cache_problem(key_cache, value_cache, key_scales, value_scales, dtype) -> nat.KvCache:
@@ -185,7 +216,29 @@ def kv_cache_append(
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
         counts: (B,) of the type of ``lengths``, or None.
     """
-    _check_no_grad("kv_cache_append", key, value, key_cache, value_cache)
+    if torch.is_grad_enabled():
+        _check_no_grad("kv_cache_append", key, value, key_cache, value_cache)
+    signature = (key.shape, key.stride(), key.dtype, key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(), key_cache.shape,
+                 key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(), value_cache.dtype,
+                 value_cache.get_device(), lengths.shape, lengths.is_contiguous(), lengths.dtype, lengths.get_device(), _vector_signature(key_scales),
+                 _vector_signature(value_scales), _vector_signature(counts))
+    hit = _APPEND_CACHE.get(signature)
+    if hit is None:
+        hit, key, value, lengths, counts = _plan_append(signature, key, value, key_cache, value_cache, lengths, key_scales, value_scales,
+                                                        counts)
+    if hit == 0:  # nothing to write
+        return
+    problem, key_strides, value_strides, m, index_bits, index = hit
+    with _on_device(index):
+        rc = nat.lib.fcr_kv_append(C.byref(problem), key_cache.data_ptr(), value_cache.data_ptr(), _address(key_scales),
+                                   _address(value_scales), key.data_ptr(), key_strides, value.data_ptr(), value_strides, m,
+                                   lengths.data_ptr(), _address(counts), index_bits, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            nat.check(rc, "fcr_kv_append")
+
+
+def _plan_append(signature, key, value, key_cache, value_cache, lengths, key_scales, value_scales, counts):
+    """Checks a call of ``kv_cache_append`` and describes it (0: nothing to write), as ``_plan_rope`` does."""
     if key.dtype != value.dtype:
         raise TypeError(f"key and value must be of one dtype; got {key.dtype} and {value.dtype}.")
     problem = _cache_problem(key_cache, value_cache, key_scales, value_scales, key.dtype)
@@ -195,7 +248,7 @@ def kv_cache_append(
     for name, x in (("key_cache", key_cache), ("value_cache", value_cache), ("key_scales", key_scales), ("value_scales", value_scales)):
         if x is not None and any(x.shape[i] > 1 and x.stride(i) == 0 for i in range(3)):
             raise ValueError(f"{name} is written: it cannot be an expanded tensor.")
-    m = key.shape[2]
+    given = (key, value, lengths, counts)
     lengths = _lengths("lengths", lengths, b)
     if counts is not None:
         if counts.dtype != lengths.dtype:
@@ -204,16 +257,12 @@ def kv_cache_append(
     _check_devices(key.device, key=key, value=value, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
                    key_scales=key_scales, value_scales=value_scales, counts=counts)
     if key.numel() == 0 or n == 0:
-        return
+        return 0, key, value, lengths, counts
     key, value = _rows(key), _rows(value)
-    index = key.device.index
-    with _on_device(index):
-        rc = nat.lib.fcr_kv_append(C.byref(problem), key_cache.data_ptr(), value_cache.data_ptr(), _address(key_scales),
-                                   _address(value_scales), key.data_ptr(), nat.strides4(key.stride()), value.data_ptr(),
-                                   nat.strides4(value.stride()), m, lengths.data_ptr(), _address(counts),
-                                   _INDEX_BITS[lengths.dtype], _stream(index))
-        if rc:
-            nat.check(rc, "fcr_kv_append")
+    hit = (problem, nat.strides4(key.stride()), nat.strides4(value.stride()), key.shape[2], _INDEX_BITS[lengths.dtype], key.device.index)
+    if all(x is y for x, y in zip(given, (key, value, lengths, counts))):
+        _keep(_APPEND_CACHE, signature, hit)
+    return hit, key, value, lengths, counts
 
 
 def kv_cache_read(
@@ -238,11 +287,38 @@ def kv_cache_read(
     Returns:
         ``(key, value)``, contiguous (B, H, n, D): what :func:`flash_colreduce` takes as keys.
     """
-    _check_no_grad("kv_cache_read", key_cache, value_cache)
+    if torch.is_grad_enabled():
+        _check_no_grad("kv_cache_read", key_cache, value_cache)
+    signature = (key_cache.shape, key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(),
+                 value_cache.dtype, value_cache.get_device(), _vector_signature(key_scales), _vector_signature(value_scales),
+                 _vector_signature(positions), n, dtype)
+    hit = _READ_CACHE.get(signature)
+    if hit is None:
+        hit, positions = _plan_read(signature, key_cache, value_cache, key_scales, value_scales, positions, n, dtype)
+    problem, shape, dtype, index_bits, device = hit
+    k_out = torch.empty(shape, dtype=dtype, device=device)
+    v_out = torch.empty(shape, dtype=dtype, device=device)
+    if k_out.numel() == 0:
+        return k_out, v_out
+    if problem.N == 0:
+        return k_out.zero_(), v_out.zero_()
+    index = device.index
+    with _on_device(index):
+        rc = nat.lib.fcr_kv_read(C.byref(problem), key_cache.data_ptr(), value_cache.data_ptr(), _address(key_scales),
+                                 _address(value_scales), _address(positions), index_bits, shape[2], k_out.data_ptr(), v_out.data_ptr(),
+                                 torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            nat.check(rc, "fcr_kv_read")
+    return k_out, v_out
+
+
+def _plan_read(signature, key_cache, value_cache, key_scales, value_scales, positions, n, dtype):
+    """Checks a call of ``kv_cache_read`` and describes it, as ``_plan_rope`` does."""
     if dtype is None:
         dtype = key_cache.dtype if key_cache.dtype in (torch.float16, torch.bfloat16) else torch.bfloat16
     problem = _cache_problem(key_cache, value_cache, key_scales, value_scales, dtype)
     b, h, cap, d = key_cache.shape
+    given = positions
     if positions is not None:
         if positions.dtype not in _INDEX_BITS or positions.dim() != 3 or positions.shape[:2] != (b, h):
             raise ValueError(f"positions must be int32 or int64 of shape ({b}, {h}, n); got {positions.dtype} {tuple(positions.shape)}.")
@@ -256,21 +332,10 @@ def kv_cache_read(
             raise ValueError(f"n = {n} must lie in [0, {cap}].")
     _check_devices(key_cache.device, key_cache=key_cache, value_cache=value_cache, key_scales=key_scales,
                    value_scales=value_scales, positions=positions)
-    k_out = torch.empty((b, h, n, d), dtype=dtype, device=key_cache.device)
-    v_out = torch.empty((b, h, n, d), dtype=dtype, device=key_cache.device)
-    if k_out.numel() == 0:
-        return k_out, v_out
-    if cap == 0:
-        return k_out.zero_(), v_out.zero_()
-    index = key_cache.device.index
-    with _on_device(index):
-        rc = nat.lib.fcr_kv_read(C.byref(problem), key_cache.data_ptr(), value_cache.data_ptr(), _address(key_scales),
-                                 _address(value_scales), _address(positions),
-                                 64 if positions is None else _INDEX_BITS[positions.dtype], n, k_out.data_ptr(), v_out.data_ptr(),
-                                 _stream(index))
-        if rc:
-            nat.check(rc, "fcr_kv_read")
-    return k_out, v_out
+    hit = (problem, (b, h, n, d), dtype, 64 if positions is None else _INDEX_BITS[positions.dtype], key_cache.device)
+    if positions is given:
+        _keep(_READ_CACHE, signature, hit)
+    return hit, positions
 
 
 def tree_attention(
@@ -307,38 +372,26 @@ def tree_attention(
         (B, Hq, M, D) of ``query``'s type, and with ``return_lse`` also the fp32 (B, Hq, M) natural log-sum-exp of
         every row's scaled scores.  Run-to-run results are bitwise identical.
     """
-    _check_no_grad("tree_attention", query, key_cache, value_cache)
-    problem = _cache_problem(key_cache, value_cache, key_scales, value_scales, query.dtype)
-    b, h, n, d = key_cache.shape
-    if query.dim() != 4 or query.shape[0] != b or query.shape[3] != d or h == 0 or query.shape[1] % h:
-        raise ValueError(f"query must be ({b}, a multiple of {h}, M, {d}); got {tuple(query.shape)}.")
-    hq, m = query.shape[1], query.shape[2]
-    if m > 256:
-        raise ValueError(f"{m} drafted tokens exceed 256.")
-    if tree_mask is not None and (tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((m, m), (1, m, m), (b, m, m))):
-        raise ValueError(f"tree_mask must be bool of shape ({m}, {m}) or ({b}, {m}, {m}); got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
-    lengths = _lengths("lengths", lengths, b)
-    scale = 1 / math.sqrt(d) if scale is None else float(scale)
-    _check_devices(query.device, query=query, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
-                   tree_mask=tree_mask, key_scales=key_scales, value_scales=value_scales)
-    out = torch.empty((b, hq, m, d), dtype=query.dtype, device=query.device)
-    lse = torch.empty((b, hq, m), dtype=torch.float32, device=query.device) if return_lse else None
-    if out.numel() == 0 or n == 0:
+    if torch.is_grad_enabled():
+        _check_no_grad("tree_attention", query, key_cache, value_cache)
+    signature = (query.shape, query.stride(), query.dtype, query.get_device(), key_cache.shape, key_cache.stride(), key_cache.dtype,
+                 key_cache.get_device(), value_cache.shape, value_cache.stride(), value_cache.dtype, value_cache.get_device(), lengths.shape,
+                 lengths.is_contiguous(), lengths.dtype, lengths.get_device(), _vector_signature(tree_mask), scale, _vector_signature(key_scales),
+                 _vector_signature(value_scales))
+    hit = _TREE_CACHE.get(signature)
+    if hit is None or query.data_ptr() % 16:
+        hit, query, lengths, tree_mask = _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, scale, key_scales,
+                                                    value_scales)
+    problem, tree, shape, dtype, device, ws_bytes = hit
+    out = torch.empty(shape, dtype=dtype, device=device)
+    lse = torch.empty(shape[:3], dtype=torch.float32, device=device) if return_lse else None
+    if ws_bytes == 0:  # no rows, or no positions that they could attend
         out.zero_()
         return (out, lse.fill_(-math.inf)) if return_lse else out
-    if query.stride(3) != 1 or query.data_ptr() % 16 or any(query.shape[i] > 1 and query.stride(i) % 8 for i in range(3)):
-        query = query.clone(memory_format=torch.contiguous_format)  # the kernels copy queries 16 bytes at a time
-    tree = nat.Tree(hq, m, (*query.stride()[:3], 1), _INDEX_BITS[lengths.dtype], (0, 0), scale)
-    if tree_mask is not None:
-        tree_mask = _rows(tree_mask)
-        tree.mask_strides[:] = (tree_mask.stride(0) if tree_mask.dim() == 3 and tree_mask.shape[0] > 1 else 0, tree_mask.stride(-2))
-    index = query.device.index
+    index = device.index
     with _on_device(index):
-        ws_bytes = nat.lib.fcr_tree_workspace_bytes(C.byref(problem), C.byref(tree), 0)
-        if ws_bytes == 0:
-            raise ValueError(nat.last_error())
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device)
-        stream = _stream(index)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        stream = torch._C._cuda_getCurrentRawStream(index)
         rc = nat.lib.fcr_tree_attention(C.byref(problem), C.byref(tree), query.data_ptr(), key_cache.data_ptr(),
                                         value_cache.data_ptr(), _address(key_scales), _address(value_scales),
                                         lengths.data_ptr(), _address(tree_mask), out.data_ptr(), _address(lse), ws.data_ptr(),
@@ -350,3 +403,37 @@ def tree_attention(
         if _debug_sync() and not torch.cuda.is_current_stream_capturing():
             nat.check(nat.lib.fcr_read_device_status(ws.data_ptr(), stream, None), "fcr_tree_attention (device)")
     return (out, lse) if return_lse else out
+
+
+def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, scale, key_scales, value_scales):
+    """Checks a call of ``tree_attention`` and describes it (no workspace: nothing to compute), as ``_plan_rope`` does."""
+    problem = _cache_problem(key_cache, value_cache, key_scales, value_scales, query.dtype)
+    b, h, n, d = key_cache.shape
+    if query.dim() != 4 or query.shape[0] != b or query.shape[3] != d or h == 0 or query.shape[1] % h:
+        raise ValueError(f"query must be ({b}, a multiple of {h}, M, {d}); got {tuple(query.shape)}.")
+    hq, m = query.shape[1], query.shape[2]
+    if m > 256:
+        raise ValueError(f"{m} drafted tokens exceed 256.")
+    if tree_mask is not None and (tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((m, m), (1, m, m), (b, m, m))):
+        raise ValueError(f"tree_mask must be bool of shape ({m}, {m}) or ({b}, {m}, {m}); got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
+    given = (query, lengths, tree_mask)
+    lengths = _lengths("lengths", lengths, b)
+    scale = 1 / math.sqrt(d) if scale is None else float(scale)
+    _check_devices(query.device, query=query, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
+                   tree_mask=tree_mask, key_scales=key_scales, value_scales=value_scales)
+    if query.numel() == 0 or n == 0:
+        return (problem, None, (b, hq, m, d), query.dtype, query.device, 0), query, lengths, tree_mask
+    if query.stride(3) != 1 or query.data_ptr() % 16 or any(query.shape[i] > 1 and query.stride(i) % 8 for i in range(3)):
+        query = query.clone(memory_format=torch.contiguous_format)  # the kernels copy queries 16 bytes at a time
+    tree = nat.Tree(hq, m, (*query.stride()[:3], 1), _INDEX_BITS[lengths.dtype], (0, 0), scale)
+    if tree_mask is not None:
+        tree_mask = _rows(tree_mask)
+        tree.mask_strides[:] = (tree_mask.stride(0) if tree_mask.dim() == 3 and tree_mask.shape[0] > 1 else 0, tree_mask.stride(-2))
+    with _on_device(query.device.index):
+        ws_bytes = nat.lib.fcr_tree_workspace_bytes(C.byref(problem), C.byref(tree), 0)
+    if ws_bytes == 0:
+        raise ValueError(nat.last_error())
+    hit = (problem, tree, (b, hq, m, d), query.dtype, query.device, ws_bytes)
+    if all(x is y for x, y in zip(given, (query, lengths, tree_mask))):
+        _keep(_TREE_CACHE, signature, hit)
+    return hit, query, lengths, tree_mask
