@@ -40,6 +40,7 @@ constexpr int kTreeMmaWarp = 8;
 constexpr int kTreeQWarp = 9;         // two warps that bring the queries; for an 8-bit cache one, and one for its scales
 constexpr int kTreeLoadWarp = 11;     // TMA; for an 8-bit cache then the warps that convert codes
 constexpr int kTreeConvertWarps = 8;
+constexpr int kTreeConvertWarpsOf = kTreeConvertWarps / 2;  // for the keys, and for the values
 template <bool QUANT>
 constexpr int tree_threads() { return 32 * (kTreeLoadWarp + 1 + (QUANT ? kTreeConvertWarps : 0)); }
 
@@ -110,7 +111,7 @@ struct TreeSmem {
   static constexpr int off_codes = off_v + VS * kTileBytes;
   static constexpr int off_stat = off_codes + SS * 128 * DPAD;  // float2 [256]; PAIR keeps none, scale bytes then lie there
   static constexpr int off_scales = PAIR ? off_stat : off_stat + 2048;
-  static constexpr int off_bars = off_stat + 2048 + (PAIR || !QUANT ? 0 : 512);
+  static constexpr int off_bars = off_stat + 2048 + (PAIR || !QUANT ? 0 : 520);
   static constexpr int kNumBars = 4 + 2 * KS + 2 * VS + 2 + 2 + 2 + 1 + (QUANT ? 2 * SS + 4 : 0);
   static constexpr int off_misc = off_bars + 8 * kNumBars;
   static constexpr int kDynamicBytes = off_misc + 48;
@@ -275,8 +276,8 @@ __device__ __forceinline__ void tree_clean_values(uint32_t tile, int row, int n,
 }
 
 // The rings of key and value tiles in shared memory (swizzled 16-bit tiles of 128 keys) and their barriers; for an 8-bit cache
-// also the rings of codes (key and value tiles in turn, slabs of 64 bytes by 128 rows) and of scale bytes (two batches of two tiles: 128
-// keys, then 128 values, per tile) that the tiles are made from.
+// also the rings of codes (key and value tiles in turn, slabs of 64 bytes by 128 rows) and of scale bytes (two batches of SB tiles: 128
+// keys, then 128 values, per tile; then a byte per tile and kind: are all scales ordinary?) that the tiles are made from.
 struct TreeRing {
   uint32_t k, v;
   uint32_t bar_k_full, bar_k_empty, bar_v_full, bar_v_empty;
@@ -356,9 +357,9 @@ __device__ __forceinline__ void tree_tma_codes(const TreeParams& p, const TreeRi
   }
 }
 
-// One warp: the scale bytes, two tiles at a time so that their loads' latencies overlap.  They may lie anywhere, at any
-// stride, so plain loads bring them.  After each two tiles `also(tiles so far)` may do other work; it returns whether to go on.
-template <typename Also>
+// One warp: the scale bytes, SB tiles at a time so that their loads' latencies overlap.  They may lie anywhere, at any
+// stride, so plain loads bring them.  After each batch `also(tiles so far)` may do other work; it returns whether to go on.
+template <int SB, typename Also>
 __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int lane,
                                                  volatile int* abort_flag, Also also) {
   TreeSegment seg{};
@@ -366,9 +367,9 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
   bool more = walk.next(seg);
   if (more) t = seg.lo;
   for (uint32_t batch = 0; more; ++batch) {
-    uint32_t byte[2][8];
+    uint32_t byte[SB][8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < SB; ++i) {
       const int h = more ? seg.group / p.row_tiles : 0;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
@@ -387,95 +388,124 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
     const uint32_t buf = batch & 1u;
     if (!WAIT_BEHIND(r.bar_sc_empty + 8u * buf, ((batch >> 1) & 1u) ^ 1u, ST_TR_WAIT_SC_EMPTY)) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < SB; ++i) {
+      const uint32_t at = SB * buf + i;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ptx::sts8(r.scales + buf * 512u + i * 256u + k * 32u + lane, byte[i][k]);
+      for (int k = 0; k < 8; ++k) ptx::sts8(r.scales + at * 256u + k * 32u + lane, byte[i][k]);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        bool all = true;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) all = all && tree_short_scale(byte[i][4 * kv + k]);
+        all = __all_sync(0xffffffffu, all);
+        if (lane == 0) ptx::sts8(r.scales + 512u * SB + at * 2u + kv, all ? 1u : 0u);
+      }
     }
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(r.bar_sc_full + 8u * buf);
-    if (!also(2LL * (batch + 1))) return;
+    if (!also((long long)SB * (batch + 1))) return;
   }
 }
 
 // kTreeConvertWarps warps: codes times scale in 16 bits.  `tid` counts these warps' threads.  (Loading the codes straight
 // into registers was built first: a warp's waits for a load include the younger loads behind it, so that there was
 // never more than one tile under way, and a pair of tiles took 5800 cycles.)
-template <typename T, int DPAD, int KS, int VS, int SS>
+template <typename T, int DPAD, int KS, int VS, int SS, int SB>
 __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int tid,
                                                    volatile int* abort_flag, volatile int* bad_flag) {
   constexpr uint32_t kTileBytes = 128 * DPAD * 2;
-  constexpr int kPasses = DPAD / 32;  // a warp takes 16 rows, 8 of one slab at a time
-  const int lane = tid & 31, row0 = (tid >> 5) * 16 + (lane >> 2), piece = lane & 3;
+  constexpr int kSlabs = DPAD / 64;
+  constexpr int kRows = 128 / kTreeConvertWarpsOf;  // a warp takes this many rows of each tile, eight of one slab at a time
+  const int lane = tid & 31, role = tid / 32, kv = role / kTreeConvertWarpsOf;  // half the warps take the keys, half the values
+  const int row0 = (role % kTreeConvertWarpsOf) * kRows + (lane >> 2), piece = lane & 3;
   // Eight lanes read two rows of 64 codes and write 16-byte pieces 2 * piece (then 2 * piece + 1) of two rows of opposite
   // parity: the swizzle puts them in eight different places, so neither access meets a bank twice.
   const uint32_t from = r.codes + row0 * 64 + piece * 16;
-  const uint32_t to = row0 * 128u, at0 = ((2u * piece) ^ (lane >> 2)) << 4, at1 = at0 ^ 16u;
-  uint32_t seq = 0, c_seq = 0;  // tiles so far; code tiles so far
+  const uint32_t to = (kv ? r.v : r.k) + row0 * 128u, at0 = ((2u * piece) ^ (lane >> 2)) << 4, at1 = at0 ^ 16u;
+  const uint32_t bar_full = kv ? r.bar_v_full : r.bar_k_full, bar_empty = kv ? r.bar_v_empty : r.bar_k_empty;
+  const uint32_t scales = r.scales + kv * 128u + row0;
+  static_assert(KS == VS, "the converters count both rings alike");
+  uint32_t seq = 0;  // tiles so far
   bool ok = true;
   TreeSegment seg{};
   while (ok && walk.next(seg)) {
-    for (int t = seg.lo; ok && t < seg.hi; ++t) {
+    for (int t = seg.lo; t < seg.hi; ++t, ++seq) {
       // rows from `drafted` on are drafted tokens', rows from `end` on nobody's
       const int drafted = seg.have - t * kTreeTile, end = seg.end - t * kTreeTile;
-      if ((seq & 1u) == 0) {
-        ok = WAIT(r.bar_sc_full + 8u * ((seq >> 1) & 1u), (seq >> 2) & 1u, ST_TR_WAIT_SC_FULL);
+      const uint32_t c_seq = 2u * seq + kv, c_slot = c_seq % SS, slot = seq % KS;
+      // the codes are there, the slot is free, the scales are there: asked for together, waited for in turn
+      const uint32_t bar_c = r.bar_c_full + 8u * c_slot, par_c = (c_seq / SS) & 1u;
+      const uint32_t bar_e = bar_empty + 8u * slot, par_e = ((seq / KS) & 1u) ^ 1u;
+      const uint32_t bar_sc = r.bar_sc_full + 8u * ((seq / SB) & 1u), par_sc = (seq / (2 * SB)) & 1u, sc_at = seq % (2 * SB);
+      const uint32_t now = ptx::mbar_try_wait(bar_c, par_c) & ptx::mbar_try_wait(bar_e, par_e) & ptx::mbar_try_wait(bar_sc, par_sc);
+      if (!__all_sync(0xffffffffu, now)) {
+        ok = WAIT(bar_c, par_c, ST_TR_WAIT_C_FULL) && WAIT(bar_sc, par_sc, ST_TR_WAIT_SC_FULL) &&
+             WAIT_BEHIND(bar_e, par_e, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
         if (!ok) break;
       }
-      const uint32_t scales = r.scales + (seq & 3u) * 256u + row0;
-#pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv, ++c_seq) {
-        const uint32_t c_slot = c_seq % SS;
-        ok = WAIT(r.bar_c_full + 8u * c_slot, (c_seq / SS) & 1u, ST_TR_WAIT_C_FULL);
-        if (!ok) break;
-        uint4 codes[kPasses];
-        const uint32_t scale[2] = {ptx::lds8(scales + kv * 128u), ptx::lds8(scales + kv * 128u + 8u)};
+      const uint32_t sc = scales + sc_at * 256u, src = from + c_slot * (128 * DPAD), dst = to + slot * kTileBytes;
+      // (a byte per tile and kind says whether all of its scales allow the short conversion)
+      const bool plain = ptx::lds8(r.scales + 512u * SB + sc_at * 2u + kv) != 0u;
+      constexpr int kGroups = kRows / 8;
+      uint4 codes[kGroups][kSlabs];
+      uint32_t scale[kGroups];
 #pragma unroll
-        for (int k = 0; k < kPasses; ++k) codes[k] = ptx::lds128(from + c_slot * (128 * DPAD) + (k >> 1) * 8192 + (k & 1) * 512);
-        if (end < kTreeTile) {
+      for (int k = 0; k < kGroups; ++k) {
+        scale[k] = ptx::lds8(sc + k * 8);
 #pragma unroll
-          for (int k = 0; k < kPasses; ++k)
-            if (row0 + (k & 1) * 8 >= end) codes[k] = make_uint4(0u, 0u, 0u, 0u);
-        }
-        const bool short_scale = __all_sync(0xffffffffu, tree_short_scale(scale[0]) && tree_short_scale(scale[1]));
-        if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);  // (every lane has its codes)
-        const uint32_t slots = kv ? VS : KS, slot = seq % slots;
-        ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ((seq / slots) & 1u) ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
-        if (!ok) break;
-        const uint32_t dst = (kv ? r.v : r.k) + slot * kTileBytes + to;
-        const bool plain = short_scale && !(kv == 1 && drafted < kTreeTile);
-        auto convert = [&](auto format) {
-          constexpr int kFormat = decltype(format)::value;
-          if (plain) {
+        for (int sl = 0; sl < kSlabs; ++sl) codes[k][sl] = ptx::lds128(src + sl * 8192 + k * 512);
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);  // the codes are in registers
+      if (end < kTreeTile) {
 #pragma unroll
-            for (int k = 0; k < kPasses; ++k) {
-              uint32_t o[8];
-              tree_convert16<T, kFormat>(codes[k], scale[k & 1], o);
-              const uint32_t a = dst + (k >> 1) * (128u * 128u) + (k & 1) * 1024u;
-              ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
-              ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
+        for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+          for (int sl = 0; sl < kSlabs; ++sl)
+            if (row0 + k * 8 >= end) codes[k][sl] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      const bool check = kv == 1 && drafted < kTreeTile;  // values of drafted tokens must be finite
+      auto convert = [&](auto format) {
+        constexpr int kFormat = decltype(format)::value;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+#pragma unroll
+          for (int sl = 0; sl < kSlabs; ++sl) {
+            uint32_t o[8];
+            if (plain) {
+              tree_convert16<T, kFormat>(codes[k][sl], scale[k], o);
+            } else {
+              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[k][sl].x, codes[k][sl].y), scale[k]);
+              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[k][sl].z, codes[k][sl].w), scale[k]);
             }
-          } else {  // unusual scales, or values of drafted tokens, which must be finite
-#pragma unroll
-            for (int k = 0; k < kPasses; ++k) {
-              const uint32_t a = dst + (k >> 1) * (128u * 128u) + (k & 1) * 1024u;
-              uint32_t o[8];
-              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[k].x, codes[k].y), scale[k & 1]);
-              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[k].z, codes[k].w), scale[k & 1]);
-              if (kv == 1 && row0 + (k & 1) * 8 >= drafted && clean_words<T>(o, 8)) *bad_flag = 1;
-              ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
-              ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
-            }
+            const uint32_t a = dst + sl * (128u * 128u) + k * 1024u;
+            ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
+            ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
           }
-        };
-        if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          ptx::mbar_arrive((kv ? r.bar_v_full : r.bar_k_full) + 8u * slot);
-          if (kv == 1 && (seq & 1u)) ptx::mbar_arrive(r.bar_sc_empty + 8u * ((seq >> 1) & 1u));
         }
+      };
+      if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
+      if (check) {
+        for (int k = 0; k < kGroups; ++k)
+          if (row0 + k * 8 >= drafted) {
+            for (int sl = 0; sl < kSlabs; ++sl)
+              for (uint32_t at : {at0, at1}) {
+                const uint32_t a = dst + sl * (128u * 128u) + k * 1024u + at;
+                uint32_t e[4];
+                *reinterpret_cast<uint4*>(e) = ptx::lds128(a);
+                if (clean_words<T>(e, 4)) {
+                  ptx::sts128(a, make_uint4(e[0], e[1], e[2], e[3]));
+                  *bad_flag = 1;
+                }
+              }
+          }
       }
-      if (ok) ++seq;
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        ptx::mbar_arrive(bar_full + 8u * slot);
+        if (seq % SB == SB - 1) ptx::mbar_arrive(r.bar_sc_empty + 8u * ((seq / SB) & 1u));
+      }
     }
   }
   tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
@@ -485,7 +515,7 @@ template <int SS>
 __device__ __forceinline__ void tree_init_code_bars(const TreeRing& r) {
   for (int i = 0; i < SS; ++i) {
     ptx::mbar_init(r.bar_c_full + 8u * i, 1);
-    ptx::mbar_init(r.bar_c_empty + 8u * i, kTreeConvertWarps);
+    ptx::mbar_init(r.bar_c_empty + 8u * i, kTreeConvertWarpsOf);
   }
   for (int i = 0; i < 2; ++i) {
     ptx::mbar_init(r.bar_sc_full + 8u * i, 1);
@@ -494,7 +524,7 @@ __device__ __forceinline__ void tree_init_code_bars(const TreeRing& r) {
 }
 
 // What the load warps do; `role` counts them.
-template <typename T, int DPAD, int KS, int VS, int SS, bool QUANT>
+template <typename T, int DPAD, int KS, int VS, int SS, int SB, bool QUANT>
 __device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeRing& ring, const CUtensorMap* tmap_k, const CUtensorMap* tmap_v,
                                                 const TreeWalk<TreeLengths>& walk, int role, int lane, volatile int* abort_flag,
                                                 volatile int* bad_flag) {
@@ -504,7 +534,7 @@ __device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeR
     if (role == 0)
       tree_tma_codes<DPAD, SS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
     else
-      tree_convert_tiles<T, DPAD, KS, VS, SS>(p, ring, walk, 32 * (role - 1) + lane, abort_flag, bad_flag);
+      tree_convert_tiles<T, DPAD, KS, VS, SS, SB>(p, ring, walk, 32 * (role - 1) + lane, abort_flag, bad_flag);
   }
 }
 
@@ -581,11 +611,11 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       ptx::mbar_init(bar_q_empty(i), PAIR ? 1 : kTreeSoftmaxWarps);
     }
     for (int i = 0; i < KS; ++i) {
-      ptx::mbar_init(bar_k_full(i), QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_k_full(i), QUANT ? kTreeConvertWarpsOf : 1);
       ptx::mbar_init(bar_k_empty(i), 1);
     }
     for (int i = 0; i < VS; ++i) {
-      ptx::mbar_init(bar_v_full(i), QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_v_full(i), QUANT ? kTreeConvertWarpsOf : 1);
       ptx::mbar_init(bar_v_empty(i), 1);
     }
     for (int w = 0; w < 2; ++w) {
@@ -651,7 +681,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       if (lane == 0) ptx::mbar_arrive(bar_q_full(buf));
     }
   } else if (QUANT && warp == kTreeQWarp + 1) {
-    tree_load_scales(p, ring, walk, lane, abort_flag, [](long long) { return true; });
+    tree_load_scales<1>(p, ring, walk, lane, abort_flag, [](long long) { return true; });
   } else if (warp == kTreeMmaWarp) {
     // ------------------------------------------------------------------- products
     // Step j: tile j (PAIR: tile j / 2) for warpgroup j mod 2.  S runs two steps ahead of P V, which also orders
@@ -736,7 +766,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   } else if (warp >= kTreeLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    tree_load_roles<T, DPAD, KS, VS, L::SS, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kTreeLoadWarp, lane, abort_flag, bad_flag);
+    tree_load_roles<T, DPAD, KS, VS, L::SS, 1, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kTreeLoadWarp, lane, abort_flag, bad_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int w = warp >> 2;

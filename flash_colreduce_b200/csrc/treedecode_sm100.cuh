@@ -55,7 +55,7 @@ struct DecodeSmem {
   static constexpr int off_q = off_p + kPBytes;
   static constexpr int off_codes = off_q + kQBuffers * kQBytes;
   static constexpr int off_scales = off_codes + SS * 128 * DPAD;
-  static constexpr int off_ref = off_scales + (QUANT ? 1024 : 0);  // float [4 warps][NR]: minus the reference of a row
+  static constexpr int off_ref = off_scales + (QUANT ? 1040 : 0);  // float [4 warps][NR]: minus the reference of a row
   static constexpr int off_top = off_ref + 4 * NR * 4;       // float [4 warps][NR]: maxima
   static constexpr int off_bars = off_top + 4 * NR * 4;
   static constexpr int kNumBars = 4 + 2 * KS + 2 * VS + 2 + 2 + 2 + 2 + (QUANT ? 2 * SS + 4 : 0);
@@ -146,11 +146,11 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       ptx::mbar_init(bar_vote + 8u * i, 4);
     }
     for (int i = 0; i < KS; ++i) {
-      ptx::mbar_init(bar_k_full + 8u * i, QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_k_full + 8u * i, QUANT ? kTreeConvertWarpsOf : 1);
       ptx::mbar_init(bar_k_empty + 8u * i, 1);
     }
     for (int i = 0; i < VS; ++i) {
-      ptx::mbar_init(bar_v_full + 8u * i, QUANT ? kTreeConvertWarps : 1);
+      ptx::mbar_init(bar_v_full + 8u * i, QUANT ? kTreeConvertWarpsOf : 1);
       ptx::mbar_init(bar_v_empty + 8u * i, 1);
     }
     if (QUANT) tree_init_code_bars<L::SS>(ring);
@@ -214,7 +214,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       // products of the segment before.
       TreeWalk<TreeLengths> scale_walk = walk;
       long long next_at = 0;  // first tile of the next segment whose queries are to come
-      tree_load_scales(p, ring, scale_walk, lane, abort_flag, [&](long long tiles) {
+      tree_load_scales<2>(p, ring, scale_walk, lane, abort_flag, [&](long long tiles) {
         while (next_at < tiles && walk.next(seg)) {
           next_at += seg.hi - seg.lo;
           if (!load_queries()) return false;
@@ -286,7 +286,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     }
   } else if (warp >= kLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    tree_load_roles<T, DPAD, KS, VS, L::SS, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kLoadWarp, lane, abort_flag, bad_flag);
+    tree_load_roles<T, DPAD, KS, VS, L::SS, 2, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kLoadWarp, lane, abort_flag, bad_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int wg = warp >> 2, wq = warp & 3;
@@ -329,10 +329,10 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const bool edge = (t + 1) * kTreeTile > seg.have;
+        const uint32_t bits = edge ? decode_row_bits(p, seg, t * kTreeTile + key, r0, W) : 0xffffffffu;
         auto load_scores = [&](uint32_t (&x)[W]) {
           tmem_row_ld<W>(s_addr, x);
           if (edge) {
-            const uint32_t bits = decode_row_bits(p, seg, t * kTreeTile + key, r0, W);
 #pragma unroll
             for (int e = 0; e < W; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xff800000u;
           }
