@@ -63,6 +63,32 @@ enum {
   ST_TR_WAIT_SC_FULL = 86,
 };
 
+// A bounded wait as elsewhere, but with its loop out of line.  These kernels have up to seven kinds of warps, and the code
+// that is running must fit the instruction cache: with the loops inline and the converters unrolled 44 % of its
+// requests missed, warps waited for instructions more than for anything else, and a change of a few instructions anywhere
+// moved the time of 16 x 8 heads of 4096 int8 keys between 82 and 129 us.
+__device__ __noinline__ bool tree_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, const WaitParams* p, int code, int bounds) {
+  const long long t0 = clock64();
+  while (true) {
+    if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+    const bool late = clock64() - t0 > bounds * p->wait_limit;
+    if (__any_sync(0xffffffffu, late || *abort_flag != 0)) {
+      if (late && *abort_flag == 0) {
+        *abort_flag = 1;
+        report_status(*p, code, (int)parity);
+      }
+      __syncwarp();
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool tree_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const WaitParams& p, int code, int bounds) {
+  if (__all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity))) return true;
+  return tree_wait_loop(bar, parity, abort_flag, &p, code, bounds);
+}
+#define TREE_WAIT(bar, par, code) tree_wait(bar, par, abort_flag, p, code, 1)
+#define TREE_WAIT_BEHIND(bar, par, code) tree_wait(bar, par, abort_flag, p, code, 2)
+
 struct TreeParams : WaitParams {
   const void* q;
   const void* cache[2];             // K, V
@@ -258,7 +284,7 @@ tree_pack_mask_kernel(const unsigned char* __restrict__ mask, long long stride_b
 // Pieces c0 .. c1 - 1 of row `row` (key n) of a value tile: zeros behind the last drafted token, and in place of what is not
 // finite in a drafted token's values.
 template <typename T, int DPAD>
-__device__ __forceinline__ void tree_clean_values(uint32_t tile, int row, int n, const TreeSegment& s, int c0, int c1, volatile int* bad_flag) {
+__device__ __noinline__ void tree_clean_values(uint32_t tile, int row, int n, const TreeSegment& s, int c0, int c1, volatile int* bad_flag) {
   if (n < s.have) return;
   for (int c = c0; c < c1; ++c) {
     const uint32_t a = tile + (uint32_t)(c >> 3) * (128u * 128u) + (uint32_t)row * 128u + (((uint32_t)c & 7u) ^ ((uint32_t)row & 7u)) * 16u;
@@ -290,8 +316,8 @@ template <int KS, int VS>
 __device__ __forceinline__ void tree_drain(const TreeParams& p, const TreeRing& r, uint32_t seq, bool ok, volatile int* abort_flag) {
   for (uint32_t i = 0; ok && i < (KS > VS ? KS : VS) && i < seq; ++i) {
     const uint32_t last = seq - 1 - i;
-    if (i < KS) ok = WAIT_BEHIND(r.bar_k_empty + 8u * (last % KS), (last / KS) & 1u, ST_TR_WAIT_DRAIN);
-    if (ok && i < VS) ok = WAIT_BEHIND(r.bar_v_empty + 8u * (last % VS), (last / VS) & 1u, ST_TR_WAIT_DRAIN);
+    if (i < KS) ok = TREE_WAIT_BEHIND(r.bar_k_empty + 8u * (last % KS), (last / KS) & 1u, ST_TR_WAIT_DRAIN);
+    if (ok && i < VS) ok = TREE_WAIT_BEHIND(r.bar_v_empty + 8u * (last % VS), (last / VS) & 1u, ST_TR_WAIT_DRAIN);
   }
 }
 
@@ -308,7 +334,7 @@ __device__ __forceinline__ void tree_tma_tiles(const TreeParams& p, const TreeRi
     constexpr uint32_t kSlots = kv ? VS : KS;
     const uint32_t slot = seq % kSlots, ph = (seq / kSlots) & 1u;
     const uint32_t full = (kv ? r.bar_v_full : r.bar_k_full) + 8u * slot;
-    ok = WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+    ok = TREE_WAIT_BEHIND((kv ? r.bar_v_empty : r.bar_k_empty) + 8u * slot, ph ^ 1u, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
     if (!ok) return;
     const bool left_out = blockIdx.x == 0 && !kv && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
     if (lane == 0 && !left_out) {
@@ -343,7 +369,7 @@ __device__ __forceinline__ void tree_tma_codes(const TreeParams& p, const TreeRi
     const int h = seg.group / p.row_tiles;
     for (int t2 = 2 * seg.lo; t2 < 2 * seg.hi; ++t2, ++seq) {
       const uint32_t slot = seq % SS, full = r.bar_c_full + 8u * slot;
-      ok = WAIT_BEHIND(r.bar_c_empty + 8u * slot, ((seq / SS) & 1u) ^ 1u, ST_TR_WAIT_C_EMPTY);
+      ok = TREE_WAIT_BEHIND(r.bar_c_empty + 8u * slot, ((seq / SS) & 1u) ^ 1u, ST_TR_WAIT_C_EMPTY);
       if (!ok) break;
       const bool left_out = blockIdx.x == 0 && (int)seq == p.skip_ring_load;  // self-test of the bounded waits
       if (lane == 0 && !left_out) {
@@ -386,7 +412,7 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
       }
     }
     const uint32_t buf = batch & 1u;
-    if (!WAIT_BEHIND(r.bar_sc_empty + 8u * buf, ((batch >> 1) & 1u) ^ 1u, ST_TR_WAIT_SC_EMPTY)) return;
+    if (!TREE_WAIT_BEHIND(r.bar_sc_empty + 8u * buf, ((batch >> 1) & 1u) ^ 1u, ST_TR_WAIT_SC_EMPTY)) return;
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
       const uint32_t at = SB * buf + i;
@@ -404,6 +430,23 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(r.bar_sc_full + 8u * buf);
     if (!also((long long)SB * (batch + 1))) return;
+  }
+}
+
+// Zeros in place of what is not finite in a converter's rows of drafted tokens.  Out of line: the last tiles only.
+template <typename T, int kSlabs, int kRows>
+__device__ __noinline__ void tree_clean_rows(uint32_t dst, uint32_t at0, uint32_t at1, int row0, int drafted, volatile int* bad_flag) {
+  for (int k = 0; k < kRows; k += 8) {
+    if (row0 + k < drafted) continue;
+    for (int sl = 0; sl < 2 * kSlabs; ++sl) {
+      const uint32_t a = dst + (sl >> 1) * (128u * 128u) + k * 128u + ((sl & 1) ? at1 : at0);
+      uint32_t e[4];
+      *reinterpret_cast<uint4*>(e) = ptx::lds128(a);
+      if (clean_words<T>(e, 4)) {
+        ptx::sts128(a, make_uint4(e[0], e[1], e[2], e[3]));
+        *bad_flag = 1;
+      }
+    }
   }
 }
 
@@ -439,70 +482,47 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
       const uint32_t bar_sc = r.bar_sc_full + 8u * ((seq / SB) & 1u), par_sc = (seq / (2 * SB)) & 1u, sc_at = seq % (2 * SB);
       const uint32_t now = ptx::mbar_try_wait(bar_c, par_c) & ptx::mbar_try_wait(bar_e, par_e) & ptx::mbar_try_wait(bar_sc, par_sc);
       if (!__all_sync(0xffffffffu, now)) {
-        ok = WAIT(bar_c, par_c, ST_TR_WAIT_C_FULL) && WAIT(bar_sc, par_sc, ST_TR_WAIT_SC_FULL) &&
-             WAIT_BEHIND(bar_e, par_e, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
+        ok = TREE_WAIT(bar_c, par_c, ST_TR_WAIT_C_FULL) && TREE_WAIT(bar_sc, par_sc, ST_TR_WAIT_SC_FULL) &&
+             TREE_WAIT_BEHIND(bar_e, par_e, kv ? ST_TR_WAIT_V_EMPTY : ST_TR_WAIT_K_EMPTY);
         if (!ok) break;
       }
       const uint32_t sc = scales + sc_at * 256u, src = from + c_slot * (128 * DPAD), dst = to + slot * kTileBytes;
       // (a byte per tile and kind says whether all of its scales allow the short conversion)
       const bool plain = ptx::lds8(r.scales + 512u * SB + sc_at * 2u + kv) != 0u;
-      constexpr int kGroups = kRows / 8;
-      uint4 codes[kGroups][kSlabs];
-      uint32_t scale[kGroups];
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        scale[k] = ptx::lds8(sc + k * 8);
-#pragma unroll
-        for (int sl = 0; sl < kSlabs; ++sl) codes[k][sl] = ptx::lds128(src + sl * 8192 + k * 512);
-      }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);  // the codes are in registers
-      if (end < kTreeTile) {
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k)
-#pragma unroll
-          for (int sl = 0; sl < kSlabs; ++sl)
-            if (row0 + k * 8 >= end) codes[k][sl] = make_uint4(0u, 0u, 0u, 0u);
-      }
       const bool check = kv == 1 && drafted < kTreeTile;  // values of drafted tokens must be finite
       auto convert = [&](auto format) {
         constexpr int kFormat = decltype(format)::value;
+#pragma unroll 1
+        for (int k = 0; k < kRows; k += 8) {
+          const uint32_t scale = ptx::lds8(sc + k);
+          uint4 codes[kSlabs];
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
+          for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = ptx::lds128(src + sl * 8192 + k * 64);
+          if (row0 + k >= end) {
+#pragma unroll
+            for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
           for (int sl = 0; sl < kSlabs; ++sl) {
             uint32_t o[8];
             if (plain) {
-              tree_convert16<T, kFormat>(codes[k][sl], scale[k], o);
+              tree_convert16<T, kFormat>(codes[sl], scale, o);
             } else {
-              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[k][sl].x, codes[k][sl].y), scale[k]);
-              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[k][sl].z, codes[k][sl].w), scale[k]);
+              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[sl].x, codes[sl].y), scale);
+              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[sl].z, codes[sl].w), scale);
             }
-            const uint32_t a = dst + sl * (128u * 128u) + k * 1024u;
+            const uint32_t a = dst + sl * (128u * 128u) + k * 128u;
             ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
             ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
           }
         }
       };
       if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
-      if (check) {
-        for (int k = 0; k < kGroups; ++k)
-          if (row0 + k * 8 >= drafted) {
-            for (int sl = 0; sl < kSlabs; ++sl)
-              for (uint32_t at : {at0, at1}) {
-                const uint32_t a = dst + sl * (128u * 128u) + k * 1024u + at;
-                uint32_t e[4];
-                *reinterpret_cast<uint4*>(e) = ptx::lds128(a);
-                if (clean_words<T>(e, 4)) {
-                  ptx::sts128(a, make_uint4(e[0], e[1], e[2], e[3]));
-                  *bad_flag = 1;
-                }
-              }
-          }
-      }
+      if (check) tree_clean_rows<T, kSlabs, kRows>(dst, at0, at1, row0, drafted, bad_flag);
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
+        ptx::mbar_arrive(r.bar_c_empty + 8u * c_slot);
         ptx::mbar_arrive(bar_full + 8u * slot);
         if (seq % SB == SB - 1) ptx::mbar_arrive(r.bar_sc_empty + 8u * ((seq / SB) & 1u));
       }
@@ -660,7 +680,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     uint32_t seq = 0;
     while (walk.next(seg)) {
       const uint32_t buf = seq % L::kQBuffers, ph = (seq / L::kQBuffers) & 1u;
-      if (!WAIT_BEHIND(bar_q_empty(buf), ph ^ 1u, ST_TR_WAIT_Q_EMPTY)) break;
+      if (!TREE_WAIT_BEHIND(bar_q_empty(buf), ph ^ 1u, ST_TR_WAIT_Q_EMPTY)) break;
       ++seq;
       const int kh = seg.group / p.row_tiles, r0 = (seg.group - kh * p.row_tiles) * 256;
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)kh * p.G * p.qh;
@@ -701,10 +721,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           ahead.next(sa);
           s_left = sa.hi - sa.lo;
           s_done = 0;
-          ok = WAIT(bar_q_full(q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
+          ok = TREE_WAIT(bar_q_full(q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
           if (!ok) return;
         }
-        ok = WAIT(bar_k_full(s_tile % KS), (s_tile / KS) & 1u, ST_TR_WAIT_K_FULL);
+        ok = TREE_WAIT(bar_k_full(s_tile % KS), (s_tile / KS) & 1u, ST_TR_WAIT_K_FULL);
         if (!ok) return;
       }
       ptx::tc_fence_after_sync();
@@ -741,10 +761,10 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         o_done = 0;
       }
       if (opens) {
-        ok = WAIT(bar_v_full(o_tile % VS), (o_tile / VS) & 1u, ST_TR_WAIT_V_FULL);
+        ok = TREE_WAIT(bar_v_full(o_tile % VS), (o_tile / VS) & 1u, ST_TR_WAIT_V_FULL);
         if (!ok) break;
       }
-      ok = WAIT_BEHIND(bar_p(w), (uint32_t)(j >> 1) & 1u, ST_TR_WAIT_P);
+      ok = TREE_WAIT_BEHIND(bar_p(w), (uint32_t)(j >> 1) & 1u, ST_TR_WAIT_P);
       if (!ok) break;
       ptx::tc_fence_after_sync();
       if (ptx::elect_one()) {
@@ -779,7 +799,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     auto sync_all = [&]() {  // a bounded barrier over the eight warps
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_merge);
-      ok = WAIT_BEHIND(bar_merge, merge_use & 1u, ST_TR_WAIT_MERGE);
+      ok = TREE_WAIT_BEHIND(bar_merge, merge_use & 1u, ST_TR_WAIT_MERGE);
       ++merge_use;
       return ok;
     };
@@ -793,7 +813,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       int mine = 0;  // tiles this warpgroup has taken
       for (int t = seg.lo; t < seg.hi; ++t, ++tile_seq) {
         if (!PAIR && (int)(tile_seq & 1u) != w) continue;
-        ok = WAIT(bar_s(w), s_use & 1u, ST_TR_WAIT_S);
+        ok = TREE_WAIT(bar_s(w), s_use & 1u, ST_TR_WAIT_S);
         if (!ok) break;
         ++s_use;
         ptx::tc_fence_after_sync();
@@ -872,7 +892,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         if (!QUANT && edge) {
           // values behind the last drafted token become zeros, and non-finite ones of the drafted tokens
           const uint32_t slot = tile_seq % VS;
-          ok = WAIT(bar_v_full(slot), (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
+          ok = TREE_WAIT(bar_v_full(slot), (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
           if (!ok) break;
           // (PAIR: each warpgroup takes half of the 16-byte pieces)
           constexpr int kPieces = PAIR ? DPAD / 16 : DPAD / 8;
@@ -888,7 +908,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       if (!ok) break;
       // ------------------------------------------------ the segment's results
       if (mine > 0) {
-        ok = WAIT(bar_o(w), o_use & 1u, ST_TR_WAIT_O);
+        ok = TREE_WAIT(bar_o(w), o_use & 1u, ST_TR_WAIT_O);
         if (!ok) break;
         ++o_use;
         ptx::tc_fence_after_sync();

@@ -187,7 +187,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     uint32_t seq = 0;
     auto load_queries = [&]() {
       const uint32_t buf = seq % L::kQBuffers;
-      if (!WAIT_BEHIND(bar_q_empty + 8u * buf, ((seq / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
+      if (!TREE_WAIT_BEHIND(bar_q_empty + 8u * buf, ((seq / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
       ++seq;
       const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)seg.group * p.G * p.qh;
       const uint32_t dst = base + L::off_q + buf * L::kQBytes;
@@ -232,13 +232,13 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     uint32_t tile = 0, q_seq = 0;
     bool ok = true;
     while (ok && walk.next(seg)) {
-      ok = WAIT(bar_q_full + 8u * (q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
+      ok = TREE_WAIT(bar_q_full + 8u * (q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
       const uint32_t b_lo = ptx::smem_desc_lo(base + L::off_q + (q_seq % L::kQBuffers) * L::kQBytes);
       for (int t = seg.lo; ok && t < seg.hi; ++t, ++tile) {
         const uint32_t buf = tile & 1u, slot = tile % KS;
-        ok = WAIT(bar_k_full + 8u * slot, (tile / KS) & 1u, ST_TR_WAIT_K_FULL);
+        ok = TREE_WAIT(bar_k_full + 8u * slot, (tile / KS) & 1u, ST_TR_WAIT_K_FULL);
         if (!ok) break;
-        if (tile >= 2) ok = WAIT_BEHIND(bar_p + 8u * buf, ((tile - 2u) >> 1) & 1u, ST_TR_WAIT_P);
+        if (tile >= 2) ok = TREE_WAIT_BEHIND(bar_p + 8u * buf, ((tile - 2u) >> 1) & 1u, ST_TR_WAIT_P);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         if (ptx::elect_one()) {
@@ -266,9 +266,9 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     while (ok && walk.next(seg)) {
       for (int t = seg.lo; ok && t < seg.hi; ++t, ++tile) {
         const uint32_t buf = tile & 1u, slot = tile % VS;
-        ok = WAIT(bar_v_full + 8u * slot, (tile / VS) & 1u, ST_TR_WAIT_V_FULL);
+        ok = TREE_WAIT(bar_v_full + 8u * slot, (tile / VS) & 1u, ST_TR_WAIT_V_FULL);
         if (!ok) break;
-        ok = WAIT_BEHIND(bar_p + 8u * buf, (tile >> 1) & 1u, ST_TR_WAIT_P);
+        ok = TREE_WAIT_BEHIND(bar_p + 8u * buf, (tile >> 1) & 1u, ST_TR_WAIT_P);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         if (ptx::elect_one()) {
@@ -304,14 +304,14 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     auto sync_group = [&]() {  // a bounded barrier over the warpgroup
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(vote_bar);
-      ok = WAIT_BEHIND(vote_bar, votes & 1u, ST_TD_WAIT_VOTE);
+      ok = TREE_WAIT_BEHIND(vote_bar, votes & 1u, ST_TD_WAIT_VOTE);
       ++votes;
       return ok;
     };
     // The product of tile `i`, at most the one before the last whose weights have been made: every product is waited for in
     // turn (tile j's weights overwrite tile j - 2's), so that no parity can be mistaken for an older phase's.
     auto wait_pv = [&](uint32_t i, int code) {
-      ok = WAIT(bar_pv + 8u * (i & 1u), (i >> 1) & 1u, code);
+      ok = TREE_WAIT(bar_pv + 8u * (i & 1u), (i >> 1) & 1u, code);
       if (ok) ptx::tc_fence_after_sync();
       return ok;
     };
@@ -325,7 +325,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       for (int t = seg.lo; t < seg.hi; ++t, ++tile_seq) {
         const uint32_t buf = tile_seq & 1u;
         const uint32_t s_addr = tmem_base + lanes + buf * NR + r0;
-        ok = WAIT(bar_s + 8u * buf, (tile_seq >> 1) & 1u, ST_TR_WAIT_S);
+        ok = TREE_WAIT(bar_s + 8u * buf, (tile_seq >> 1) & 1u, ST_TR_WAIT_S);
         if (!ok) break;
         ptx::tc_fence_after_sync();
         const bool edge = (t + 1) * kTreeTile > seg.have;
@@ -403,7 +403,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         }
         if (!QUANT && edge) {
           const uint32_t slot = tile_seq % VS;
-          ok = WAIT(bar_v_full + 8u * slot, (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
+          ok = TREE_WAIT(bar_v_full + 8u * slot, (tile_seq / VS) & 1u, ST_TR_WAIT_V_FULL_SM);
           if (!ok) break;
           constexpr int kPieces = DPAD / 8 / kGroups;  // each warpgroup takes its share of the 16-byte pieces
           tree_clean_values<T, DPAD>(base + L::off_v + slot * L::kTileBytes, key, t * kTreeTile + key, seg, wg * kPieces, (wg + 1) * kPieces, bad_flag);
