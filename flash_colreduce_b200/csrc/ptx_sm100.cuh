@@ -180,6 +180,20 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "n"(ACCUMULATE ? 1 : 0)
       : "memory");
 }
+// The same with the choice at run time, for a rolled loop.
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t"
+      "}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(kDescHi), "r"((uint32_t)accumulate)
+      : "memory");
+}
 // Same for fp32 operands taken as TF32 (K = 8 per instruction: again 32 bytes of each row).
 template <bool ACCUMULATE>
 __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {

@@ -86,7 +86,7 @@ __device__ __forceinline__ void tmem_row_st(uint32_t taddr, const uint32_t (&r)[
 }
 
 // Bits of the rows r0 .. r0 + width - 1 that attend key n; what it says of rows beyond the last one does not matter.
-__device__ __forceinline__ uint32_t decode_row_bits(const TreeParams& p, const TreeSegment& s, int n, int r0, int width) {
+__device__ __noinline__ uint32_t decode_row_bits(const TreeParams& p, const TreeSegment& s, int n, int r0, int width) {
   if (n < s.have) return 0xffffffffu;
   if (n >= s.end) return 0u;
   const int j = n - s.have;
@@ -277,7 +277,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           const uint32_t d = tmem_base + 2 * NR;
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)  // 16 keys: 2048 bytes of either operand
-            ptx::umma_step<false>(d, a_lo + kk * (2048u >> 4), b_lo + kk * (2048u >> 4), p.idesc_o, t == seg.lo && kk == 0);
+            ptx::umma_f16(d, a_lo + kk * (2048u >> 4), b_lo + kk * (2048u >> 4), p.idesc_o, t > seg.lo || kk > 0);
           ptx::umma_commit(bar_pv + 8u * buf);
           ptx::umma_commit(bar_v_empty + 8u * slot);
         }
@@ -413,7 +413,10 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(bar_p + 8u * buf);
 #pragma unroll
-        for (int e = 0; e < W; ++e) l[e] += w[e];
+        for (int e = 0; e < W; e += 2) {
+          const float2 sum = __fadd2_rn(make_float2(l[e], l[e + 1]), make_float2(w[e], w[e + 1]));
+          l[e] = sum.x, l[e + 1] = sum.y;
+        }
       }
       if (!ok) break;
       // ------------------------------------------------ the segment's results
