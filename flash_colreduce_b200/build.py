@@ -37,7 +37,6 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC", "-ldl",
-    "--split-compile=0",  # the many kernel instantiations are optimised on all cores
 ]
 
 

@@ -211,32 +211,40 @@ static int launch_tree_kernel(void (*kern)(const CUtensorMap, const CUtensorMap,
   }
   return FCR_OK;
 }
-template <typename T, int DPAD, bool PAIR, bool QUANT>
+template <typename T, int DPAD, bool PAIR, int FORMAT>
 static int launch_tree_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
-  return launch_tree_kernel<T, DPAD>(tree_attention_kernel<T, DPAD, PAIR, QUANT>, TreeSmem<DPAD, PAIR, QUANT>::kDynamicBytes, tree_threads<QUANT>(),
+  constexpr bool kQuant = FORMAT != FCR_KV_16BIT;
+  return launch_tree_kernel<T, DPAD>(tree_attention_kernel<T, DPAD, PAIR, FORMAT>, TreeSmem<DPAD, PAIR, kQuant>::kDynamicBytes, tree_threads<kQuant>(),
                                      opted_in, map_k, map_v, p, pl, stream);
 }
-template <typename T, int DPAD, int NR, bool QUANT>
+template <typename T, int DPAD, int NR, int FORMAT>
 static int launch_tree_keys(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
   static std::atomic<unsigned long long> opted_in{0};
-  return launch_tree_kernel<T, DPAD>(tree_decode_kernel<T, DPAD, NR, QUANT>, DecodeSmem<DPAD, NR, QUANT>::kDynamicBytes, decode_threads<NR, QUANT>(),
+  constexpr bool kQuant = FORMAT != FCR_KV_16BIT;
+  return launch_tree_kernel<T, DPAD>(tree_decode_kernel<T, DPAD, NR, FORMAT>, DecodeSmem<DPAD, NR, kQuant>::kDynamicBytes, decode_threads<NR, kQuant>(),
                                      opted_in,
                                      map_k, map_v, p, pl, stream);
 }
-template <typename T, int DPAD, bool QUANT>
+template <typename T, int DPAD, int FORMAT>
 static int launch_tree(const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl, cudaStream_t stream) {
-  if (pl.pair) return launch_tree_rows<T, DPAD, true, QUANT>(map_k, map_v, p, pl, stream);
-  if (pl.decode_rows == 0) return launch_tree_rows<T, DPAD, false, QUANT>(map_k, map_v, p, pl, stream);
-  if (pl.decode_rows == 16) return launch_tree_keys<T, DPAD, 16, QUANT>(map_k, map_v, p, pl, stream);
-  if (pl.decode_rows == 32) return launch_tree_keys<T, DPAD, 32, QUANT>(map_k, map_v, p, pl, stream);
-  return launch_tree_keys<T, DPAD, 64, QUANT>(map_k, map_v, p, pl, stream);
+  if (pl.pair) return launch_tree_rows<T, DPAD, true, FORMAT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 0) return launch_tree_rows<T, DPAD, false, FORMAT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 16) return launch_tree_keys<T, DPAD, 16, FORMAT>(map_k, map_v, p, pl, stream);
+  if (pl.decode_rows == 32) return launch_tree_keys<T, DPAD, 32, FORMAT>(map_k, map_v, p, pl, stream);
+  return launch_tree_keys<T, DPAD, 64, FORMAT>(map_k, map_v, p, pl, stream);
+}
+template <typename T, int DPAD>
+static int launch_tree_f(int format, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
+                         cudaStream_t stream) {
+  if (format == FCR_KV_FP8) return launch_tree<T, DPAD, FCR_KV_FP8>(map_k, map_v, p, pl, stream);
+  if (format == FCR_KV_INT8) return launch_tree<T, DPAD, FCR_KV_INT8>(map_k, map_v, p, pl, stream);
+  return launch_tree<T, DPAD, FCR_KV_16BIT>(map_k, map_v, p, pl, stream);
 }
 template <typename T>
-static int launch_tree_d(int d_pad, bool quant, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
+static int launch_tree_d(int d_pad, int format, const CUtensorMap& map_k, const CUtensorMap& map_v, const TreeParams& p, const TreePlan& pl,
                          cudaStream_t stream) {
-  if (d_pad == 64) return quant ? launch_tree<T, 64, true>(map_k, map_v, p, pl, stream) : launch_tree<T, 64, false>(map_k, map_v, p, pl, stream);
-  return quant ? launch_tree<T, 128, true>(map_k, map_v, p, pl, stream) : launch_tree<T, 128, false>(map_k, map_v, p, pl, stream);
+  return d_pad == 64 ? launch_tree_f<T, 64>(format, map_k, map_v, p, pl, stream) : launch_tree_f<T, 128>(format, map_k, map_v, p, pl, stream);
 }
 
 }  // namespace fcr
@@ -505,7 +513,6 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.words = pl.words;
   p.mask_shared = t.mask_strides[0] == 0;
   p.index_bits = t.index_bits;
-  p.format = c.format;
   float s2 = fabsf(t.scale) * 1.4426950408889634f;
   if (!(s2 >= 1e-30f)) s2 = 1e-30f;  // scale 0: every score becomes (numerically) zero
   p.scale2 = s2;
@@ -543,8 +550,8 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
     if (e == cudaSuccess) e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "mask packing launch");
   }
-  return c.dtype == FCR_F16 ? launch_tree_d<__half>(pl.d_pad, quant, map_k, map_v, p, pl, stream)
-                            : launch_tree_d<__nv_bfloat16>(pl.d_pad, quant, map_k, map_v, p, pl, stream);
+  return c.dtype == FCR_F16 ? launch_tree_d<__half>(pl.d_pad, c.format, map_k, map_v, p, pl, stream)
+                            : launch_tree_d<__nv_bfloat16>(pl.d_pad, c.format, map_k, map_v, p, pl, stream);
 }
 
 }  // extern "C"

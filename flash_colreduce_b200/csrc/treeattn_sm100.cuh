@@ -36,13 +36,16 @@ namespace fcr {
 
 constexpr int kTreeMaxM = 256;
 constexpr int kTreeSoftmaxWarps = 8;  // two warpgroups
-constexpr int kTreeMmaWarp = 8;
-constexpr int kTreeQWarp = 9;         // two warps that bring the queries; for an 8-bit cache one, and one for its scales
-constexpr int kTreeLoadWarp = 11;     // TMA; for an 8-bit cache then the warps that convert codes
+constexpr int kTreeMmaWarp = 8;       // two warps, one per warpgroup
+constexpr int kTreeQWarp = 10;        // first of those that bring the queries
+template <bool QUANT>
+constexpr int kTreeQWarps = QUANT ? 1 : 4;  // with an 8-bit cache one, which brings its scales too
+template <bool QUANT>
+constexpr int kTreeLoadWarp = kTreeQWarp + kTreeQWarps<QUANT>;  // TMA; for an 8-bit cache then the warps that convert codes
 constexpr int kTreeConvertWarps = 8;
 constexpr int kTreeConvertWarpsOf = kTreeConvertWarps / 2;  // for the keys, and for the values
 template <bool QUANT>
-constexpr int tree_threads() { return 32 * (kTreeLoadWarp + 1 + (QUANT ? kTreeConvertWarps : 0)); }
+constexpr int tree_threads() { return 32 * (kTreeLoadWarp<QUANT> + 1 + (QUANT ? kTreeConvertWarps : 0)); }
 
 enum {
   ST_TR_WAIT_Q_EMPTY = 71,
@@ -106,7 +109,7 @@ struct TreeParams : WaitParams {
   int row_tiles, groups;            // groups = Hk * row_tiles
   int part_rows;
   int words, mask_shared;
-  int index_bits, format;
+  int index_bits;
   float scale2;                     // |scale| * log2(e)
   uint32_t idesc_s, idesc_o;
   int k_steps;                      // 32-byte steps of a key row that hold data
@@ -128,9 +131,12 @@ struct TreeSmem {
   static constexpr int kQBuffers = PAIR ? 1 : 2;
   // a query buffer doubles as the space in which the two warpgroups merge: 256 lanes x 32 columns of fp32
   static constexpr int kQBytes = PAIR ? 2 * kTileBytes : 32768;
-  static constexpr int KS = DPAD == 64 ? (QUANT ? 3 : 5) : (QUANT ? 2 : 3);  // key and value tiles in flight
-  static constexpr int VS = DPAD == 64 ? (QUANT ? 3 : 4) : 2;
-  static constexpr int SS = QUANT ? (DPAD == 64 ? 5 : 2) : 0;               // tiles of codes in flight
+  // Key and value tiles in flight.  Where the warpgroups take turns the numbers are even: a slot then always belongs to the
+  // same warpgroup, which sees every phase of its barriers.
+  static constexpr int KS = DPAD == 64 ? (QUANT ? 2 : 4) : (QUANT || !PAIR ? 2 : 3);
+  static constexpr int VS = DPAD == 64 ? (QUANT ? 2 : 4) : 2;
+  static constexpr int SS = QUANT ? (DPAD == 64 ? 8 : 2) : 0;               // tiles of codes in flight
+  static_assert(PAIR || (KS % 2 == 0 && VS % 2 == 0), "see above");
   static constexpr int off_q = 0;
   static constexpr int off_k = off_q + kQBuffers * kQBytes;
   static constexpr int off_v = off_k + KS * kTileBytes;
@@ -237,14 +243,14 @@ __device__ __forceinline__ bool clean_words(uint32_t* e, int n) {
 }
 
 // The values of a drafted token that the product left out because they are not finite; 0 for a finite one.
-template <typename T, bool QUANT>
+template <typename T, int FORMAT>
 __device__ __forceinline__ float tree_non_finite(const TreeParams& p, int b, int h, int n, int d) {
   const long long at = b * p.cb[1] + h * p.ch[1] + n * p.cn[1] + d;
   float v;
-  if (QUANT) {
+  if (FORMAT != FCR_KV_16BIT) {
     float c[4];
     const uint32_t byte = reinterpret_cast<const unsigned char*>(p.cache[1])[at];
-    if (p.format == FCR_KV_FP8) unpack_codes4<FCR_KV_FP8>(byte, c); else unpack_codes4<FCR_KV_INT8>(byte, c);
+    unpack_codes4<FORMAT>(byte, c);
     v = c[0] * kv_scale(p.scales[1][b * p.sb[1] + h * p.sh[1] + n * p.sn[1]]);
   } else {
     v = to_f32(reinterpret_cast<const T*>(p.cache[1])[at]);
@@ -252,7 +258,7 @@ __device__ __forceinline__ float tree_non_finite(const TreeParams& p, int b, int
   v = to_f32(from_f32<T>(v));  // as the product would have had it
   return fabsf(v) < INFINITY ? 0.f : v;
 }
-template <typename T, bool QUANT>
+template <typename T, int FORMAT>
 __device__ __noinline__ void tree_add_non_finite(const TreeParams& p, const TreeSegment& s, const uint32_t* words, int m, int d0, int nd,
                                                  float* o) {
   const int h = s.group / p.row_tiles;
@@ -260,7 +266,7 @@ __device__ __noinline__ void tree_add_non_finite(const TreeParams& p, const Tree
   for (int n = max(s.have, s.lo * kTreeTile); n < hi; ++n) {
     const int j = n - s.have;
     if (words ? !(words[j >> 5] >> (j & 31) & 1u) : j > m) continue;
-    for (int d = 0; d < nd && d0 + d < p.D; ++d) o[d] += tree_non_finite<T, QUANT>(p, s.b, h, n, d0 + d);
+    for (int d = 0; d < nd && d0 + d < p.D; ++d) o[d] += tree_non_finite<T, FORMAT>(p, s.b, h, n, d0 + d);
   }
 }
 
@@ -393,18 +399,25 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
   bool more = walk.next(seg);
   if (more) t = seg.lo;
   for (uint32_t batch = 0; more; ++batch) {
-    uint32_t byte[SB][8];
+    uint32_t word[SB][2];  // a lane has four neighbouring keys
+    bool all[SB][2];
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
-      const int h = more ? seg.group / p.row_tiles : 0;
+      const int h = more ? seg.group / p.row_tiles : 0, n0 = t * kTreeTile + 4 * lane;
+      const int upto = more ? seg.end - n0 : 0;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const unsigned char* src = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv];
+        const long long step = p.sn[kv];
+        const unsigned char* src = p.scales[kv] + seg.b * p.sb[kv] + h * p.sh[kv] + n0 * step;
+        uint32_t byte[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const long long n = t * kTreeTile + k * 32 + lane;
-          byte[i][4 * kv + k] = more && n < seg.end ? src[n * p.sn[kv]] : 127u;
+          byte[k] = 127u;
+          if (k < upto) byte[k] = *src;
+          src += step;
         }
+        word[i][kv] = byte[0] | byte[1] << 8 | byte[2] << 16 | byte[3] << 24;
+        all[i][kv] = tree_short_scale(byte[0]) && tree_short_scale(byte[1]) && tree_short_scale(byte[2]) && tree_short_scale(byte[3]);
       }
       if (more && ++t == seg.hi) {
         more = walk.next(seg);
@@ -417,14 +430,10 @@ __device__ __forceinline__ void tree_load_scales(const TreeParams& p, const Tree
     for (int i = 0; i < SB; ++i) {
       const uint32_t at = SB * buf + i;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ptx::sts8(r.scales + at * 256u + k * 32u + lane, byte[i][k]);
-#pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        bool all = true;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) all = all && tree_short_scale(byte[i][4 * kv + k]);
-        all = __all_sync(0xffffffffu, all);
-        if (lane == 0) ptx::sts8(r.scales + 512u * SB + at * 2u + kv, all ? 1u : 0u);
+        ptx::sts32(r.scales + at * 256u + kv * 128u + 4u * lane, word[i][kv]);
+        const uint32_t ordinary = __all_sync(0xffffffffu, all[i][kv]) ? 1u : 0u;
+        if (lane == 0) ptx::sts8(r.scales + 512u * SB + at * 2u + kv, ordinary);
       }
     }
     __syncwarp();
@@ -453,7 +462,7 @@ __device__ __noinline__ void tree_clean_rows(uint32_t dst, uint32_t at0, uint32_
 // kTreeConvertWarps warps: codes times scale in 16 bits.  `tid` counts these warps' threads.  (Loading the codes straight
 // into registers was built first: a warp's waits for a load include the younger loads behind it, so that there was
 // never more than one tile under way, and a pair of tiles took 5800 cycles.)
-template <typename T, int DPAD, int KS, int VS, int SS, int SB>
+template <typename T, int FORMAT, int DPAD, int KS, int VS, int SS, int SB>
 __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const TreeRing& r, TreeWalk<TreeLengths> walk, int tid,
                                                    volatile int* abort_flag, volatile int* bad_flag) {
   constexpr uint32_t kTileBytes = 128 * DPAD * 2;
@@ -467,7 +476,6 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
   const uint32_t to = (kv ? r.v : r.k) + row0 * 128u, at0 = ((2u * piece) ^ (lane >> 2)) << 4, at1 = at0 ^ 16u;
   const uint32_t bar_full = kv ? r.bar_v_full : r.bar_k_full, bar_empty = kv ? r.bar_v_empty : r.bar_k_empty;
   const uint32_t scales = r.scales + kv * 128u + row0;
-  static_assert(KS == VS, "the converters count both rings alike");
   uint32_t seq = 0;  // tiles so far
   bool ok = true;
   TreeSegment seg{};
@@ -475,10 +483,11 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
     for (int t = seg.lo; t < seg.hi; ++t, ++seq) {
       // rows from `drafted` on are drafted tokens', rows from `end` on nobody's
       const int drafted = seg.have - t * kTreeTile, end = seg.end - t * kTreeTile;
-      const uint32_t c_seq = 2u * seq + kv, c_slot = c_seq % SS, slot = seq % KS;
+      const uint32_t c_seq = 2u * seq + kv, c_slot = c_seq % SS;
+      const uint32_t slot = kv ? seq % VS : seq % KS, use = kv ? seq / VS : seq / KS;
       // the codes are there, the slot is free, the scales are there: asked for together, waited for in turn
       const uint32_t bar_c = r.bar_c_full + 8u * c_slot, par_c = (c_seq / SS) & 1u;
-      const uint32_t bar_e = bar_empty + 8u * slot, par_e = ((seq / KS) & 1u) ^ 1u;
+      const uint32_t bar_e = bar_empty + 8u * slot, par_e = (use & 1u) ^ 1u;
       const uint32_t bar_sc = r.bar_sc_full + 8u * ((seq / SB) & 1u), par_sc = (seq / (2 * SB)) & 1u, sc_at = seq % (2 * SB);
       const uint32_t now = ptx::mbar_try_wait(bar_c, par_c) & ptx::mbar_try_wait(bar_e, par_e) & ptx::mbar_try_wait(bar_sc, par_sc);
       if (!__all_sync(0xffffffffu, now)) {
@@ -490,34 +499,30 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
       // (a byte per tile and kind says whether all of its scales allow the short conversion)
       const bool plain = ptx::lds8(r.scales + 512u * SB + sc_at * 2u + kv) != 0u;
       const bool check = kv == 1 && drafted < kTreeTile;  // values of drafted tokens must be finite
-      auto convert = [&](auto format) {
-        constexpr int kFormat = decltype(format)::value;
 #pragma unroll 1
-        for (int k = 0; k < kRows; k += 8) {
-          const uint32_t scale = ptx::lds8(sc + k);
-          uint4 codes[kSlabs];
+      for (int k = 0; k < kRows; k += 8) {
+        const uint32_t scale = ptx::lds8(sc + k);
+        uint4 codes[kSlabs];
 #pragma unroll
-          for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = ptx::lds128(src + sl * 8192 + k * 64);
-          if (row0 + k >= end) {
+        for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = ptx::lds128(src + sl * 8192 + k * 64);
+        if (row0 + k >= end) {
 #pragma unroll
-            for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = make_uint4(0u, 0u, 0u, 0u);
-          }
-#pragma unroll
-          for (int sl = 0; sl < kSlabs; ++sl) {
-            uint32_t o[8];
-            if (plain) {
-              tree_convert16<T, kFormat>(codes[sl], scale, o);
-            } else {
-              *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, kFormat>(make_uint2(codes[sl].x, codes[sl].y), scale);
-              *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, kFormat>(make_uint2(codes[sl].z, codes[sl].w), scale);
-            }
-            const uint32_t a = dst + sl * (128u * 128u) + k * 128u;
-            ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
-            ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
-          }
+          for (int sl = 0; sl < kSlabs; ++sl) codes[sl] = make_uint4(0u, 0u, 0u, 0u);
         }
-      };
-      if (p.format == FCR_KV_FP8) convert(std::integral_constant<int, FCR_KV_FP8>{}); else convert(std::integral_constant<int, FCR_KV_INT8>{});
+#pragma unroll
+        for (int sl = 0; sl < kSlabs; ++sl) {
+          uint32_t o[8];
+          if (plain) {
+            tree_convert16<T, FORMAT>(codes[sl], scale, o);
+          } else {
+            *reinterpret_cast<uint4*>(o) = tree_convert8_any<T, FORMAT>(make_uint2(codes[sl].x, codes[sl].y), scale);
+            *reinterpret_cast<uint4*>(o + 4) = tree_convert8_any<T, FORMAT>(make_uint2(codes[sl].z, codes[sl].w), scale);
+          }
+          const uint32_t a = dst + sl * (128u * 128u) + k * 128u;
+          ptx::sts128(a + at0, make_uint4(o[0], o[1], o[2], o[3]));
+          ptx::sts128(a + at1, make_uint4(o[4], o[5], o[6], o[7]));
+        }
+      }
       if (check) tree_clean_rows<T, kSlabs, kRows>(dst, at0, at1, row0, drafted, bad_flag);
       ptx::fence_proxy_async_smem();
       __syncwarp();
@@ -529,6 +534,30 @@ __device__ __forceinline__ void tree_convert_tiles(const TreeParams& p, const Tr
     }
   }
   tree_drain<KS, VS>(p, r, seq, ok, abort_flag);
+}
+
+// The query warp: load(segment, its number) brings a segment's queries.  With an 8-bit cache it also brings the scales; a segment's queries
+// follow the scales of its first tiles, which never wait for queries, while those may wait for the products of the segment before.
+template <int SB, bool QUANT, typename Load>
+__device__ __forceinline__ void tree_query_role(const TreeParams& p, const TreeRing& ring, TreeWalk<TreeLengths> walk, int lane,
+                                                volatile int* abort_flag, Load load) {
+  uint32_t number = 0;
+  if constexpr (QUANT) {
+    TreeWalk<TreeLengths> scale_walk = walk;
+    long long next_at = 0;  // first tile of the next segment whose queries are to come
+    tree_load_scales<SB>(p, ring, scale_walk, lane, abort_flag, [&](long long tiles) {
+      while (next_at < tiles) {
+        TreeSegment s;
+        if (!walk.next(s)) return true;
+        next_at += s.hi - s.lo;
+        if (!load(s, number++)) return false;
+      }
+      return true;
+    });
+  } else {
+    TreeSegment s;
+    while (walk.next(s) && load(s, number)) ++number;
+  }
 }
 
 template <int SS>
@@ -544,17 +573,17 @@ __device__ __forceinline__ void tree_init_code_bars(const TreeRing& r) {
 }
 
 // What the load warps do; `role` counts them.
-template <typename T, int DPAD, int KS, int VS, int SS, int SB, bool QUANT>
+template <typename T, int DPAD, int KS, int VS, int SS, int SB, int FORMAT>
 __device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeRing& ring, const CUtensorMap* tmap_k, const CUtensorMap* tmap_v,
                                                 const TreeWalk<TreeLengths>& walk, int role, int lane, volatile int* abort_flag,
                                                 volatile int* bad_flag) {
-  if constexpr (!QUANT) {
+  if constexpr (FORMAT == FCR_KV_16BIT) {
     tree_tma_tiles<DPAD, KS, VS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
   } else {
     if (role == 0)
       tree_tma_codes<DPAD, SS>(p, ring, tmap_k, tmap_v, walk, lane, abort_flag);
     else
-      tree_convert_tiles<T, DPAD, KS, VS, SS, SB>(p, ring, walk, 32 * (role - 1) + lane, abort_flag, bad_flag);
+      tree_convert_tiles<T, FORMAT, DPAD, KS, VS, SS, SB>(p, ring, walk, 32 * (role - 1) + lane, abort_flag, bad_flag);
   }
 }
 
@@ -588,13 +617,13 @@ __device__ __forceinline__ void tree_find_piece(const TreeParams& p, const TreeL
   if (lane == 0) *start_n = hi - lo;
 }
 
-template <typename T, int DPAD, bool PAIR, bool QUANT>
-__global__ void __launch_bounds__(tree_threads<QUANT>(), 1)
+template <typename T, int DPAD, bool PAIR, int FORMAT>
+__global__ void __launch_bounds__(tree_threads<FORMAT != FCR_KV_16BIT>(), 1)
 tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ TreeParams p) {
+  constexpr bool QUANT = FORMAT != FCR_KV_16BIT;
   using L = TreeSmem<DPAD, PAIR, QUANT>;
-  constexpr int KS = L::KS, VS = L::VS;
-  constexpr int kTreeQWarps = QUANT ? 1 : 2;
+  constexpr int KS = L::KS, VS = L::VS, kLoadWarp = kTreeLoadWarp<QUANT>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = ptx::smem_u32(smem);
   if ((base & 1023u) != 0) {
@@ -627,16 +656,16 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kQBuffers; ++i) {
-      ptx::mbar_init(bar_q_full(i), kTreeQWarps);
-      ptx::mbar_init(bar_q_empty(i), PAIR ? 1 : kTreeSoftmaxWarps);
+      ptx::mbar_init(bar_q_full(i), kTreeQWarps<QUANT>);
+      ptx::mbar_init(bar_q_empty(i), PAIR ? 2 : kTreeSoftmaxWarps + 2);
     }
     for (int i = 0; i < KS; ++i) {
       ptx::mbar_init(bar_k_full(i), QUANT ? kTreeConvertWarpsOf : 1);
-      ptx::mbar_init(bar_k_empty(i), 1);
+      ptx::mbar_init(bar_k_empty(i), PAIR ? 2 : 1);
     }
     for (int i = 0; i < VS; ++i) {
       ptx::mbar_init(bar_v_full(i), QUANT ? kTreeConvertWarpsOf : 1);
-      ptx::mbar_init(bar_v_empty(i), 1);
+      ptx::mbar_init(bar_v_empty(i), PAIR ? 2 : 1);
     }
     for (int w = 0; w < 2; ++w) {
       ptx::mbar_init(bar_s(w), 1);
@@ -653,7 +682,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
     ptx::tmem_relinquish();
   }
-  if (warp == kTreeLoadWarp && lane == 0) {
+  if (warp == kLoadWarp && lane == 0) {
     ptx::prefetch_tensormap(&tmap_k);
     ptx::prefetch_tensormap(&tmap_v);
   }
@@ -661,7 +690,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   ptx::grid_dependency_wait();  // the kernel before this one may have written lengths, cache or queries
   if (blockIdx.x == 0 && threadIdx.x < 4) p.status[threadIdx.x] = 0;
   const TreeLengths lengths{p.lengths, p.index_bits};
-  if (warp == kTreeQWarp) {
+  if (warp >= kTreeQWarp && warp < kLoadWarp) {
     tree_find_piece(p, lengths, lane, start_b, start_off, start_n);
   }
   ptx::tc_fence_before_sync();
@@ -673,64 +702,87 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   walk.start(n_tiles > 0 ? *start_b : 0, *start_off, n_tiles);
   TreeSegment seg{};
 
-  if (warp >= kTreeQWarp && warp < kTreeQWarp + kTreeQWarps) {
+  if (warp >= kTreeQWarp && warp < kLoadWarp) {
     // ----------------------------------------------------- queries of the next segment
-    const int tid = threadIdx.x - 32 * kTreeQWarp;
-    constexpr int kRowsHere = PAIR ? 256 : 128;
-    uint32_t seq = 0;
-    while (walk.next(seg)) {
-      const uint32_t buf = seq % L::kQBuffers, ph = (seq / L::kQBuffers) & 1u;
-      if (!TREE_WAIT_BEHIND(bar_q_empty(buf), ph ^ 1u, ST_TR_WAIT_Q_EMPTY)) break;
-      ++seq;
-      const int kh = seg.group / p.row_tiles, r0 = (seg.group - kh * p.row_tiles) * 256;
-      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)kh * p.G * p.qh;
+    // (all copies of a segment under way at once: behind the flood of key and value tiles each wait costs microseconds)
+    auto load_queries = [&](const TreeSegment s, uint32_t number) {
+      const uint32_t buf = number % L::kQBuffers;
+      if (!TREE_WAIT_BEHIND(bar_q_empty(buf), ((number / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
+      const int kh = s.group / p.row_tiles, r0 = (s.group - kh * p.row_tiles) * 256;
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + s.b * p.qb + (long long)kh * p.G * p.qh;
       const uint32_t dst0 = base + L::off_q + buf * L::kQBytes;
+      const long long qh = p.qh, qm = p.qm;
+      const int M = p.M, rows = p.rows - r0;
       constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
-      // (all copies of a segment under way at once: behind the flood of key and value tiles each wait costs microseconds)
-      for (int i = tid; i < kRowsHere * kChunks; i += 32 * kTreeQWarps) {
-        const int row = i / kChunks, c = i % kChunks, d0 = c * 8, r = r0 + row;
-        const int g = r / p.M, m = r - g * p.M;
-        const bool on = r < p.rows && d0 < p.D;
+      constexpr int kStep = 32 * kTreeQWarps<QUANT> / kChunks;
+      const int first = 32 * (warp - kTreeQWarp) + lane, c = first % kChunks, d0 = c * 8;
+      const bool on_d = d0 < p.D;
+      int row = first / kChunks, g = (r0 + row) / M, m = r0 + row - g * M;
+#pragma unroll 4
+      for (int i = 0; i < (PAIR ? 256 : 128) / kStep; ++i) {
+        const bool on = row < rows && on_d;
         const uint32_t tile = dst0 + (uint32_t)(row >> 7) * L::kTileBytes, in = (uint32_t)(row & 127);
         ptx::cp_async16(tile + (uint32_t)(c >> 3) * L::kSlabBytes + in * 128u + (((uint32_t)c & 7u) ^ (in & 7u)) * 16u,
-                        on ? q + g * p.qh + m * p.qm + d0 : q, on);
+                        on ? q + g * qh + m * qm + d0 : q, on);
+        row += kStep;
+        for (m += kStep; m >= M; m -= M) ++g;
       }
       ptx::cp_async_wait_all();
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar_q_full(buf));
-    }
-  } else if (QUANT && warp == kTreeQWarp + 1) {
-    tree_load_scales<1>(p, ring, walk, lane, abort_flag, [](long long) { return true; });
-  } else if (warp == kTreeMmaWarp) {
+      return true;
+    };
+    tree_query_role<1, QUANT>(p, ring, walk, lane, abort_flag, load_queries);
+  } else if (warp == kTreeMmaWarp || warp == kTreeMmaWarp + 1) {
     // ------------------------------------------------------------------- products
-    // Step j: tile j (PAIR: tile j / 2) for warpgroup j mod 2.  S runs two steps ahead of P V, which also orders
-    // the buffers: S of step j + 2 overwrites the P that the products of step j have read.
-    TreeWalk<TreeLengths> ahead = walk;
-    TreeSegment sa;
-    int s_left = 0, o_left = 0, s_done = 0;     // tiles left in the segment that S / P V is in
-    uint32_t s_tile = 0, o_tile = 0, q_seq = 0; // tiles so far
-    int o_done = 0;
-    bool ok = true;
-    const int per_tile = PAIR ? 2 : 1;
-    const long long steps = n_tiles * per_tile;
-    auto issue_s = [&](uint32_t w) {
-      const bool opens = !PAIR || w == 0, closes = !PAIR || w == 1;
-      if (opens) {
-        if (s_left == 0) {
-          ahead.next(sa);
-          s_left = sa.hi - sa.lo;
-          s_done = 0;
-          ok = TREE_WAIT(bar_q_full(q_seq % L::kQBuffers), (q_seq / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
-          if (!ok) return;
-        }
-        ok = TREE_WAIT(bar_k_full(s_tile % KS), (s_tile / KS) & 1u, ST_TR_WAIT_K_FULL);
-        if (!ok) return;
+    // A warp per warpgroup: S of its next tile follows P V of the last one, which orders the buffer they share (S
+    // overwrites the P that the product has read), and while one warpgroup takes exponentials the other's products run.
+    // (One warp that issued for both in turn kept the tensor pipe idle whenever it waited for either: 144 us for 64 tokens
+    // over 8 x 8 heads of 16384 keys.)
+    const uint32_t w = (uint32_t)(warp - kTreeMmaWarp);
+    struct Cursor {
+      TreeWalk<TreeLengths> walk;
+      TreeSegment s;
+      int t;
+      uint32_t tile, seg;
+      bool on;
+      __device__ __forceinline__ void step() {
+        ++tile;
+        if (++t < s.hi) return;
+        on = walk.next(s);
+        t = s.lo;
+        ++seg;
       }
+    };
+    constexpr int kStride = PAIR ? 1 : 2;  // own tiles: all, or every other one
+    auto first_own = [&]() {
+      Cursor c{walk, TreeSegment{}, 0, 0, 0, false};
+      c.on = c.walk.next(c.s);
+      c.t = c.s.lo;
+      if (!PAIR && w == 1 && c.on) c.step();
+      return c;
+    };
+    auto next_own = [&](Cursor& c) {
+      c.step();
+      if (!PAIR && c.on) c.step();
+    };
+    Cursor sc = first_own(), oc = sc;
+    uint32_t q_waited = 0, p_use = 0;
+    bool ok = true;
+    auto issue_s = [&]() {
+      // every segment's queries in turn, also those of a segment without a tile for this warpgroup: no phase is skipped,
+      // and none can pass unseen, as the buffer is given back by this warp too
+      for (; ok && q_waited <= sc.seg; ++q_waited) {
+        if (!PAIR && q_waited > 0 && lane == 0) ptx::mbar_arrive(bar_q_empty((q_waited - 1u) % L::kQBuffers));
+        ok = TREE_WAIT(bar_q_full(q_waited % L::kQBuffers), (q_waited / L::kQBuffers) & 1u, ST_TR_WAIT_Q_FULL);
+      }
+      if (ok) ok = TREE_WAIT(bar_k_full(sc.tile % KS), (sc.tile / KS) & 1u, ST_TR_WAIT_K_FULL);
+      if (!ok) return;
       ptx::tc_fence_after_sync();
       if (ptx::elect_one()) {
-        const uint32_t a_lo = ptx::smem_desc_lo(base + L::off_q + (q_seq % L::kQBuffers) * L::kQBytes + (PAIR ? w * L::kTileBytes : 0));
-        const uint32_t b_lo = ptx::smem_desc_lo(base + L::off_k + (s_tile % KS) * L::kTileBytes);
+        const uint32_t a_lo = ptx::smem_desc_lo(base + L::off_q + (sc.seg % L::kQBuffers) * L::kQBytes + (PAIR ? w * L::kTileBytes : 0));
+        const uint32_t b_lo = ptx::smem_desc_lo(base + L::off_k + (sc.tile % KS) * L::kTileBytes);
         const uint32_t d = tmem_base + 2 * DPAD + w * 128;
 #pragma unroll
         for (int kk = 0; kk < DPAD / 16; ++kk) {
@@ -738,55 +790,36 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           if (kk < p.k_steps) ptx::umma_step<false>(d, a_lo + off, b_lo + off, p.idesc_s, kk == 0);
         }
         ptx::umma_commit(bar_s(w));
-        if (closes) {
-          ptx::umma_commit(bar_k_empty(s_tile % KS));
-          if (PAIR && s_left == 1) ptx::umma_commit(bar_q_empty(q_seq % L::kQBuffers));
-        }
+        ptx::umma_commit(bar_k_empty(sc.tile % KS));
+        if (PAIR && sc.t + 1 == sc.s.hi) ptx::umma_commit(bar_q_empty(sc.seg % L::kQBuffers));
       }
       __syncwarp();
-      if (closes) {
-        ++s_tile;
-        ++s_done;
-        if (--s_left == 0) ++q_seq;
-      }
+      next_own(sc);
     };
-    if (steps > 0) issue_s(0);
-    if (ok && steps > 1) issue_s(1);
-    for (long long j = 0; ok && j < steps; ++j) {
-      const uint32_t w = (uint32_t)j & 1u;
-      const bool opens = !PAIR || w == 0, closes = !PAIR || w == 1;
-      if (opens && o_left == 0) {
-        walk.next(seg);
-        o_left = seg.hi - seg.lo;
-        o_done = 0;
-      }
-      if (opens) {
-        ok = TREE_WAIT(bar_v_full(o_tile % VS), (o_tile / VS) & 1u, ST_TR_WAIT_V_FULL);
-        if (!ok) break;
-      }
-      ok = TREE_WAIT_BEHIND(bar_p(w), (uint32_t)(j >> 1) & 1u, ST_TR_WAIT_P);
+    if (sc.on) issue_s();
+    while (ok && oc.on) {
+      ok = TREE_WAIT(bar_v_full(oc.tile % VS), (oc.tile / VS) & 1u, ST_TR_WAIT_V_FULL);
       if (!ok) break;
+      ok = TREE_WAIT_BEHIND(bar_p(w), p_use & 1u, ST_TR_WAIT_P);
+      if (!ok) break;
+      ++p_use;
       ptx::tc_fence_after_sync();
       if (ptx::elect_one()) {
-        const uint32_t b_lo = ptx::smem_desc_lo_mn(base + L::off_v + (o_tile % VS) * L::kTileBytes, L::kSlabBytes);
+        const uint32_t b_lo = ptx::smem_desc_lo_mn(base + L::off_v + (oc.tile % VS) * L::kTileBytes, L::kSlabBytes);
         const uint32_t a = tmem_base + 2 * DPAD + w * 128, d = tmem_base + w * DPAD;
-        const bool first = o_done < (PAIR ? 1 : 2);  // this warpgroup's first tile of the segment
+        const bool first = oc.t - oc.s.lo < kStride;  // this warpgroup's first tile of the segment
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) ptx::umma_f16_ts(d, a + 8 * kk, b_lo + kk * (2048u >> 4), p.idesc_o, !(first && kk == 0));
-        if (closes) ptx::umma_commit(bar_v_empty(o_tile % VS));
-        if (o_left <= (PAIR ? 1 : 2)) ptx::umma_commit(bar_o(w));  // ... and its last one
+        ptx::umma_commit(bar_v_empty(oc.tile % VS));
+        if (oc.s.hi - oc.t <= kStride) ptx::umma_commit(bar_o(w));  // ... and its last one
       }
       __syncwarp();
-      if (closes) {
-        ++o_tile;
-        ++o_done;
-        --o_left;
-      }
-      if (j + 2 < steps) issue_s(w);
+      next_own(oc);
+      if (sc.on) issue_s();
     }
-  } else if (warp >= kTreeLoadWarp) {
+  } else if (warp >= kLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    tree_load_roles<T, DPAD, KS, VS, L::SS, 1, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kTreeLoadWarp, lane, abort_flag, bad_flag);
+    tree_load_roles<T, DPAD, KS, VS, L::SS, 1, FORMAT>(p, ring, &tmap_k, &tmap_v, walk, warp - kLoadWarp, lane, abort_flag, bad_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int w = warp >> 2;
@@ -930,7 +963,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           if (*bad_flag) {
             float fix[32];
             for (int e = 0; e < 32; ++e) fix[e] = o[e];
-            tree_add_non_finite<T, QUANT>(p, seg, words, m, 32 * c, 32, fix);
+            tree_add_non_finite<T, FORMAT>(p, seg, words, m, 32 * c, 32, fix);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = fix[e];
           }
@@ -999,7 +1032,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
               if (*bad_flag) {
                 float o[4] = {sum.x, sum.y, sum.z, sum.w};
                 const int rm = r % p.M;
-                tree_add_non_finite<T, QUANT>(p, seg, p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + rm) * p.words : nullptr,
+                tree_add_non_finite<T, FORMAT>(p, seg, p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + rm) * p.words : nullptr,
                                               rm, d, 4, o);
                 sum = make_float4(o[0], o[1], o[2], o[3]);
               }

@@ -46,9 +46,10 @@ struct DecodeSmem {
   // that, and the two buffers lie side by side.
   static constexpr int kPBytes = NR == 64 ? 2 * kSlabBytes : kSlabBytes;
   static constexpr int kPStep = NR == 64 ? kSlabBytes : 64;  // from one buffer to the other
+  static constexpr int kValueSlots = NR == 64 ? 1 : 2, kCodeSlots = 4;
   static constexpr int KS = DPAD == 64 ? (QUANT ? 4 : 5) : (QUANT ? 2 : 3);
-  static constexpr int VS = DPAD == 64 ? (QUANT ? 4 : 5) : (QUANT || NR == 64 ? 2 : 3);
-  static constexpr int SS = QUANT ? (DPAD == 64 ? 6 : NR == 64 ? 2 : 4) : 0;  // tiles of codes in flight
+  static constexpr int VS = DPAD == 64 ? (QUANT ? 4 : 5) : (QUANT ? kValueSlots : NR == 64 ? 2 : 3);
+  static constexpr int SS = QUANT ? (DPAD == 64 ? 6 : kCodeSlots) : 0;  // tiles of codes in flight
   static constexpr int off_k = 0;
   static constexpr int off_v = off_k + KS * kTileBytes;
   static constexpr int off_p = off_v + VS * kTileBytes;
@@ -102,10 +103,11 @@ __device__ __noinline__ uint32_t decode_row_bits(const TreeParams& p, const Tree
   return bits;
 }
 
-template <typename T, int DPAD, int NR, bool QUANT>
-__global__ void __launch_bounds__((decode_threads<NR, QUANT>()), 1)
+template <typename T, int DPAD, int NR, int FORMAT>
+__global__ void __launch_bounds__((decode_threads<NR, FORMAT != FCR_KV_16BIT>()), 1)
 tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                    const __grid_constant__ TreeParams p) {
+  constexpr bool QUANT = FORMAT != FCR_KV_16BIT;
   using L = DecodeSmem<DPAD, NR, QUANT>;
   constexpr int KS = L::KS, VS = L::VS;
   constexpr int W = NR < 32 ? NR : 32;                 // rows that a warpgroup owns
@@ -184,24 +186,24 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
   if (warp == kQWarp) {
     // ----------------------------------------------------- queries of the next segment
     // (all copies of a segment under way at once: behind the flood of key and value tiles each wait costs microseconds)
-    uint32_t seq = 0;
-    auto load_queries = [&]() {
-      const uint32_t buf = seq % L::kQBuffers;
-      if (!TREE_WAIT_BEHIND(bar_q_empty + 8u * buf, ((seq / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
-      ++seq;
-      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + seg.b * p.qb + (long long)seg.group * p.G * p.qh;
+    auto load_queries = [&](const TreeSegment s, uint32_t number) {
+      const uint32_t buf = number % L::kQBuffers;
+      if (!TREE_WAIT_BEHIND(bar_q_empty + 8u * buf, ((number / L::kQBuffers) & 1u) ^ 1u, ST_TR_WAIT_Q_EMPTY)) return false;
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + s.b * p.qb + (long long)s.group * p.G * p.qh;
+      const long long qh = p.qh, qm = p.qm;
+      const int M = p.M, rows = p.rows;
       const uint32_t dst = base + L::off_q + buf * L::kQBytes;
       constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
       constexpr int kRowsAtATime = 32 / kChunks;
       const int c = lane % kChunks, d0 = c * 8;
-      int row = lane / kChunks, g = row / p.M, m = row - g * p.M;
+      int row = lane / kChunks, g = row / M, m = row - g * M;
 #pragma unroll 4
       for (int i = 0; i < NR / kRowsAtATime; ++i) {
-        const bool on = row < p.rows && d0 < p.D;
+        const bool on = row < rows && d0 < p.D;
         ptx::cp_async16(dst + (uint32_t)(c >> 3) * L::kQSlabBytes + (uint32_t)row * 128u + (((uint32_t)c & 7u) ^ ((uint32_t)row & 7u)) * 16u,
-                        on ? q + g * p.qh + m * p.qm + d0 : q, on);
+                        on ? q + g * qh + m * qm + d0 : q, on);
         row += kRowsAtATime;
-        for (m += kRowsAtATime; m >= p.M; m -= p.M) ++g;
+        for (m += kRowsAtATime; m >= M; m -= M) ++g;
       }
       ptx::cp_async_wait_all();
       ptx::fence_proxy_async_smem();
@@ -209,22 +211,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
       if (lane == 0) ptx::mbar_arrive(bar_q_full + 8u * buf);
       return true;
     };
-    if constexpr (QUANT) {
-      // The queries of a segment follow the scales of its first tiles: those never wait for queries, which may wait for the
-      // products of the segment before.
-      TreeWalk<TreeLengths> scale_walk = walk;
-      long long next_at = 0;  // first tile of the next segment whose queries are to come
-      tree_load_scales<2>(p, ring, scale_walk, lane, abort_flag, [&](long long tiles) {
-        while (next_at < tiles && walk.next(seg)) {
-          next_at += seg.hi - seg.lo;
-          if (!load_queries()) return false;
-        }
-        return true;
-      });
-    } else {
-      while (walk.next(seg) && load_queries()) {
-      }
-    }
+    tree_query_role<2, QUANT>(p, ring, walk, lane, abort_flag, load_queries);
   } else if (warp == kSWarp) {
     // ------------------------------------------------------------------- S^T = K Q^T
     // Two score buffers: tile j may be written once the weights of tile j - 2 have been made.  (One warp that issued
@@ -286,7 +273,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
     }
   } else if (warp >= kLoadWarp) {
     // -------------------------------------------------------- key and value tiles
-    tree_load_roles<T, DPAD, KS, VS, L::SS, 2, QUANT>(p, ring, &tmap_k, &tmap_v, walk, warp - kLoadWarp, lane, abort_flag, bad_flag);
+    tree_load_roles<T, DPAD, KS, VS, L::SS, 2, FORMAT>(p, ring, &tmap_k, &tmap_v, walk, warp - kLoadWarp, lane, abort_flag, bad_flag);
   } else {
     // -------------------------------------------------------------- softmax warps
     const int wg = warp >> 2, wq = warp & 3;
@@ -332,7 +319,9 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         const uint32_t bits = edge ? decode_row_bits(p, seg, t * kTreeTile + key, r0, W) : 0xffffffffu;
         auto load_scores = [&](uint32_t (&x)[W]) {
           tmem_row_ld<W>(s_addr, x);
-          if (edge) {
+          int masked = edge;
+          asm volatile("" : "+r"(masked));  // (or the compiler makes a second copy of the whole tile for edge tiles)
+          if (masked) {
 #pragma unroll
             for (int e = 0; e < W; ++e) x[e] = (bits >> e) & 1u ? x[e] : 0xff800000u;
           }
@@ -355,7 +344,10 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         if (vote[buf] == (int)tile_seq) {
           // the rows' maxima over the tile's 128 keys; O^T, the sums and the reference follow where a row has grown
           float top = -INFINITY;
-          load_scores(x);  // (again: in registers they would crowd out the loop's values)
+          // (Scores and references are read again: kept in registers for this rare path they spilled the common one's values,
+          // 64 bf16 rows over 16 x 8 heads of 4096 keys took 90 us instead of 70.)
+          asm volatile("" ::: "memory");
+          load_scores(x);
 #pragma unroll
           for (int e = 0; e < W; ++e) {
             const float largest = ptx::redux_max(__uint_as_float(x[e]));
@@ -455,7 +447,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         for (int r = r0; r < min(r0 + W, p.rows); ++r) {
           const int m = r % p.M;
           float fix = 0.f;
-          tree_add_non_finite<T, QUANT>(p, seg, p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + m) * p.words : nullptr, m, key, 1, &fix);
+          tree_add_non_finite<T, FORMAT>(p, seg, p.mask ? p.mask + ((size_t)(p.mask_shared ? 0 : seg.b) * p.M + m) * p.words : nullptr, m, key, 1, &fix);
 #pragma unroll
           for (int e = 0; e < W; ++e)
             if (e == r - r0) o[e] = __float_as_uint(__uint_as_float(o[e]) + fix);

@@ -603,3 +603,19 @@ def test_another_device_than_the_current_one():
     with torch.cuda.device(1):
         got = _serve(x, cache, lens, w, freq, mask, hq, h, m)
     assert all(torch.equal(a, e) for a, e in zip(got, want))
+
+
+@pytest.mark.parametrize("fmt", ["16", FP8])
+@pytest.mark.parametrize("hq,h,m,n,d", [(24, 1, 3, 130, 128), (9, 3, 32, 100, 64), (32, 32, 70, 128, 128), (10, 5, 64, 700, 64), (64, 16, 20, 140, 128)])
+def test_many_short_groups(fmt, hq, h, m, n, d):
+    """More groups of one or two tiles than CTAs, 65 to 128 rows each: a warpgroup has no tile in every other group."""
+    b = 40
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, n - m + 1, (b,), generator=g).tolist()
+    q, cache, x = _make(b, hq, h, m, n, d, fmt, BF, seed=n)
+    got, lse = _run(q, cache, lens)
+    pick = [0, 17, b - 1]
+    _check_attention(got[pick], lse[pick], q[pick], x[0][pick], x[1][pick], [lens[i] for i in pick], None)
+    # every sequence alone gives the same up to the order in which partial sums are added
+    one, _ = _run(q[5:6], [None if c is None else c[5:6] for c in cache], lens[5:6])
+    assert (one.float() - got[5:6].float()).abs().max() <= 4 * _u(BF) * x[1].abs().max()
