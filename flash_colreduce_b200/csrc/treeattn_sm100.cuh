@@ -39,13 +39,12 @@ constexpr int kTreeSoftmaxWarps = 8;  // two warpgroups
 constexpr int kTreeMmaWarp = 8;       // two warps, one per warpgroup
 constexpr int kTreeQWarp = 10;        // first of those that bring the queries
 template <bool QUANT>
-constexpr int kTreeQWarps = QUANT ? 1 : 4;  // with an 8-bit cache one, which brings its scales too
-template <bool QUANT>
-constexpr int kTreeLoadWarp = kTreeQWarp + kTreeQWarps<QUANT>;  // TMA; for an 8-bit cache then the warps that convert codes
+__host__ __device__ constexpr int tree_q_warps() { return QUANT ? 1 : 4; }  // with an 8-bit cache one, which brings its scales too
+// then TMA, and for an 8-bit cache the warps that convert codes
 constexpr int kTreeConvertWarps = 8;
 constexpr int kTreeConvertWarpsOf = kTreeConvertWarps / 2;  // for the keys, and for the values
 template <bool QUANT>
-constexpr int tree_threads() { return 32 * (kTreeLoadWarp<QUANT> + 1 + (QUANT ? kTreeConvertWarps : 0)); }
+constexpr int tree_threads() { return 32 * (kTreeQWarp + tree_q_warps<QUANT>() + 1 + (QUANT ? kTreeConvertWarps : 0)); }
 
 enum {
   ST_TR_WAIT_Q_EMPTY = 71,
@@ -151,7 +150,7 @@ struct TreeSmem {
 };
 
 // Bits of the keys n0 .. n0 + 31 that row m attends.
-__device__ __forceinline__ uint32_t tree_bits(const TreeParams& p, const uint32_t* words, int m, int n0, int have, int end) {
+__device__ __noinline__ uint32_t tree_bits(const TreeParams& p, const uint32_t* words, int m, int n0, int have, int end) {
   if (n0 + 32 <= have) return 0xffffffffu;
   if (n0 >= end) return 0u;
   const int j0 = n0 - have;  // place of the first key among the drafted tokens, negative: cached positions come first
@@ -623,7 +622,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                       const __grid_constant__ TreeParams p) {
   constexpr bool QUANT = FORMAT != FCR_KV_16BIT;
   using L = TreeSmem<DPAD, PAIR, QUANT>;
-  constexpr int KS = L::KS, VS = L::VS, kLoadWarp = kTreeLoadWarp<QUANT>;
+  constexpr int KS = L::KS, VS = L::VS, kLoadWarp = kTreeQWarp + tree_q_warps<QUANT>();
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base = ptx::smem_u32(smem);
   if ((base & 1023u) != 0) {
@@ -656,7 +655,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kQBuffers; ++i) {
-      ptx::mbar_init(bar_q_full(i), kTreeQWarps<QUANT>);
+      ptx::mbar_init(bar_q_full(i), tree_q_warps<QUANT>());
       ptx::mbar_init(bar_q_empty(i), PAIR ? 2 : kTreeSoftmaxWarps + 2);
     }
     for (int i = 0; i < KS; ++i) {
@@ -714,7 +713,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const long long qh = p.qh, qm = p.qm;
       const int M = p.M, rows = p.rows - r0;
       constexpr int kChunks = DPAD / 8;  // 16-byte pieces of a row
-      constexpr int kStep = 32 * kTreeQWarps<QUANT> / kChunks;
+      constexpr int kStep = 32 * tree_q_warps<QUANT>() / kChunks;
       const int first = 32 * (warp - kTreeQWarp) + lane, c = first % kChunks, d0 = c * 8;
       const bool on_d = d0 < p.D;
       int row = first / kChunks, g = (r0 + row) / M, m = r0 + row - g * M;
@@ -851,73 +850,93 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         ++s_use;
         ptx::tc_fence_after_sync();
         const bool edge = (t + 1) * kTreeTile > seg.have;
-        uint32_t ra[32];
-        float top = -INFINITY;
-        for (int c = 0; c < 4; ++c) {
-          ptx::tmem_ld<32>(s_addr + 32 * c, ra);
-          ptx::tmem_ld_wait<32>(ra);
-          if (edge) {
-            const uint32_t bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+        uint32_t bits[4];  // the tile's keys that this row attends
+        if (edge) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ra[e] = (bits >> e) & 1u ? ra[e] : 0xff800000u;
-          }
-          float t0 = __uint_as_float(ra[0]), t1 = __uint_as_float(ra[1]);
-#pragma unroll
-          for (int e = 2; e < 32; e += 4) {
-            t0 = ptx::max3(t0, __uint_as_float(ra[e]), __uint_as_float(ra[e + 1]));
-            if (e + 3 < 32) t1 = ptx::max3(t1, __uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3]));
-          }
-          top = ptx::max3(top, t0, t1);
+          for (int c = 0; c < 4; ++c) bits[c] = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
         }
-        top *= p.scale2;
-        // the reference moves when the maximum has grown by more than 2^8: P stays below that, far from any type's limits
-        const bool grow = real && top > m_ref + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? top : m_ref;
-          const float alpha = m_new == m_ref ? 1.f : ptx::ex2(m_ref - m_new);
-          m_ref = m_new;
-          l *= alpha;
-          if (mine > 0) {
-            for (int c = 0; c < DPAD / 32; ++c) {
-              ptx::tmem_ld<32>(o_addr + 32 * c, ra);
-              ptx::tmem_ld_wait<32>(ra);
+        // Columns at a time: a load from tensor memory is waited for twice per pass instead of four times, where the
+        // converters leave the registers for it.
+        constexpr int CW = QUANT ? 32 : 64;
+        auto load_scores = [&](int c, uint32_t (&x)[CW]) {
+          ptx::tmem_ld<CW>(s_addr + CW * c, x);
+          ptx::tmem_ld_wait<CW>(x);
+          if (edge) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) ra[e] = __float_as_uint(__uint_as_float(ra[e]) * alpha);
-              ptx::tmem_st32(o_addr + 32 * c, ra);
+            for (int i = 0; i < CW / 32; ++i) {
+              const int at = c * (CW / 32) + i;
+              const uint32_t now = at == 0 ? bits[0] : at == 1 ? bits[1] : at == 2 ? bits[2] : bits[3];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[32 * i + e] = (now >> e) & 1u ? x[32 * i + e] : 0xff800000u;
             }
           }
-        }
-        const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
-        float2 s01 = make_float2(0.f, 0.f), s23 = make_float2(0.f, 0.f);
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-          ptx::tmem_ld<32>(s_addr + 32 * c, ra);
-          ptx::tmem_ld_wait<32>(ra);
-          uint32_t bits = 0xffffffffu;
-          if (edge) bits = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+        };
+        auto largest = [&](const uint32_t (&x)[CW], float top) {
+          float t0 = top, t1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float2 a = __ffma2_rn(make_float2(__uint_as_float(ra[e]), __uint_as_float(ra[e + 1])), make_float2(p.scale2, p.scale2),
+          for (int e = 0; e < CW; e += 4) {
+            t0 = ptx::max3(t0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            t1 = ptx::max3(t1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          }
+          return fmaxf(t0, t1);
+        };
+        float2 s01, s23;
+        auto weigh = [&](const uint32_t (&x)[CW], uint32_t (&pk)[CW / 2]) {
+          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+#pragma unroll
+          for (int e = 0; e < CW; e += 4) {
+            float2 a = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(p.scale2, p.scale2),
                                   make_float2(nm, nm));
-            float2 b = __ffma2_rn(make_float2(__uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3])), make_float2(p.scale2, p.scale2),
+            float2 b = __ffma2_rn(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), make_float2(p.scale2, p.scale2),
                                   make_float2(nm, nm));
             a.x = ptx::ex2(a.x);
             a.y = ptx::ex2(a.y);
             b.x = ptx::ex2(b.x);
             b.y = ptx::ex2(b.y);
-            if (edge) {
-              a.x = (bits >> e) & 1u ? a.x : 0.f;
-              a.y = (bits >> (e + 1)) & 1u ? a.y : 0.f;
-              b.x = (bits >> (e + 2)) & 1u ? b.x : 0.f;
-              b.y = (bits >> (e + 3)) & 1u ? b.y : 0.f;
-            }
             s01 = __fadd2_rn(s01, a);
             s23 = __fadd2_rn(s23, b);
             pk[e / 2] = pack2(a.x, a.y, T());
             pk[e / 2 + 1] = pack2(b.x, b.y, T());
           }
-          // P chunk c covers columns 16 c .. 16 c + 15: scores that this thread has read
-          ptx::tmem_st16(s_addr + 16 * c, pk);
+        };
+        // The reference moves when the maximum has grown by more than 2^8: P stays below that, far from any type's limits.
+        auto follow = [&](float top) {
+          const bool grow = real && top > m_ref + 8.f;
+          if (!__any_sync(0xffffffffu, grow)) return;
+          const float m_new = grow ? top : m_ref;
+          const float alpha = m_new == m_ref ? 1.f : ptx::ex2(m_ref - m_new);
+          m_ref = m_new;
+          l *= alpha;
+          if (mine > 0) {
+            uint32_t o[32];
+            for (int c = 0; c < DPAD / 32; ++c) {
+              ptx::tmem_ld<32>(o_addr + 32 * c, o);
+              ptx::tmem_ld_wait<32>(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              ptx::tmem_st32(o_addr + 32 * c, o);
+            }
+          }
+        };
+        // Two passes over the scores, for the maximum and for the weights.  (One pass that keeps the tile's weights in registers
+        // until the maximum beside them is known spilled 700 bytes a thread, with 168 registers: 151 -> 212 us for 64
+        // tokens over 8 x 8 heads of 16384 keys.)
+        uint32_t x[CW];
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 128 / CW; ++c) {
+          load_scores(c, x);
+          top = largest(x, top);
+        }
+        follow(top * p.scale2);
+        s01 = s23 = make_float2(0.f, 0.f);
+#pragma unroll 1
+        for (int c = 0; c < 128 / CW; ++c) {
+          uint32_t pk[CW / 2];
+          load_scores(c, x);
+          weigh(x, pk);
+          // P chunk c covers columns CW / 2 * c and on: scores that this thread has read
+          if constexpr (CW == 64) ptx::tmem_st32(s_addr + 32 * c, pk); else ptx::tmem_st16(s_addr + 16 * c, pk);
         }
         l += (s01.x + s01.y) + (s23.x + s23.y);
         ptx::tmem_st_wait();
