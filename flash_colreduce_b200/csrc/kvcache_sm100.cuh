@@ -32,7 +32,6 @@ struct KvAppendParams {
   long long xb[2], xh[2], xm[2];
   int B, H, N, D, M;
   int group;               // lanes per row: the power of two that covers D in steps of 8
-  int blocks_per_head;
   const void* lengths;
   const void* counts;      // null: all M tokens
   int index_bits;
@@ -42,7 +41,7 @@ struct KvReadParams {
   KvTensor t[2];
   void* y[2];              // contiguous (B, H, n, D)
   int B, H, N, D, n;
-  int group, blocks_per_head;
+  int group;
   const void* positions;   // (B, H, n) contiguous or null: 0 .. n-1
   int index_bits;
 };
@@ -124,8 +123,9 @@ constexpr int kKvRows = 4;
 struct KvPlace {
   int kv, b, h, row0, step;  // first row of this thread, distance to its next
 };
-__device__ __forceinline__ KvPlace kv_place(int B, int H, int group, int blocks_per_head) {
-  const int combo = blockIdx.x / blocks_per_head, block = blockIdx.x - combo * blocks_per_head;
+__device__ __forceinline__ KvPlace kv_place(int B, int H, int group) {
+  // neighbouring blocks take the same rows of all heads, which lie side by side in a projection's output
+  const int combos = 2 * B * H, block = blockIdx.x / combos, combo = blockIdx.x - block * combos;
   KvPlace r;
   r.kv = combo / (B * H);
   const int bh = combo - r.kv * (B * H);
@@ -142,19 +142,16 @@ kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   const int group = p.group;
   const int gl = threadIdx.x & (group - 1), d0 = gl * 8;
   const bool on = d0 < p.D;
-  const KvPlace at = kv_place(p.B, p.H, group, p.blocks_per_head);
+  const KvPlace at = kv_place(p.B, p.H, group);
   const KvTensor& t = p.t[at.kv];
   const T* x = reinterpret_cast<const T*>(p.x[at.kv]) + at.b * p.xb[at.kv] + at.h * p.xh[at.kv] + d0;
-  const long long first = load_index(p.lengths, p.index_bits, at.b);
-  // tokens that are written: m < count, and their positions exist
-  long long count = p.counts ? min(load_index(p.counts, p.index_bits, at.b), (long long)p.M) : p.M;
-  count = first < 0 ? 0 : min(count, (long long)p.N - first);
+  // (the rows are read whether they will be written or not: the loads need not wait for the lengths)
   uint4 raw[kKvRows];
 #pragma unroll
   for (int u = 0; u < kKvRows; ++u) {
     const int m = at.row0 + u * at.step;
     raw[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (m < count && on) {
+    if (m < p.M && on) {
       if (VEC) {
         raw[u] = *reinterpret_cast<const uint4*>(x + m * p.xm[at.kv]);
       } else {
@@ -165,6 +162,10 @@ kv_append_kernel(const __grid_constant__ KvAppendParams p) {
       }
     }
   }
+  const long long first = load_index(p.lengths, p.index_bits, at.b);
+  // tokens that are written: m < count, and their positions exist
+  long long count = p.counts ? min(load_index(p.counts, p.index_bits, at.b), (long long)p.M) : p.M;
+  count = first < 0 ? 0 : min(count, (long long)p.N - first);
 #pragma unroll
   for (int u = 0; u < kKvRows; ++u) {
     const int m = at.row0 + u * at.step;
@@ -199,8 +200,12 @@ kv_append_kernel(const __grid_constant__ KvAppendParams p) {
     const float lim = kv_largest<T, FORMAT>();
     uint32_t code[2] = {0u, 0u};
     if (fine) {
+      if (__uint_as_float(top) > lim) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -lim), lim) * inv;
+        for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -lim), lim);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= inv;
       if (FORMAT == FCR_KV_FP8) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -232,7 +237,7 @@ kv_read_kernel(const __grid_constant__ KvReadParams p) {
   const int group = p.group;
   const int gl = threadIdx.x & (group - 1), d0 = gl * 8;
   if (d0 >= p.D) return;
-  const KvPlace at = kv_place(p.B, p.H, group, p.blocks_per_head);
+  const KvPlace at = kv_place(p.B, p.H, group);
   const KvTensor& t = p.t[at.kv];
   const long long row_base = ((long long)at.b * p.H + at.h) * p.n;
   const long long data_base = at.b * t.sb + at.h * t.sh + d0, scale_base = at.b * t.ssb + at.h * t.ssh;

@@ -87,10 +87,9 @@ static int kv_group(int D) {
 }
 
 // Blocks for `rows` rows of each of 2 * B * H (K or V, sequence, head); 0 when the grid would be too large.
-static unsigned kv_blocks(int B, int H, int rows, int group, int* blocks_per_head) {
+static unsigned kv_blocks(int B, int H, int rows, int group) {
   const int per_block = 256 / group * kKvRows;
-  *blocks_per_head = (rows + per_block - 1) / per_block;
-  const long long blocks = 2LL * B * H * *blocks_per_head;
+  const long long blocks = 2LL * B * H * ((rows + per_block - 1) / per_block);
   return blocks > 0x7fffffffLL ? 0u : (unsigned)blocks;
 }
 
@@ -346,7 +345,7 @@ int fcr_kv_append(const fcr_kv_cache* cache, void* k_cache, void* v_cache, void*
   const int32_t sizes[3] = {c.B, c.H, M};
   const bool vec = cache_vectors(c, k_cache, v_cache) && kv_aligned(key, key_strides, sizes, 3, 2, 16) &&
                    kv_aligned(value, value_strides, sizes, 3, 2, 16);
-  const unsigned blocks = kv_blocks(c.B, c.H, M, p.group, &p.blocks_per_head);
+  const unsigned blocks = kv_blocks(c.B, c.H, M, p.group);
   if (blocks == 0) return fail(FCR_ERR_UNSUPPORTED, "too many rows");
   int sms = 0;
   rc = device_sm_count(&sms);  // refuses a device that this library has no code for
@@ -383,7 +382,7 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
   p.index_bits = index_bits;
   const bool vec = cache_vectors(c, k_cache, v_cache) && reinterpret_cast<uintptr_t>(k_out) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_out) % 16 == 0;
-  const unsigned blocks = kv_blocks(c.B, c.H, n, p.group, &p.blocks_per_head);
+  const unsigned blocks = kv_blocks(c.B, c.H, n, p.group);
   if (blocks == 0) return fail(FCR_ERR_UNSUPPORTED, "too many rows");
   int sms = 0;
   rc = device_sm_count(&sms);  // refuses a device that this library has no code for

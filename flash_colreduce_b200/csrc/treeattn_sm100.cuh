@@ -855,36 +855,29 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 #pragma unroll
           for (int c = 0; c < 4; ++c) bits[c] = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
         }
-        // Columns at a time: a load from tensor memory is waited for twice per pass instead of four times, where the
-        // converters leave the registers for it.
-        constexpr int CW = QUANT ? 32 : 64;
-        auto load_scores = [&](int c, uint32_t (&x)[CW]) {
-          ptx::tmem_ld<CW>(s_addr + CW * c, x);
-          ptx::tmem_ld_wait<CW>(x);
+        auto load_scores = [&](int c, uint32_t (&x)[32]) {
+          ptx::tmem_ld<32>(s_addr + 32 * c, x);
+          ptx::tmem_ld_wait<32>(x);
           if (edge) {
+            const uint32_t now = c == 0 ? bits[0] : c == 1 ? bits[1] : c == 2 ? bits[2] : bits[3];
 #pragma unroll
-            for (int i = 0; i < CW / 32; ++i) {
-              const int at = c * (CW / 32) + i;
-              const uint32_t now = at == 0 ? bits[0] : at == 1 ? bits[1] : at == 2 ? bits[2] : bits[3];
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[32 * i + e] = (now >> e) & 1u ? x[32 * i + e] : 0xff800000u;
-            }
+            for (int e = 0; e < 32; ++e) x[e] = (now >> e) & 1u ? x[e] : 0xff800000u;
           }
         };
-        auto largest = [&](const uint32_t (&x)[CW], float top) {
+        auto largest = [&](const uint32_t (&x)[32], float top) {
           float t0 = top, t1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < CW; e += 4) {
+          for (int e = 0; e < 32; e += 4) {
             t0 = ptx::max3(t0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
             t1 = ptx::max3(t1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
           return fmaxf(t0, t1);
         };
         float2 s01, s23;
-        auto weigh = [&](const uint32_t (&x)[CW], uint32_t (&pk)[CW / 2]) {
+        auto weigh = [&](const uint32_t (&x)[32], uint32_t (&pk)[16]) {
           const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
 #pragma unroll
-          for (int e = 0; e < CW; e += 4) {
+          for (int e = 0; e < 32; e += 4) {
             float2 a = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(p.scale2, p.scale2),
                                   make_float2(nm, nm));
             float2 b = __ffma2_rn(make_float2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), make_float2(p.scale2, p.scale2),
@@ -921,22 +914,22 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         // Two passes over the scores, for the maximum and for the weights.  (One pass that keeps the tile's weights in registers
         // until the maximum beside them is known spilled 700 bytes a thread, with 168 registers: 151 -> 212 us for 64
         // tokens over 8 x 8 heads of 16384 keys.)
-        uint32_t x[CW];
+        uint32_t x[32];
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < 128 / CW; ++c) {
+        for (int c = 0; c < 4; ++c) {
           load_scores(c, x);
           top = largest(x, top);
         }
         follow(top * p.scale2);
         s01 = s23 = make_float2(0.f, 0.f);
 #pragma unroll 1
-        for (int c = 0; c < 128 / CW; ++c) {
-          uint32_t pk[CW / 2];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
           load_scores(c, x);
           weigh(x, pk);
-          // P chunk c covers columns CW / 2 * c and on: scores that this thread has read
-          if constexpr (CW == 64) ptx::tmem_st32(s_addr + 32 * c, pk); else ptx::tmem_st16(s_addr + 16 * c, pk);
+          // P chunk c covers columns 16 c .. 16 c + 15: scores that this thread has read
+          ptx::tmem_st16(s_addr + 16 * c, pk);
         }
         l += (s01.x + s01.y) + (s23.x + s23.y);
         ptx::tmem_st_wait();

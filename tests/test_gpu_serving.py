@@ -619,3 +619,89 @@ def test_many_short_groups(fmt, hq, h, m, n, d):
     # every sequence alone gives the same up to the order in which partial sums are added
     one, _ = _run(q[5:6], [None if c is None else c[5:6] for c in cache], lens[5:6])
     assert (one.float() - got[5:6].float()).abs().max() <= 4 * _u(BF) * x[1].abs().max()
+
+
+# ----------------------------------------------------------------------------------------------- expired bounded waits
+@pytest.mark.parametrize("skip", [0, 3])
+@pytest.mark.parametrize("fmt", ["16", I8])
+@pytest.mark.parametrize("hq,h,m,d", [(4, 1, 1, 128), (4, 1, 8, 64), (4, 1, 16, 128), (4, 1, 24, 128), (4, 1, 64, 128)])
+def test_an_expired_wait_is_reported_and_the_next_call_is_right(skip, fmt, hq, h, m, d, monkeypatch):
+    """Every attention kernel with one tile's load left out (nothing is in flight for its slot) and waits of a millisecond: the
+    CTA gives up in an orderly way, the status reaches the host, and the call after the one that reports it runs."""
+    import ctypes as C
+
+    from flash_colreduce_b200 import _native as nat
+
+    monkeypatch.setenv("FCR_DEBUG_SYNC", "0")
+    q, cache, x = _make(1, hq, h, m, 2000, d, fmt, BF, seed=m)
+    before, lse = _run(q, cache, [2000 - m])
+    torch.cuda.synchronize()
+    nat.check(nat.lib.fcr_self_test_hooks(2_000_000, skip), "fcr_self_test_hooks")
+    try:
+        _run(q, cache, [2000 - m])
+    finally:
+        nat.check(nat.lib.fcr_self_test_hooks(0, -1), "fcr_self_test_hooks")
+    torch.cuda.synchronize()
+    code = C.c_int32(-1)
+    rc = nat.lib.fcr_poll_device_status(C.byref(code))
+    # 16 tiles on 16 CTAs: CTA 0 has one tile of a 16-bit cache (load 0), two loads of an 8-bit one (0 and 1)
+    if skip == 0:
+        assert rc == nat.FCR_ERR_DEVICE_TIMEOUT and 71 <= code.value <= 92, (rc, code.value)
+    else:
+        assert rc == nat.FCR_OK
+    after, lse2 = _run(q, cache, [2000 - m])
+    assert torch.equal(before, after) and torch.equal(lse, lse2)
+
+
+def test_the_next_attention_call_raises_for_the_failed_one(monkeypatch):
+    from flash_colreduce_b200 import _native as nat
+
+    monkeypatch.setenv("FCR_DEBUG_SYNC", "0")
+    q, cache, x = _make(1, 4, 1, 2, 2000, 128, "16", BF)
+    want, _ = _run(q, cache, [1998])
+    nat.check(nat.lib.fcr_self_test_hooks(2_000_000, 0), "fcr_self_test_hooks")
+    try:
+        _run(q, cache, [1998])
+    finally:
+        nat.check(nat.lib.fcr_self_test_hooks(0, -1), "fcr_self_test_hooks")
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="status 4.*earlier call"):
+        _run(q, cache, [1998])
+    got, _ = _run(q, cache, [1998])
+    assert torch.equal(got, want)
+
+
+def test_repeated_signatures_with_unaligned_queries_and_other_types():
+    """A signature that was checked once: the same shapes at an unaligned base, other types of lengths, scales as bytes."""
+    q, cache, x = _make(2, 4, 2, 3, 300, 64, I8, BF, seed=21)
+    lens = torch.tensor([290, 17], device=DEV)
+    want = fc.tree_attention(q.to(DEV), cache[0], cache[1], lens, key_scales=cache[2], value_scales=cache[3])
+    flat = torch.empty(q.numel() + 1, dtype=BF, device=DEV)
+    odd = flat[1:].view(q.shape)
+    odd.copy_(q)
+    for _ in range(2):
+        assert torch.equal(fc.tree_attention(odd, cache[0], cache[1], lens, key_scales=cache[2], value_scales=cache[3]), want)
+        assert torch.equal(fc.tree_attention(q.to(DEV), cache[0], cache[1], lens.int(), key_scales=cache[2].view(torch.uint8),
+                                             value_scales=cache[3].view(torch.uint8)), want)
+    with pytest.raises(ValueError, match="lengths"):
+        fc.tree_attention(q.to(DEV), cache[0], cache[1], lens.float(), key_scales=cache[2], value_scales=cache[3])
+    leaf = q.to(DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        fc.tree_attention(leaf, cache[0], cache[1], lens, key_scales=cache[2], value_scales=cache[3])
+    with torch.no_grad():
+        assert torch.equal(fc.tree_attention(leaf, cache[0], cache[1], lens, key_scales=cache[2], value_scales=cache[3]), want)
+
+
+def test_the_rows_are_quantised_alike_wherever_they_lie():
+    """Appending a prompt at once, in pieces, or token by token leaves the same bits."""
+    g = torch.Generator().manual_seed(31)
+    k, v = (torch.randn(2, 3, 70, 96, generator=g).to(HF).to(DEV) for _ in range(2))
+    caches = [_empty_cache(2, 3, 80, 96, FP8) for _ in range(3)]
+    start = torch.tensor([0, 5], device=DEV, dtype=torch.int32)
+    for c, sizes in zip(caches, ([70], [33, 1, 36], [1] * 70)):
+        at = 0
+        for s in sizes:
+            fc.kv_cache_append(k[:, :, at : at + s], v[:, :, at : at + s], c[0], c[1], start + at, c[2], c[3])
+            at += s
+    for c in caches[1:]:
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(c, caches[0]))
