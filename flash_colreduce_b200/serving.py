@@ -93,6 +93,7 @@ def qk_norm_rope(
     """
     if torch.is_grad_enabled():
         _check_no_grad("qk_norm_rope", query, key, q_weight, k_weight, inv_freq)
+    eps, interleaved = float(eps), bool(interleaved)  # (plain values: a signature must not hold a tensor)
     signature = (query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype, key.get_device(), positions.shape,
                  positions.stride(), positions.dtype, positions.get_device(), inv_freq.shape, inv_freq.is_contiguous(), inv_freq.dtype, inv_freq.get_device(),
                  _vector_signature(q_weight), _vector_signature(k_weight), eps, interleaved)
@@ -141,9 +142,9 @@ def _plan_rope(signature, query, key, positions, inv_freq, q_weight, k_weight, e
     used = (_rows(query), _rows(key), inv_freq.contiguous(), *(None if w is None else w.contiguous() for w in (q_weight, k_weight)))
     query, key, inv_freq = used[:3]
     p = nat.Rope(b, hq, hk, m, d, 2 * inv_freq.shape[0], (*query.stride()[:3], 1), (*key.stride()[:3], 1),
-                 _DTYPE_CODES[query.dtype], _DTYPE_CODES[weights[0].dtype] if weights else 0, 1 if interleaved else 0,
+                 _DTYPE_CODES[query.dtype], _DTYPE_CODES[weights[0].dtype] if weights else 0, int(interleaved),
                  _INDEX_BITS[positions.dtype], (positions.stride(0) if positions.dim() == 2 else 0, positions.stride(-1)),
-                 float(eps))
+                 eps)
     if all(x is y for x, y in zip(given, used)):
         _keep(_ROPE_CACHE, signature, p)
     return (p, *used)
@@ -211,7 +212,8 @@ def kv_cache_append(
 
     Args:
         key, value: (B, H, M, D) fp16 or bf16, D <= 256; any strides with innermost 1 (others are copied).
-        key_cache, value_cache: (B, H, N, D) of the same type (plain copies), float8_e4m3fn or int8.
+        key_cache, value_cache: (B, H, N, D) of the same type (plain copies), float8_e4m3fn or int8; they overlap neither
+            each other nor the inputs.
         lengths: (B,) int32 or int64.
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
         counts: (B,) of the type of ``lengths``, or None.
@@ -289,6 +291,8 @@ def kv_cache_read(
     """
     if torch.is_grad_enabled():
         _check_no_grad("kv_cache_read", key_cache, value_cache)
+    if n is not None:
+        n = int(n)
     signature = (key_cache.shape, key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(),
                  value_cache.dtype, value_cache.get_device(), _vector_signature(key_scales), _vector_signature(value_scales),
                  _vector_signature(positions), n, dtype)
@@ -327,7 +331,7 @@ def _plan_read(signature, key_cache, value_cache, key_scales, value_scales, posi
         n = positions.shape[2]
         positions = positions.contiguous()
     else:
-        n = cap if n is None else int(n)
+        n = cap if n is None else n
         if not 0 <= n <= cap:
             raise ValueError(f"n = {n} must lie in [0, {cap}].")
     _check_devices(key_cache.device, key_cache=key_cache, value_cache=value_cache, key_scales=key_scales,
@@ -374,6 +378,8 @@ def tree_attention(
     """
     if torch.is_grad_enabled():
         _check_no_grad("tree_attention", query, key_cache, value_cache)
+    if scale is not None:
+        scale = float(scale)
     signature = (query.shape, query.stride(), query.dtype, query.get_device(), key_cache.shape, key_cache.stride(), key_cache.dtype,
                  key_cache.get_device(), value_cache.shape, value_cache.stride(), value_cache.dtype, value_cache.get_device(), lengths.shape,
                  lengths.is_contiguous(), lengths.dtype, lengths.get_device(), _vector_signature(tree_mask), scale, _vector_signature(key_scales),
@@ -418,7 +424,7 @@ def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, sca
         raise ValueError(f"tree_mask must be bool of shape ({m}, {m}) or ({b}, {m}, {m}); got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
     given = (query, lengths, tree_mask)
     lengths = _lengths("lengths", lengths, b)
-    scale = 1 / math.sqrt(d) if scale is None else float(scale)
+    scale = 1 / math.sqrt(d) if scale is None else scale
     _check_devices(query.device, query=query, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
                    tree_mask=tree_mask, key_scales=key_scales, value_scales=value_scales)
     if query.numel() == 0 or n == 0:

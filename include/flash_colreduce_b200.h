@@ -382,7 +382,10 @@ int fcr_select_above(const void* scores, int32_t dtype, int32_t rows, int32_t n,
  * cache (optionally in 8 bits) and read back, and drafted tokens attend the
  * cache.  The reference has none of this; its README names the token pruning
  * that these feed.  All launches go to `stream`; nothing synchronises,
- * allocates or keeps a pointer, and every call may be captured into a graph.
+ * allocates device memory or keeps a pointer, and calls may be captured into a
+ * graph.  fcr_tree_attention waits on the device with the same bounds and
+ * reports expired waits in the same way as fcr_colreduce; like it, it makes the
+ * device's status mailbox with its first call, which belongs outside a capture.
  */
 
 /*

@@ -705,3 +705,32 @@ def test_the_rows_are_quantised_alike_wherever_they_lie():
             at += s
     for c in caches[1:]:
         assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(c, caches[0]))
+
+
+@pytest.mark.parametrize("fmt", ["16", FP8, I8])
+@pytest.mark.parametrize("m,g", [(1, 4), (6, 8), (12, 4), (30, 4), (64, 8)])
+def test_a_nan_among_the_cached_positions_reaches_every_row(fmt, m, g):
+    """Every row attends every cached position: a key or value that is NaN makes the rows of its head NaN, and no others."""
+    for which in (0, 1):
+        q, cache, x = _make(2, 2 * g, 2, m, 300, 64, fmt, BF, seed=3)
+        if fmt == "16":
+            cache[which][0, 1, 40, 5] = float("nan")
+        else:
+            cache[2 + which].view(torch.uint8)[0, 1, 40] = 255
+        got, lse = _run(q, cache, [200, 230])
+        clean = torch.ones(2, 2 * g, dtype=torch.bool)
+        clean[0, g:] = False
+        assert torch.isfinite(got[clean.to(DEV)].float()).all()
+        bad = got[0, g:]
+        assert (bad[..., 5].isnan().all() if which and fmt == "16" else bad.isnan().all())
+        assert lse[0, g:].isnan().all() == (which == 0)
+
+
+def test_options_given_as_tensors_are_read_anew():
+    q, cache, x = _make(1, 2, 1, 2, 200, 64, "16", HF)
+    scale = torch.tensor(0.1)
+    a, _ = _run(q, cache, [190], scale=scale)
+    scale.fill_(0.3)
+    b, _ = _run(q, cache, [190], scale=scale)
+    _check_attention(a, None, q, x[0], x[1], [190], None, 0.1)
+    _check_attention(b, None, q, x[0], x[1], [190], None, 0.3)
