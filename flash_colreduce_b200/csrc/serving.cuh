@@ -120,7 +120,7 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
   if (c.B <= 0 || c.H <= 0 || c.N <= 0 || c.D <= 0 || t.Hq <= 0 || t.M <= 0)
     return fail(FCR_ERR_BAD_ARG, "attention sizes must be positive");
   if (t.Hq % c.H) return fail(FCR_ERR_BAD_ARG, "query heads must be a multiple of the cache's heads");
-  if (t.M > 256) return fail(FCR_ERR_UNSUPPORTED, std::to_string(t.M) + " drafted tokens exceed 256");
+  if (t.M > kTreeMaxM) return fail(FCR_ERR_UNSUPPORTED, std::to_string(t.M) + " drafted tokens exceed " + std::to_string(kTreeMaxM));
   if (c.D > 128 || c.D % (c.format == FCR_KV_16BIT ? 8 : 16))
     return fail(FCR_ERR_UNSUPPORTED, "attention takes head dimensions up to 128, multiples of 8 for a 16-bit cache and of 16 for an 8-bit one");
   if (t.index_bits != 32 && t.index_bits != 64) return fail(FCR_ERR_BAD_ARG, "index_bits must be 32 or 64");
