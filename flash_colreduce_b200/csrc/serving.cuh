@@ -3,6 +3,8 @@
 // Included by colreduce_sm100.cu after the other entry points (needs fail, cuda_fail, launch_kernel, device_info).
 #pragma once
 
+#include <cfloat>
+
 namespace fcr {
 
 static bool kv_aligned(const void* ptr, const int64_t* strides, const int32_t* sizes, int dims, int elem_bytes, int bytes) {
@@ -125,6 +127,7 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
     return fail(FCR_ERR_UNSUPPORTED, "attention takes head dimensions up to 128, multiples of 8 for a 16-bit cache and of 16 for an 8-bit one");
   if (t.index_bits != 32 && t.index_bits != 64) return fail(FCR_ERR_BAD_ARG, "index_bits must be 32 or 64");
   if (t.q_strides[3] != 1) return fail(FCR_ERR_UNSUPPORTED, "innermost stride of the queries must be 1");
+  if (!(fabsf(t.scale) <= FLT_MAX)) return fail(FCR_ERR_BAD_ARG, "the scale must be finite");
   const int32_t sizes[3] = {c.B, c.H, c.N};
   const int elem = c.format == FCR_KV_16BIT ? 2 : 1;
   for (const int64_t* st : {c.k_strides, c.v_strides}) {

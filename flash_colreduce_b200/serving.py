@@ -369,7 +369,7 @@ def tree_attention(
             and strides are multiples of 16 bytes.
         lengths: (B,) int32 or int64, on the GPU: a captured graph may be replayed with other values.
         tree_mask: (M, M), (1, M, M) or (B, M, M) bool, or None.
-        scale: softmax scale, default ``1 / sqrt(D)``.
+        scale: softmax scale, finite, default ``1 / sqrt(D)``.
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
 
     Returns:
@@ -417,6 +417,8 @@ def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, sca
     b, h, n, d = key_cache.shape
     if query.dim() != 4 or query.shape[0] != b or query.shape[3] != d or h == 0 or query.shape[1] % h:
         raise ValueError(f"query must be ({b}, a multiple of {h}, M, {d}); got {tuple(query.shape)}.")
+    if d == 0:
+        raise ValueError("the head dimension must be positive.")
     hq, m = query.shape[1], query.shape[2]
     if m > 256:
         raise ValueError(f"{m} drafted tokens exceed 256.")
@@ -425,6 +427,8 @@ def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, sca
     given = (query, lengths, tree_mask)
     lengths = _lengths("lengths", lengths, b)
     scale = 1 / math.sqrt(d) if scale is None else scale
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError(f"scale must be a finite fp32 number; got {scale}.")
     _check_devices(query.device, query=query, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
                    tree_mask=tree_mask, key_scales=key_scales, value_scales=value_scales)
     if query.numel() == 0 or n == 0:

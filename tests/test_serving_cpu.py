@@ -266,3 +266,21 @@ def test_every_tile_belongs_to_one_cta_and_partial_results_have_no_gaps(sms, b, 
         groups.setdefault((seq, head, rt), set()).add(cta)
     for key, owners in groups.items():
         assert owners == set(range(min(owners), max(owners) + 1))
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e300])
+def test_attention_refuses_a_scale_that_is_not_a_finite_fp32_number(scale):
+    kc, vc, ks, vs = _cache()
+    with pytest.raises(ValueError, match="scale"):
+        fc.tree_attention(torch.zeros(2, 4, 5, 32, dtype=H16), kc, vc, torch.zeros(2, dtype=torch.int32), key_scales=ks, value_scales=vs,
+                          scale=scale)
+    p = nat.KvCache(2, 2, 16, 32, nat.FCR_KV_INT8, nat.FCR_F16, (1024, 512, 32, 1), (1024, 512, 32, 1), (32, 16, 1), (32, 16, 1))
+    t = nat.Tree(4, 5, (640, 160, 32, 1), 32, (0, 0), scale)
+    assert nat.lib.fcr_tree_workspace_bytes(C.byref(p), C.byref(t), 148) == 0
+    assert "scale" in nat.last_error()
+
+
+def test_attention_refuses_a_head_dimension_of_zero():
+    x = torch.zeros(1, 2, 3, 0, dtype=H16)
+    with pytest.raises(ValueError, match="head dimension"):
+        fc.tree_attention(x, x, x.clone(), torch.zeros(1, dtype=torch.int32))
