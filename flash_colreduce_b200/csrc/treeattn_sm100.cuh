@@ -72,8 +72,8 @@ enum {
 
 // A bounded wait as elsewhere, but with its loop out of line.  These kernels have up to seven kinds of warps, and the code
 // that is running must fit the instruction cache: with the loops inline and the converters unrolled 44 % of its
-// requests missed, warps waited for instructions more than for anything else, and a change of a few instructions anywhere
-// moved the time of 16 x 8 heads of 4096 int8 keys between 82 and 129 us; it is 59 now, with 10 % misses.
+// requests missed, warps waited for instructions nearly as much as for data (4.8 against 5.4 of them at each issue), and a
+// change of a few instructions anywhere moved the time of 16 x 8 heads of 4096 int8 keys between 82 and 129 us; it is 59 now, with 10 % misses.
 __device__ __noinline__ bool tree_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, const WaitParams* p, int code, int bounds) {
   const long long t0 = clock64();
   while (true) {

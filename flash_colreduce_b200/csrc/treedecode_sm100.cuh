@@ -15,8 +15,8 @@
 // What bounds it: with a 16-bit cache reading it (32 x 8 heads of 8191 bf16 keys, 4 rows: 170 us, 1.02 of the measured copy
 // rate's floor; 8 heads of 131072 fp16 keys: 93 us, 1.12 of it).  With an 8-bit cache the converters: 32768 codes per pair of
 // tiles at seven integer instructions per four, half rate, beside the waits; 32 x 8 heads of 8191 int8 keys take 163 us, the
-// floor is 84.  Up to 64 rows the rows-on-lanes form, with the rows held in 2 or 4 copies, was no faster: 188 us and 501 us for
-// the same two.
+// floor is 84.  Up to 64 rows the rows-on-lanes form, with the rows held in 2 or 4 copies, was slower: 188 us and 501 us for
+// the same two, where this form's first version (8-bit codes loaded by the converters, as there) took 171 and 365.
 //
 // Included by colreduce_sm100.cu after treeattn_sm100.cuh (TreeParams, the rings, the walk over the tiles).
 #pragma once
