@@ -859,6 +859,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         if (edge) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) bits[c] = tree_bits(p, words, m, t * kTreeTile + 32 * c, seg.have, seg.end);
+          __syncwarp();  // the lanes took different ways; tensor memory is read by a converged warp
         }
         auto load_scores = [&](int c, uint32_t (&x)[32]) {
           ptx::tmem_ld<32>(s_addr + 32 * c, x);
@@ -906,6 +907,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           m_ref = m_new;
           l *= alpha;
           if (mine > 0) {
+            __syncwarp();
             uint32_t o[32];
             for (int c = 0; c < DPAD / 32; ++c) {
               ptx::tmem_ld<32>(o_addr + 32 * c, o);
@@ -970,6 +972,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
         const int in_part = w * 128 + lane_row;
         for (int c = 0; c < DPAD / 32; ++c) {
+          __syncwarp();  // rows beyond the last one leave the previous step early
           uint32_t ra[32];
           ptx::tmem_ld<32>(o_addr + 32 * c, ra);
           ptx::tmem_ld_wait<32>(ra);
@@ -1025,6 +1028,7 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             p.lse[out_row0 + row] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * 0.69314718055994531f;
         }
         for (int c = 0; ok && 32 * c < p.D; ++c) {
+          __syncwarp();  // only some lanes had statistics to write
           uint32_t ra[32];
           if (mine > 0) {
             ptx::tmem_ld<32>(o_addr + 32 * c, ra);

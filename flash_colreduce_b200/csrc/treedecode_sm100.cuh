@@ -320,6 +320,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         ptx::tc_fence_after_sync();
         const bool edge = (t + 1) * kTreeTile > seg.have;
         const uint32_t bits = edge ? decode_row_bits(p, seg, t * kTreeTile + key, r0, W) : 0xffffffffu;
+        if (edge) __syncwarp();  // the lanes took different ways; tensor memory is read by a converged warp
         auto load_scores = [&](uint32_t (&x)[W]) {
           tmem_row_ld<W>(s_addr, x);
           int masked = edge;
@@ -444,6 +445,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         else if (p.lse)
           p.lse[out_row0 + my_row] = sum == 0.f ? -INFINITY : (m_ref + log2f(sum)) * 0.69314718055994531f;
       }
+      __syncwarp();  // only some lanes had statistics to write
       uint32_t o[W];
       tmem_row_ld<W>(o_addr, o);
       if (*bad_flag && key < p.D) {

@@ -1,0 +1,49 @@
+"""The attention of drafted tokens where its kernels' warps, types and lengths meet an edge (needs a B200).
+
+Tolerances are those of test_gpu_serving.py; what a test adds to them is derived beside it.
+"""
+import math
+
+import pytest
+import torch
+
+import flash_colreduce_b200 as fc
+from oracle.serving_oracle import attention
+from test_gpu_serving import BF, DEV, FP8, HF, I8, _check_attention, _make, _run, _tree
+
+pytestmark = pytest.mark.gpu
+
+
+def _check_strictly(got, lse, q, k, v, lens, mask, scale=None):
+    """As ``_check_attention``, and infinite entries of the output and of the log-sum-exp are equal with their signs."""
+    _check_attention(got, lse, q, k, v, lens, mask, scale)
+    want, want_lse, _ = attention(q, k, v, lens, mask, scale)
+    for g, w in ((got.cpu().double(), want), (lse.cpu().double(), want_lse)):
+        assert torch.equal(g.isinf(), w.isinf()) and torch.equal(g[w.isinf()], w[w.isinf()])
+
+
+# --------------------------------------------------------------------------- warps of which only some lanes hold a row
+@pytest.mark.parametrize("fmt", ["16", FP8])
+@pytest.mark.parametrize("have", [60, 2900])  # one CTA has all of a head's keys; several share them
+@pytest.mark.parametrize("hq,h,m,d", [
+    (10, 2, 7, 128), (8, 2, 5, 64), (6, 2, 13, 128), (3, 1, 27, 80), (3, 1, 41, 64), (7, 1, 26, 128), (10, 2, 67, 64),
+])
+def test_warps_that_hold_fewer_rows_than_lanes(fmt, have, hq, h, m, d):
+    """35, 20, 39, 81, 123, 182 and 335 rows per key head: lanes without a row leave the epilogue early, the others write
+    statistics and put non-finite drafted values back."""
+    q, cache, x = _make(1, hq, h, m, have + m + 3, d, fmt, HF, seed=m)
+    mask = _tree(1, m, seed=m)
+    mask[0, : m // 2, 2:5] = False
+    mask[0, m // 2 :, 2] = True
+    mask[0, m - 1, 4] = True
+    for head, token, col, value in ((0, 2, 3, math.nan), (0, 2, 7, -math.inf), (0, 2, 12, math.inf), (h - 1, 4, 7, math.inf)):
+        if fmt == "16":
+            cache[1][0, head, have + token, col] = value
+            x[1][0, head, have + token, col] = value
+    if fmt == FP8:
+        cache[3].view(torch.uint8)[0, 0, have + 2] = 255
+        x[1][0, 0, have + 2] = math.nan
+    got, lse = _run(q, cache, [have], mask)
+    _check_strictly(got, lse, q, x[0], x[1], [have], mask)
+    again, lse2 = _run(q, cache, [have], mask)
+    assert torch.equal(got.nan_to_num(7.0), again.nan_to_num(7.0)) and torch.equal(lse, lse2)
