@@ -286,6 +286,7 @@ keystream_kernel(const __grid_constant__ CUtensorMap tmap_q,
                 dst[q4] = make_float4(__uint_as_float(ra[4 * q4]), __uint_as_float(ra[4 * q4 + 1]),
                                       __uint_as_float(ra[4 * q4 + 2]), __uint_as_float(ra[4 * q4 + 3]));
             }
+            if (p.dump != nullptr) __syncwarp();  // the next load of tensor memory is a converged warp's
             if (need_mask)
               rows_chunk<true, kChunkRows>(ra, p.scale2, lim_hi - kChunkRows * c, m_run, l_run);
             else

@@ -47,3 +47,13 @@ def test_warps_that_hold_fewer_rows_than_lanes(fmt, have, hq, h, m, d):
     _check_strictly(got, lse, q, x[0], x[1], [have], mask)
     again, lse2 = _run(q, cache, [have], mask)
     assert torch.equal(got.nan_to_num(7.0), again.nan_to_num(7.0)) and torch.equal(lse, lse2)
+
+@pytest.mark.parametrize("m", [1, 5, 16])
+def test_column_reduction_with_a_score_cache_and_lanes_without_a_query(m):
+    """Few queries and long keys: the key-streaming rows pass keeps its scores; lanes beyond the last query keep none."""
+    g = torch.Generator().manual_seed(m)
+    q, k = torch.randn(2, 3, m, 128, generator=g).to(BF), torch.randn(2, 3, 5000, 128, generator=g).to(BF)
+    got = fc.flash_colreduce(q.to(DEV), k.to(DEV), "sum")
+    want = torch.softmax(q.double() @ k.double().transpose(-1, -2) / math.sqrt(128), -1).sum(2)
+    # the operator's bar: 2e-3 relative and 1e-5, and one rounding to bf16
+    assert ((got.cpu().double() - want).abs() <= 1e-5 + (2e-3 + 2.0 ** -8) * want.abs()).all()
