@@ -14,7 +14,9 @@
 //   O += P V     tcgen05, A = P from tensor memory, B = V as it lies in the cache (rows are the K dimension)
 //
 // with m a reference that follows the running maximum only when that has grown by more than 2^8: O is then rescaled in
-// tensor memory, otherwise the loop carries no correction.  Two warpgroups take turns, so that the exponentials of one
+// tensor memory, otherwise the loop carries no correction.  For fp16 the reference is kept 7 below the maximum it follows, so that
+// a row's largest weight lies in 2^7 .. 2^15: fp16 keeps 11 bits down to 2^-14 only and nothing below 2^-25, and many small
+// weights add up.  What is lost of a row is at most 2^-32 of its sum per key.  Two warpgroups take turns, so that the exponentials of one
 // tile run under the products of the other.  With more than 128 rows (PAIR) they are two row tiles over the same keys;
 // with 65 to 128, two runs of keys (every other tile) whose results are merged.  Up to 64 rows treedecode_sm100.cuh takes.
 //
@@ -172,6 +174,10 @@ __device__ __noinline__ uint32_t tree_bits(const TreeParams& p, const uint32_t* 
   if (n0 + 32 > end) bits &= (1u << (end - n0)) - 1u;
   return bits;
 }
+
+// log2 of the weight that a row's largest score gets when the reference moves.
+template <typename T>
+__host__ __device__ constexpr float tree_aim() { return std::is_same<T, __half>::value ? 7.f : 0.f; }
 
 template <typename T>
 __device__ __forceinline__ bool non_finite16(uint32_t h) {
@@ -898,11 +904,12 @@ tree_attention_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             pk[e / 2 + 1] = pack2(b.x, b.y, T());
           }
         };
-        // The reference moves when the maximum has grown by more than 2^8: P stays below that, far from any type's limits.
+        // The reference moves when the maximum has grown by more than 2^8: P stays within 2^15.
+        constexpr float kAim = tree_aim<T>();
         auto follow = [&](float top) {
-          const bool grow = real && top > m_ref + 8.f;
+          const bool grow = real && top > m_ref + (8.f + kAim);
           if (!__any_sync(0xffffffffu, grow)) return;
-          const float m_new = grow ? top : m_ref;
+          const float m_new = grow ? top - kAim : m_ref;
           const float alpha = m_new == m_ref ? 1.f : ptx::ex2(m_ref - m_new);
           m_ref = m_new;
           l *= alpha;

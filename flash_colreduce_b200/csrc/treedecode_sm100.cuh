@@ -8,7 +8,7 @@
 // A product then costs NR / 128 of what the rows-on-lanes form pays whatever the rows are, each thread has NR scores per tile
 // to take the exponential of instead of 128, and four softmax warps keep up with the memory.  A maximum would need the
 // threads to exchange values for every tile; instead they share a reference m per row and only agree (one barrier of
-// four warps) whether any score has passed it by more than 2^8.  That happens in a segment's first tile and rarely after; then the
+// four warps) whether any score has passed it by more than 2^8 (for fp16, whose reference lies 7 below the maximum, 2^15).  That happens in a segment's first tile and rarely after; then the
 // rows' maxima are formed, O^T and the sums are rescaled and the reference moves.  Sums stay in registers, a
 // thread's keys apart from the others', and are added up when a segment ends.
 //
@@ -332,7 +332,8 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
         };
         uint32_t x[W];
         load_scores(x);
-        // exponents against the reference as it is: has one passed 8?
+        // exponents against the reference as it is: has one passed 8 above the aim?
+        constexpr float kAim = tree_aim<T>();
         float w[W];
         float most = -INFINITY;
 #pragma unroll
@@ -343,7 +344,7 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           most = ptx::max3(ptx::max3(most, a.x, a.y), b.x, b.y);
           w[e] = a.x, w[e + 1] = a.y, w[e + 2] = b.x, w[e + 3] = b.y;
         }
-        if (__any_sync(0xffffffffu, most > 8.f) && lane == 0) vote[buf] = (int)tile_seq;
+        if (__any_sync(0xffffffffu, most > 8.f + kAim) && lane == 0) vote[buf] = (int)tile_seq;
         if (!sync_group()) break;
         if (vote[buf] == (int)tile_seq) {
           // the rows' maxima over the tile's 128 keys; O^T, the sums and the reference follow where a row has grown
@@ -363,9 +364,10 @@ tree_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_cons
           if (lane < W) {
             top = fmaxf(fmaxf(top_s[lane], top_s[NR + lane]), fmaxf(top_s[2 * NR + lane], top_s[3 * NR + lane])) * p.scale2;
             const float nm = ref_s[lane];
-            if (top + nm > 8.f) {
-              alpha = nm == kNothingSeen ? 0.f : ptx::ex2(-nm - top);
-              ref_s[lane] = -top;
+            if (top + nm > 8.f + kAim) {
+              const float now = kAim - top;
+              alpha = nm == kNothingSeen ? 0.f : ptx::ex2(now - nm);
+              ref_s[lane] = now;
             }
           }
           __syncwarp();

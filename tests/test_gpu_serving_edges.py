@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import flash_colreduce_b200 as fc
-from oracle.serving_oracle import attention
+from oracle.serving_oracle import attention, dequantize_rows, quantize_rows
 from test_gpu_serving import BF, DEV, FP8, HF, I8, _check_attention, _make, _run, _tree
 
 pytestmark = pytest.mark.gpu
@@ -48,6 +48,7 @@ def test_warps_that_hold_fewer_rows_than_lanes(fmt, have, hq, h, m, d):
     again, lse2 = _run(q, cache, [have], mask)
     assert torch.equal(got.nan_to_num(7.0), again.nan_to_num(7.0)) and torch.equal(lse, lse2)
 
+
 @pytest.mark.parametrize("m", [1, 5, 16])
 def test_column_reduction_with_a_score_cache_and_lanes_without_a_query(m):
     """Few queries and long keys: the key-streaming rows pass keeps its scores; lanes beyond the last query keep none."""
@@ -57,3 +58,51 @@ def test_column_reduction_with_a_score_cache_and_lanes_without_a_query(m):
     want = torch.softmax(q.double() @ k.double().transpose(-1, -2) / math.sqrt(128), -1).sum(2)
     # the operator's bar: 2e-3 relative and 1e-5, and one rounding to bf16
     assert ((got.cpu().double() - want).abs() <= 1e-5 + (2e-3 + 2.0 ** -8) * want.abs()).all()
+
+
+# ------------------------------------------------------------------------------------- fp16 weights far below the largest
+@pytest.mark.parametrize("fmt", ["16", FP8, I8])
+@pytest.mark.parametrize("m,g", [(1, 4), (6, 4), (8, 8), (20, 4), (40, 4)])  # every form of the kernels
+@pytest.mark.parametrize("gap,first", [(14.0, True), (17.0, True), (17.5, False), (20.0, True)])
+def test_a_strong_key_and_many_weak_ones_in_fp16(fmt, m, g, gap, first):
+    """One key `gap` nats above 16384 others and with value 0: the output is what the others' weights, 2^-20 to 2^-30 of its
+    own, add up to.
+
+    A weight is rounded to fp16 once, by half a step: u of itself, or 2^-25 below 2^-14.  The row's largest weight in a CTA
+    is 2^7 at least, so that each key adds at most 2^-32 of the row's sum times its value to the usual bound.
+    """
+    heads, n, d = 148, 16384, 64  # a head per CTA
+    at = 0 if first else n - 1
+    gen = torch.Generator().manual_seed(m)
+    k, v = torch.zeros(n + m, d), torch.empty(n + m, d)
+    k[:, 1] = 0.5 * torch.rand(n + m, generator=gen)
+    k[at, :2] = torch.tensor([gap, 0.0])
+    v.copy_(0.5 + torch.rand(n + m, d, generator=gen))
+    v[at] = 0
+    q = torch.zeros(1, 1, m, d)
+    q[..., :2] = 1
+    q, x = q.to(HF), torch.stack([k, v]).to(HF)[:, None, None]
+    if fmt == "16":
+        one, values = [x[0], x[1], None, None], x.double()
+    else:
+        one, values = [None] * 4, []
+        for i in range(2):
+            codes, bits = quantize_rows(x[i], fmt)
+            one[i], one[2 + i] = codes.to(fmt), bits
+            values.append(dequantize_rows(codes, bits))
+    cache = []
+    for c in one:
+        if c is None:
+            cache.append(None)
+            continue
+        raw = c.view({2: torch.int16, 1: torch.uint8}[c.element_size()]).to(DEV)
+        cache.append(raw.expand(1, heads, *raw.shape[2:]).contiguous().view(c.dtype))
+    got, lse = _run(q.expand(1, heads * g, m, d), cache, [n], scale=1.0)
+    want, want_lse, weight = attention(q, values[0], values[1], [n], None, 1.0)
+    u = 2.0 ** -11
+    big = gap + 1.0
+    score = big * (d / 16 + 4) * 2.0 ** -22 + big * 2.0 ** -23 + 2.0 ** -21
+    bound = u * want.abs() + 2 * (u + score) * weight + n * 2.0 ** -32 * values[1].abs().max() + 2.0 ** -24
+    worst = ((got.cpu().double() - want).abs() / bound).max().item()
+    assert worst <= 1.0, worst
+    assert ((lse.cpu().double() - want_lse).abs() <= score + 2.0 ** -22 * want_lse.abs() + 2.0 ** -20).all()
