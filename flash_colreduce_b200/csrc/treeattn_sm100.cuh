@@ -54,10 +54,10 @@ template <bool QUANT>
 constexpr int tree_threads() { return 32 * (kTreeQWarp + tree_q_warps<QUANT>() + 1 + (QUANT ? kTreeConvertWarps : 0)); }
 
 enum {
-  ST_TR_WAIT_Q_EMPTY = 71,
-  ST_TR_WAIT_K_EMPTY = 72,
-  ST_TR_WAIT_V_EMPTY = 73,
-  ST_TR_WAIT_Q_FULL = 74,
+  ST_TR_WAIT_Q_EMPTY = 87,
+  ST_TR_WAIT_K_EMPTY = 88,
+  ST_TR_WAIT_V_EMPTY = 89,
+  ST_TR_WAIT_Q_FULL = 90,
   ST_TR_WAIT_K_FULL = 75,
   ST_TR_WAIT_V_FULL = 76,
   ST_TR_WAIT_P = 77,

@@ -2,14 +2,17 @@
 
 Tolerances are those of test_gpu_serving.py; what a test adds to them is derived beside it.
 """
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import flash_colreduce_b200 as fc
+from flash_colreduce_b200 import _native as nat
 from oracle.serving_oracle import attention, dequantize_rows, quantize_rows
 from test_gpu_serving import BF, DEV, FP8, HF, I8, _check_attention, _make, _run, _tree
+from test_serving_edges_cpu import status_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +109,25 @@ def test_a_strong_key_and_many_weak_ones_in_fp16(fmt, m, g, gap, first):
     worst = ((got.cpu().double() - want).abs() / bound).max().item()
     assert worst <= 1.0, worst
     assert ((lse.cpu().double() - want_lse).abs() <= score + 2.0 ** -22 * want_lse.abs() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("fmt,hq,m", [("16", 4, 1), (I8, 4, 16), ("16", 4, 24), (I8, 4, 64)])
+def test_an_expired_wait_has_a_code_of_the_attention_kernels(fmt, hq, m, monkeypatch):
+    """One tile's load is left out and waits last a millisecond: the code that reaches the host is of no other kernel."""
+    own = {code for name, code in status_codes() if name.startswith(("ST_TR_", "ST_TD_"))}
+    own -= {code for name, code in status_codes() if not name.startswith(("ST_TR_", "ST_TD_"))}
+    monkeypatch.setenv("FCR_DEBUG_SYNC", "0")
+    q, cache, x = _make(1, hq, 1, m, 2000, 128, fmt, BF, seed=m)
+    before, lse = _run(q, cache, [2000 - m])
+    torch.cuda.synchronize()
+    nat.check(nat.lib.fcr_self_test_hooks(2_000_000, 0), "fcr_self_test_hooks")
+    try:
+        _run(q, cache, [2000 - m])
+    finally:
+        nat.check(nat.lib.fcr_self_test_hooks(0, -1), "fcr_self_test_hooks")
+    torch.cuda.synchronize()
+    code = C.c_int32(-1)
+    assert nat.lib.fcr_poll_device_status(C.byref(code)) == nat.FCR_ERR_DEVICE_TIMEOUT
+    assert code.value in own, code.value
+    after, lse2 = _run(q, cache, [2000 - m])
+    assert torch.equal(before, after) and torch.equal(lse, lse2)
