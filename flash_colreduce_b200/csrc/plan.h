@@ -104,16 +104,17 @@ FCR_HD T hd_max(T a, T b) { return a > b ? a : b; }
 // whatever the sequences' lengths are: lengths live on the device, so every CTA finds its piece itself.
 constexpr int kTreeTile = 128;  // keys per tile
 
-// Cached positions in front of the drafted tokens, and 128-key tiles up to the last one of them.
-FCR_HD int tree_have(long long length, int N) { return (int)(length < 0 ? 0 : length > N ? N : length); }
-FCR_HD int tree_end(int have, int M, int N) { return N - have < M ? N : have + M; }
-FCR_HD int tree_tiles(int have, int M, int N) { return (tree_end(have, M, N) + kTreeTile - 1) / kTreeTile; }
+// Cached positions in front of the drafted tokens, and 128-key tiles up to the last one of them.  A sequence of negative length
+// has no positions, drafted ones neither (have = -1, end = 0); its one tile, all masked, is there for its rows to be written.
+FCR_HD int tree_have(long long length, int N) { return (int)(length < 0 ? -1 : length > N ? N : length); }
+FCR_HD int tree_end(int have, int M, int N) { return have < 0 ? 0 : N - have < M ? N : have + M; }
+FCR_HD int tree_tiles(int have, int M, int N) { return have < 0 ? 1 : (tree_end(have, M, N) + kTreeTile - 1) / kTreeTile; }
 
 // One CTA's walk over its piece: segments are runs of tiles of one group.
 struct TreeSegment {
   int b, group;          // sequence; key head * row tiles + row tile
   int lo, hi, tiles;     // tiles [lo, hi) of the group's `tiles`
-  int have, end;         // cached positions, end of the drafted tokens' positions
+  int have, end;         // cached positions (-1: no positions at all), end of the drafted tokens' positions
   FCR_HD bool whole() const { return lo == 0 && hi == tiles; }
   FCR_HD int slot() const { return lo == 0 ? 1 : 0; }  // which of its CTA's two partial results it leaves, when not whole
 };

@@ -358,8 +358,8 @@ def tree_attention(
     The drafted tokens' own keys and values lie in the cache at positions ``lengths[b] .. lengths[b] + M - 1``
     (:func:`kv_cache_append` with the same ``lengths`` puts them there).  Every token attends the ``lengths[b]``
     positions before them and, among the drafted tokens, those its row of ``tree_mask`` names; without a mask they
-    are a chain (token ``m`` attends drafted tokens ``j <= m``).  Positions beyond the capacity do not exist.  A row that
-    attends nothing returns 0 (and a log-sum-exp of -inf).  What masked and unwritten positions hold does not
+    are a chain (token ``m`` attends drafted tokens ``j <= m``).  Positions beyond the capacity do not exist, and a sequence
+    of negative length has none, drafted ones neither.  A row that attends nothing returns 0 (and a log-sum-exp of -inf).  What masked and unwritten positions hold does not
     matter, NaN and infinities included.
 
     Args:

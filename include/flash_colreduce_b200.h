@@ -467,7 +467,8 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
  * and, of the drafted tokens, which lie at lengths[b] .. lengths[b]+M-1
  * (fcr_kv_append puts them there), those j with mask[b,m,j] != 0; a null mask
  * is a chain (j <= m), which with M = 1 is plain decoding.  Positions >= N do
- * not exist; a negative length counts as 0.
+ * not exist, and a sequence of negative length has none (fcr_kv_append leaves
+ * its tokens out, too).
  * out: contiguous (B,Hq,M,D) of the cache's dtype; lse (may be null): fp32
  * (B,Hq,M), natural logarithm of the sum of exponentials.  A row that attends
  * nothing has out 0 and lse -inf.  What masked and unwritten positions hold

@@ -67,7 +67,9 @@ def attention(q, k, v, lengths, mask=None, scale=None):
     wgt = torch.zeros_like(out)
     lse = torch.full((b, hq, m), -math.inf, dtype=torch.float64)
     for i in range(b):
-        have = min(max(int(lengths[i]), 0), n)
+        if int(lengths[i]) < 0:  # no positions, drafted ones neither
+            continue
+        have = min(int(lengths[i]), n)
         drafted = min(m, n - have)
         tree = torch.ones(m, m).tril().bool() if mask is None else (mask if mask.dim() == 2 else mask[i])
         for r in range(m):

@@ -11,7 +11,7 @@ import torch
 import flash_colreduce_b200 as fc
 from flash_colreduce_b200 import _native as nat
 from oracle.serving_oracle import attention, dequantize_rows, quantize_rows
-from test_gpu_serving import BF, DEV, FP8, HF, I8, _check_attention, _make, _run, _tree
+from test_gpu_serving import BF, DEV, FP8, HF, I8, _bits, _check_attention, _make, _run, _tree
 from test_serving_edges_cpu import status_codes
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +131,32 @@ def test_an_expired_wait_has_a_code_of_the_attention_kernels(fmt, hq, m, monkeyp
     assert code.value in own, code.value
     after, lse2 = _run(q, cache, [2000 - m])
     assert torch.equal(before, after) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("fmt", ["16", FP8, I8])
+@pytest.mark.parametrize("m,g,d", [(1, 4, 128), (6, 4, 64), (8, 8, 128), (20, 4, 64), (150, 4, 128)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_sequence_of_negative_length_has_no_positions(fmt, m, g, d, masked):
+    """The append leaves its tokens out, and the attention attends nothing: not what lies at the first positions either."""
+    n = 700
+    q, cache, x = _make(4, g, 1, m, n, d, fmt, BF, seed=m)
+    for i in range(2):
+        if fmt == "16":
+            cache[i][1, :, :] = math.nan
+        else:
+            cache[2 + i].view(torch.uint8)[1] = 255
+    before = [None if c is None else _bits(c).clone() for c in cache]
+    lens = [500, -1, 3, -(2 ** 31)]
+    new = torch.ones(4, 1, m, d, dtype=BF, device=DEV)
+    fc.kv_cache_append(new, new, cache[0], cache[1], torch.tensor(lens, device=DEV), cache[2], cache[3])
+    for c, old in zip(cache, before):
+        assert c is None or (torch.equal(_bits(c)[1::2], old[1::2]) and not torch.equal(_bits(c)[::2], old[::2]))
+    mask = _tree(4, m, seed=2) if masked else None
+    got, lse = _run(q, cache, lens, mask)
+    assert (got[1::2] == 0).all() and (lse[1::2] == -math.inf).all()
+    k, v = fc.kv_cache_read(*cache, dtype=BF)
+    pick = [0, 2]
+    _check_strictly(got[pick], lse[pick], q[pick], k.cpu().double()[pick], v.cpu().double()[pick], [lens[i] for i in pick],
+                    None if mask is None else mask[pick])
+    want, want_lse, _ = attention(q, k.cpu().double(), v.cpu().double(), lens, mask)
+    assert (want[1::2] == 0).all() and (want_lse[1::2] == -math.inf).all()

@@ -1,8 +1,14 @@
 """The serving operators without a GPU: what the host decides at their edges."""
+import ctypes as C
 import os
 import re
 
+import pytest
+import torch
+
 import flash_colreduce_b200 as fc
+from flash_colreduce_b200 import _native as nat
+from oracle.serving_oracle import attention
 
 CSRC = os.path.join(os.path.dirname(fc.__file__), "csrc")
 
@@ -24,3 +30,25 @@ def test_a_status_code_names_one_wait():
     for name, code in found:
         codes.setdefault(code, []).append(name)
     assert {c: n for c, n in codes.items() if len(n) > 1} == {}
+
+
+@pytest.mark.parametrize("m", [1, 200])
+def test_a_sequence_of_negative_length_takes_one_tile(m):
+    """It has no positions, but somebody has to write its zeros: one tile per group, whatever the drafted tokens are."""
+    b, h, n, lens = 3, 2, 1000, [-1, 300, -(2 ** 40)]
+    strides = (h * n * 128, n * 128, 128, 1)
+    cache = nat.KvCache(b, h, n, 128, nat.FCR_KV_16BIT, nat.FCR_BF16, strides, strides, (0, 0, 0), (0, 0, 0))
+    tree = nat.Tree(h, m, (h * m * 128, m * 128, 128, 1), 32, (0, 0), 0.1)
+    buf, tiles, i = (C.c_int32 * 10)(), {}, 0
+    while nat.lib.fcr_tree_segment(C.byref(cache), C.byref(tree), 1, (C.c_int64 * b)(*lens), 0, i, buf) == nat.FCR_OK:
+        tiles[buf[0], buf[1]] = buf[5]
+        i += 1
+    assert tiles == {(s, k): -(-(300 + m) // 128) if s == 1 else 1 for s in range(b) for k in range(h)}
+
+
+def test_the_oracle_knows_negative_lengths():
+    q = torch.zeros(2, 2, 3, 8)
+    k = torch.randn(2, 1, 10, 8, generator=torch.Generator().manual_seed(1))
+    out, lse, _ = attention(q, k, k, torch.tensor([-1, 0]))
+    assert (out[0] == 0).all() and (lse[0] == -float("inf")).all()
+    assert torch.allclose(out[1, :, 2], k[1, 0, :3].double().mean(0).expand(2, 8))
