@@ -20,6 +20,7 @@ from .op import _DTYPE_CODES, _debug_sync, _on_device
 
 __all__ = ["qk_norm_rope", "kv_cache_append", "kv_cache_read", "tree_attention"]
 
+_increment_version = torch.autograd.graph.increment_version
 _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
 _FORMATS = {torch.float16: nat.FCR_KV_16BIT, torch.bfloat16: nat.FCR_KV_16BIT, torch.float8_e4m3fn: nat.FCR_KV_FP8,
             torch.int8: nat.FCR_KV_INT8}
@@ -237,6 +238,8 @@ def kv_cache_append(
                                    lengths.data_ptr(), _address(counts), index_bits, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             nat.check(rc, "fcr_kv_append")
+    # autograd cannot see a write through a pointer: a cache that an operation saved for its backward pass must not change unnoticed
+    _increment_version([x for x in (key_cache, value_cache, key_scales, value_scales) if x is not None])
 
 
 def _plan_append(signature, key, value, key_cache, value_cache, lengths, key_scales, value_scales, counts):

@@ -11,7 +11,7 @@ import torch
 import flash_colreduce_b200 as fc
 from flash_colreduce_b200 import _native as nat
 from oracle.serving_oracle import attention, dequantize_rows, quantize_rows
-from test_gpu_serving import BF, DEV, FP8, HF, I8, _bits, _check_attention, _make, _run, _tree
+from test_gpu_serving import BF, DEV, FP8, HF, I8, _bits, _check_attention, _empty_cache, _make, _run, _tree
 from test_serving_edges_cpu import status_codes
 
 pytestmark = pytest.mark.gpu
@@ -160,3 +160,33 @@ def test_a_sequence_of_negative_length_has_no_positions(fmt, m, g, d, masked):
                     None if mask is None else mask[pick])
     want, want_lse, _ = attention(q, k.cpu().double(), v.cpu().double(), lens, mask)
     assert (want[1::2] == 0).all() and (want_lse[1::2] == -math.inf).all()
+
+
+# --------------------------------------------------------------------------------------------------------- autograd
+@pytest.mark.parametrize("fmt", [BF, FP8])
+def test_an_append_raises_the_versions_of_what_it_writes(fmt):
+    """A cache that an earlier operation saved for its backward pass cannot change unnoticed."""
+    cache = _empty_cache(2, 2, 20, 64, fmt)
+    new = torch.randn(2, 2, 3, 64, device=DEV).to(BF)
+    lens = torch.tensor([4, 5], device=DEV)
+    given = [new, lens, *[c for c in cache if c is not None]]
+    before = [x._version for x in given]
+    fc.kv_cache_append(new, new, cache[0], cache[1], lens, cache[2], cache[3])
+    assert [x._version > v for x, v in zip(given, before)] == [False, False] + [True] * (len(given) - 2)
+    before = [x._version for x in given]
+    fc.kv_cache_append(new[:, :, :0], new[:, :, :0], cache[0], cache[1], lens, cache[2], cache[3])  # nothing to write
+    fc.kv_cache_read(*cache, dtype=BF)
+    assert [x._version for x in given] == before
+    if fmt == BF:
+        weight = torch.ones(2, 2, 20, 64, dtype=BF, device=DEV, requires_grad=True)
+        cache[1].zero_()
+        for part in (cache[1], cache[1][:, :, 8:]):  # saved whole, and as a view
+            loss = (weight[:, :, -part.shape[2] :] * part).sum()
+            fc.kv_cache_append(new, new, cache[0], cache[1], lens)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+    with torch.inference_mode():  # whose tensors have no versions
+        mine = [None if c is None else c.clone() for c in cache]
+        fc.kv_cache_append(new, new, mine[0], mine[1], lens, mine[2], mine[3])
+        got = fc.kv_cache_read(*mine, dtype=BF)
+    assert torch.equal(got[0][0, :, 4:7], fc.kv_cache_read(*cache, dtype=BF)[0][0, :, 4:7])
