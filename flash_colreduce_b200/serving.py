@@ -5,7 +5,8 @@
 :func:`topk_columns` selected), and ``tree_attention`` lets drafted tokens -- or the one token of plain decoding --
 attend that cache.  The reference has no counterpart; its README.md:9 names the token pruning these belong to.
 
-All of it is forward only: inputs that require a gradient are refused while gradients are recorded.
+All of it is forward only: inputs that require a gradient are refused while gradients are recorded, and inputs that carry a
+tangent of forward-mode differentiation always.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .op import _DTYPE_CODES, _debug_sync, _on_device
@@ -37,9 +39,17 @@ def _check_devices(device: torch.device, **tensors) -> None:
             raise ValueError(f"All tensors must be on one device; got {name} on {x.device}, not {device}.")
 
 
+def _derivatives() -> bool:
+    """Whether gradients are recorded or tangents may be carried (no_grad does not end those)."""
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 def _check_no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+    given = [x for x in tensors if x is not None]
+    if torch.is_grad_enabled() and any(x.requires_grad for x in given):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad().")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in given):
+        raise RuntimeError(f"{what} has no forward-mode derivative: pass the primal (torch.autograd.forward_ad.unpack_dual).")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -92,7 +102,7 @@ def qk_norm_rope(
     Returns:
         ``(query, key)``, new contiguous tensors of the inputs' type.
     """
-    if torch.is_grad_enabled():
+    if _derivatives():
         _check_no_grad("qk_norm_rope", query, key, q_weight, k_weight, inv_freq)
     eps, interleaved = float(eps), bool(interleaved)  # (plain values: a signature must not hold a tensor)
     signature = (query.shape, query.stride(), query.dtype, query.get_device(), key.shape, key.stride(), key.dtype, key.get_device(), positions.shape,
@@ -219,7 +229,7 @@ def kv_cache_append(
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
         counts: (B,) of the type of ``lengths``, or None.
     """
-    if torch.is_grad_enabled():
+    if _derivatives():
         _check_no_grad("kv_cache_append", key, value, key_cache, value_cache)
     signature = (key.shape, key.stride(), key.dtype, key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(), key_cache.shape,
                  key_cache.stride(), key_cache.dtype, key_cache.get_device(), value_cache.shape, value_cache.stride(), value_cache.dtype,
@@ -292,7 +302,7 @@ def kv_cache_read(
     Returns:
         ``(key, value)``, contiguous (B, H, n, D): what :func:`flash_colreduce` takes as keys.
     """
-    if torch.is_grad_enabled():
+    if _derivatives():
         _check_no_grad("kv_cache_read", key_cache, value_cache)
     if n is not None:
         n = int(n)
@@ -379,7 +389,7 @@ def tree_attention(
         (B, Hq, M, D) of ``query``'s type, and with ``return_lse`` also the fp32 (B, Hq, M) natural log-sum-exp of
         every row's scaled scores.  Run-to-run results are bitwise identical.
     """
-    if torch.is_grad_enabled():
+    if _derivatives():
         _check_no_grad("tree_attention", query, key_cache, value_cache)
     if scale is not None:
         scale = float(scale)

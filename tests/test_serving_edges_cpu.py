@@ -5,6 +5,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flash_colreduce_b200 as fc
 from flash_colreduce_b200 import _native as nat
@@ -52,3 +53,39 @@ def test_the_oracle_knows_negative_lengths():
     out, lse, _ = attention(q, k, k, torch.tensor([-1, 0]))
     assert (out[0] == 0).all() and (lse[0] == -float("inf")).all()
     assert torch.allclose(out[1, :, 2], k[1, 0, :3].double().mean(0).expand(2, 8))
+
+
+def _dual(x):
+    return forward_ad.make_dual(x, torch.ones_like(x))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("call,name", [(fc.qk_norm_rope, n) for n in ("query", "key", "inv_freq", "q_weight", "k_weight")] +
+                         [(fc.kv_cache_append, n) for n in ("key", "value", "key_cache", "value_cache")] +
+                         [(fc.kv_cache_read, n) for n in ("key_cache", "value_cache")] +
+                         [(fc.tree_attention, n) for n in ("query", "key_cache", "value_cache")])
+def test_tangents_are_refused(call, name, grad):
+    """Forward-mode derivatives pass through no_grad; an input that carries one is refused like one that requires a gradient."""
+    x = torch.zeros(1, 2, 3, 16, dtype=torch.float16)
+    args = {fc.qk_norm_rope: dict(query=x, key=x, positions=torch.arange(3), inv_freq=torch.zeros(8), q_weight=x[0, 0, 0], k_weight=x[0, 0, 1]),
+            fc.kv_cache_append: dict(key=x, value=x, key_cache=x, value_cache=x, lengths=torch.zeros(1, dtype=torch.int32)),
+            fc.kv_cache_read: dict(key_cache=x, value_cache=x),
+            fc.tree_attention: dict(query=x, key_cache=x, value_cache=x, lengths=torch.zeros(1, dtype=torch.int32))}[call]
+    args = {n: t.clone() for n, t in args.items()}
+    with torch.set_grad_enabled(grad):
+        with forward_ad.dual_level():
+            dual = {**args, name: _dual(args[name])}
+            with pytest.raises(RuntimeError, match=f"{call.__name__} has no forward-mode derivative"):
+                call(**dual)
+            with pytest.raises(RuntimeError, match=f"{call.__name__} has no forward-mode derivative"):
+                call(**{**dual, name: dual[name][:]})  # a view carries its base's tangent
+            with pytest.raises(ValueError, match="CUDA device"):  # without tangents: the usual refusal of these CPU tensors
+                call(**{**dual, name: forward_ad.unpack_dual(dual[name]).primal})
+        with pytest.raises(ValueError, match="CUDA device"):
+            call(**dual)  # the level is gone, and the tangents with it
+
+
+def test_tangents_of_functional_transforms_are_refused():
+    x = torch.zeros(1, 2, 3, 16, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="kv_cache_read has no forward-mode derivative"):
+        torch.func.jvp(lambda k: fc.kv_cache_read(k, x)[0], (x,), (x,))
