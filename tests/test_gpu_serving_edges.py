@@ -190,3 +190,88 @@ def test_an_append_raises_the_versions_of_what_it_writes(fmt):
         fc.kv_cache_append(new, new, mine[0], mine[1], lens, mine[2], mine[3])
         got = fc.kv_cache_read(*mine, dtype=BF)
     assert torch.equal(got[0][0, :, 4:7], fc.kv_cache_read(*cache, dtype=BF)[0][0, :, 4:7])
+
+
+# ------------------------------------------------------------------------------------- codes and scales at every size
+@pytest.mark.parametrize("fmt", [FP8, I8])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 33])
+def test_rows_of_every_scale_are_read_in_either_type(fmt, dtype, d):
+    """All 256 scale bytes by all 256 codes, read in the type they were not written from too: one rounding of code * 2^e."""
+    codes = torch.arange(256).repeat(256, 1).to(torch.uint8)
+    codes = torch.cat([codes, codes[:, : -256 % d]], 1).view(256, -1, d).transpose(0, 1)[None].contiguous()  # (1, heads, 256 scales, d)
+    scales = torch.arange(256).to(torch.uint8).expand(codes.shape[:3]).contiguous()
+    data = codes.to(DEV).view(fmt)
+    got = fc.kv_cache_read(data, data, scales.to(DEV), scales.to(DEV), dtype=dtype)
+    want = dequantize_rows(codes.view(fmt), scales).to(dtype)
+    for g in got:
+        assert torch.equal(g.cpu().isnan(), want.isnan()) and torch.equal(g.cpu().nan_to_num(3.0, 7.0, -7.0), want.nan_to_num(3.0, 7.0, -7.0))
+
+
+def _scaled(b, hq, h, m, n, d, fmt, dtype, shifts, seed):
+    """Queries and a cache of 8 bits whose rows' exponents are moved by one of `shifts` (keys, values); the values as read."""
+    q, cache, _ = _make(b, hq, h, m, n, d, fmt, dtype, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    for i in range(2):
+        by = torch.tensor(shifts[i])[torch.randint(0, len(shifts[i]), (b, h, n), generator=g)]
+        by[:, :, 128:256] = 0  # a tile of ordinary scales
+        bits = cache[2 + i].view(torch.uint8)
+        bits.copy_((bits.cpu().int() + by).to(torch.uint8))
+    return q, cache
+
+
+@pytest.mark.parametrize("fmt", [FP8, I8])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,g,d", [(1, 4, 128), (6, 4, 80), (8, 8, 64), (20, 4, 128), (40, 4, 64)])
+def test_attention_over_finite_scales_of_any_size(fmt, dtype, m, g, d):
+    """Scales far outside 2^-24 .. 2^5, beside ordinary ones in the same tile and alone."""
+    for shifts in (((0, -40, -100), (0, 8, -26)) if dtype is HF else ((0, -40, -100), (0, 60, -60)), ((-30,), (-20,)), ((0,), (7,))):
+        q, cache = _scaled(2, 2 * g, 2, m, 600, d, fmt, dtype, shifts, seed=m)
+        lens = [600 - m, 300]
+        mask = _tree(2, m, seed=3)
+        got, lse = _run(q, cache, lens, mask)
+        k, v = (x.cpu().double() for x in fc.kv_cache_read(*cache, dtype=dtype))
+        assert torch.isfinite(v).all()
+        _check_strictly(got, lse, q, k, v, lens, mask)
+
+
+@pytest.mark.parametrize("fmt", [FP8, I8])
+@pytest.mark.parametrize("m,g,d", [(1, 4, 128), (6, 4, 80), (8, 8, 64), (20, 4, 128), (40, 4, 64)])
+def test_values_that_fp16_cannot_hold_are_infinite(fmt, m, g, d):
+    """Attention in fp16 over rows written from bf16: such a value is read as an infinity, by the rows that attend it."""
+    q, cache, _ = _make(2, 2 * g, 2, m, 600, d, fmt, HF, seed=m)
+    lens = [600 - m, 300]
+    one = torch.full((1, 1, 1, d), 1.0, dtype=BF, device=DEV)
+    one[..., 1::2] = -1
+    zero = torch.zeros_like(one)
+    for row, at, value in ((0, 40, one * 1e6 * (torch.arange(d, device=DEV) == 5)), (1, 300 + m // 2, one * 3e5)):
+        part = [c[row : row + 1, 1:] for c in cache]
+        fc.kv_cache_append(zero, value.to(BF), part[0], part[1], torch.tensor([at], device=DEV), part[2], part[3])
+    mask = _tree(2, m, seed=3)
+    got, lse = _run(q, cache, lens, mask)
+    k, v = (x.cpu().double() for x in fc.kv_cache_read(*cache, dtype=HF))
+    assert v[0, 1, 40, 5] == -math.inf and v[0, 1, 40].isinf().sum() == 1 and v[1, 1, 300 + m // 2].isinf().all()
+    _check_strictly(got, lse, q, k, v, lens, mask)
+    assert (got[0, g:, :, 5] == -math.inf).all()
+
+
+@pytest.mark.parametrize("fmt", ["16", FP8, I8])
+@pytest.mark.parametrize("m,g", [(1, 4), (6, 8), (12, 4), (30, 4), (64, 8)])
+def test_a_nan_among_the_cached_positions_leaves_the_rest_as_it_is(fmt, m, g):
+    """What it must not reach is compared with the oracle: other heads, other columns, and the log-sum-exp for a value."""
+    lens = [200, 230]
+    for which in (0, 1):
+        q, cache, x = _make(2, 2 * g, 2, m, 300, 64, fmt, BF, seed=3)
+        if fmt == "16":
+            cache[which][0, 1, 40, 5] = math.nan
+            x[which][0, 1, 40, 5] = math.nan
+        else:
+            cache[2 + which].view(torch.uint8)[0, 1, 40] = 255
+            x[which][0, 1, 40] = math.nan
+        got, lse = _run(q, cache, lens)
+        _check_strictly(got, lse, q, x[0], x[1], lens, None)
+        hit = torch.zeros(2, 2 * g, dtype=torch.bool, device=DEV)
+        hit[0, g:] = True
+        assert torch.isfinite(lse[~hit]).all() and torch.isfinite(got[~hit].float()).all()
+        assert torch.isfinite(lse[hit]).all() if which else lse[hit].isnan().all()
+        assert got[hit][..., 5].isnan().all() and got[hit][..., 6].isnan().all() == (fmt != "16" or which == 0)
