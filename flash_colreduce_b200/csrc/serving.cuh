@@ -7,6 +7,8 @@
 
 namespace fcr {
 
+constexpr float kLog2E = 1.4426950408889634f;
+
 static bool kv_aligned(const void* ptr, const int64_t* strides, const int32_t* sizes, int dims, int elem_bytes, int bytes) {
   if (reinterpret_cast<uintptr_t>(ptr) % bytes) return false;
   for (int i = 0; i < dims; ++i)
@@ -127,7 +129,7 @@ static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
     return fail(FCR_ERR_UNSUPPORTED, "attention takes head dimensions up to 128, multiples of 8 for a 16-bit cache and of 16 for an 8-bit one");
   if (t.index_bits != 32 && t.index_bits != 64) return fail(FCR_ERR_BAD_ARG, "index_bits must be 32 or 64");
   if (t.q_strides[3] != 1) return fail(FCR_ERR_UNSUPPORTED, "innermost stride of the queries must be 1");
-  if (!(fabsf(t.scale) <= FLT_MAX)) return fail(FCR_ERR_BAD_ARG, "the scale must be finite");
+  if (!(fabsf(t.scale) * kLog2E <= FLT_MAX)) return fail(FCR_ERR_BAD_ARG, "the scale must be finite in fp32, and times log2(e)");
   const int32_t sizes[3] = {c.B, c.H, c.N};
   const int elem = c.format == FCR_KV_16BIT ? 2 : 1;
   for (const int64_t* st : {c.k_strides, c.v_strides}) {
@@ -515,7 +517,7 @@ int fcr_tree_attention(const fcr_kv_cache* cache, const fcr_tree* tree, const vo
   p.words = pl.words;
   p.mask_shared = t.mask_strides[0] == 0;
   p.index_bits = t.index_bits;
-  float s2 = fabsf(t.scale) * 1.4426950408889634f;
+  float s2 = fabsf(t.scale) * kLog2E;
   if (!(s2 >= 1e-30f)) s2 = 1e-30f;  // scale 0: every score becomes (numerically) zero
   p.scale2 = s2;
   p.idesc_s = instr_desc(c.dtype, t.scale < 0.f);

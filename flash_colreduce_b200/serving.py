@@ -382,7 +382,7 @@ def tree_attention(
             and strides are multiples of 16 bytes.
         lengths: (B,) int32 or int64, on the GPU: a captured graph may be replayed with other values.
         tree_mask: (M, M), (1, M, M) or (B, M, M) bool, or None.
-        scale: softmax scale, finite, default ``1 / sqrt(D)``.
+        scale: softmax scale, finite (up to 2.3e38), default ``1 / sqrt(D)``.
         key_scales, value_scales: (B, H, N) float8_e8m0fnu or uint8, for 8-bit caches.
 
     Returns:
@@ -440,8 +440,8 @@ def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, sca
     given = (query, lengths, tree_mask)
     lengths = _lengths("lengths", lengths, b)
     scale = 1 / math.sqrt(d) if scale is None else scale
-    if not abs(scale) <= torch.finfo(torch.float32).max:
-        raise ValueError(f"scale must be a finite fp32 number; got {scale}.")
+    if not abs(scale) <= 2.3e38:  # scale * log2(e) must be a finite fp32 number
+        raise ValueError(f"scale must be a finite fp32 number of magnitude up to 2.3e38; got {scale}.")
     _check_devices(query.device, query=query, key_cache=key_cache, value_cache=value_cache, lengths=lengths,
                    tree_mask=tree_mask, key_scales=key_scales, value_scales=value_scales)
     if query.numel() == 0 or n == 0:

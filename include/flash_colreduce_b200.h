@@ -479,7 +479,7 @@ typedef struct fcr_tree {
   int64_t q_strides[4];
   int32_t index_bits;            /* of lengths: 32 or 64 */
   int64_t mask_strides[2];       /* bytes, (B,M); the innermost stride is 1; 0 for a mask that sequences share */
-  float scale;
+  float scale;                   /* finite, and scale * log2(e) too */
 } fcr_tree;
 
 /* Bytes of workspace (256-byte aligned, any contents) for a device with num_sms SMs (0: the current device); 0 on error. */

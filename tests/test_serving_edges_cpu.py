@@ -89,3 +89,16 @@ def test_tangents_of_functional_transforms_are_refused():
     x = torch.zeros(1, 2, 3, 16, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="kv_cache_read has no forward-mode derivative"):
         torch.func.jvp(lambda k: fc.kv_cache_read(k, x)[0], (x,), (x,))
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.4e38])
+def test_a_scale_that_overflows_in_base_2_is_refused(scale):
+    """The kernels multiply by scale * log2(e): an infinite factor would turn scores of 0 into NaN."""
+    x = torch.zeros(1, 2, 3, 16, dtype=torch.float16)
+    with pytest.raises(ValueError, match="scale"):
+        fc.tree_attention(x, x, x.clone(), torch.zeros(1, dtype=torch.int32), scale=scale)
+    cache = nat.KvCache(1, 2, 3, 16, nat.FCR_KV_16BIT, nat.FCR_F16, (96, 48, 16, 1), (96, 48, 16, 1), (0, 0, 0), (0, 0, 0))
+    for s, fine in ((scale, False), (2.3e38, True), (-2.3e38, True)):
+        tree = nat.Tree(2, 3, (96, 48, 16, 1), 32, (0, 0), s)
+        assert (nat.lib.fcr_tree_workspace_bytes(C.byref(cache), C.byref(tree), 148) > 0) == fine
+        assert fine or "scale" in nat.last_error()
