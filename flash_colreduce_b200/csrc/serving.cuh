@@ -9,6 +9,9 @@ namespace fcr {
 
 constexpr float kLog2E = 1.4426950408889634f;
 
+constexpr int32_t kMaxRows = 1 << 30;  // rows, positions and heads are counted in 32 bits, in steps of up to 1024
+static int too_many(const char* what) { return fail(FCR_ERR_UNSUPPORTED, std::string("more than ") + std::to_string(kMaxRows) + " " + what); }
+
 static bool kv_aligned(const void* ptr, const int64_t* strides, const int32_t* sizes, int dims, int elem_bytes, int bytes) {
   if (reinterpret_cast<uintptr_t>(ptr) % bytes) return false;
   for (int i = 0; i < dims; ++i)
@@ -53,6 +56,8 @@ static int check_cache(const fcr_kv_cache& c, const void* k, const void* v, cons
   if (!k || !v) return fail(FCR_ERR_BAD_ARG, "null cache");
   if (c.B <= 0 || c.H <= 0 || c.N <= 0 || c.D <= 0) return fail(FCR_ERR_BAD_ARG, "cache sizes must be positive");
   if (c.D > 256) return fail(FCR_ERR_UNSUPPORTED, "head dimension " + std::to_string(c.D) + " exceeds 256");
+  if (c.N > kMaxRows) return too_many("positions");
+  if ((long long)c.B * c.H > kMaxRows) return too_many("heads of sequences");
   if (c.dtype != FCR_F16 && c.dtype != FCR_BF16) return fail(FCR_ERR_UNSUPPORTED, "a cache holds fp16 or bf16 values");
   if (c.format != FCR_KV_16BIT && c.format != FCR_KV_FP8 && c.format != FCR_KV_INT8)
     return fail(FCR_ERR_BAD_ARG, "invalid cache format");
@@ -123,6 +128,9 @@ static cudaError_t launch_read_f(int format, const KvReadParams& p, bool vec, un
 static int check_tree(const fcr_kv_cache& c, const fcr_tree& t) {
   if (c.B <= 0 || c.H <= 0 || c.N <= 0 || c.D <= 0 || t.Hq <= 0 || t.M <= 0)
     return fail(FCR_ERR_BAD_ARG, "attention sizes must be positive");
+  if (c.N > kMaxRows) return too_many("positions");
+  if ((long long)c.B * c.H > kMaxRows) return too_many("heads of sequences");
+  if ((long long)(t.Hq / c.H) * t.M > kMaxRows) return too_many("query rows per cache head");
   if (t.Hq % c.H) return fail(FCR_ERR_BAD_ARG, "query heads must be a multiple of the cache's heads");
   if (t.M > kTreeMaxM) return fail(FCR_ERR_UNSUPPORTED, std::to_string(t.M) + " drafted tokens exceed " + std::to_string(kTreeMaxM));
   if (c.D > 128 || c.D % (c.format == FCR_KV_16BIT ? 8 : 16))
@@ -260,8 +268,10 @@ int fcr_qk_norm_rope(const fcr_rope* problem, const void* q, const void* k, cons
                      void* k_out, void* stream_v) {
   if (!problem) return fail(FCR_ERR_BAD_ARG, "null argument");
   const fcr_rope& r = *problem;
-  if (r.B <= 0 || r.M <= 0 || r.D <= 0 || r.Hq < 0 || r.Hk < 0 || r.Hq + r.Hk <= 0)
+  if (r.B <= 0 || r.M <= 0 || r.D <= 0 || r.Hq < 0 || r.Hk < 0 || (r.Hq == 0 && r.Hk == 0))
     return fail(FCR_ERR_BAD_ARG, "sizes must be positive");
+  if (r.M > kMaxRows) return too_many("tokens");
+  if ((long long)r.Hq + r.Hk > kMaxRows) return too_many("heads");
   if (r.D > 256) return fail(FCR_ERR_UNSUPPORTED, "head dimension " + std::to_string(r.D) + " exceeds 256");
   if (r.rotary < 0 || r.rotary > r.D || r.rotary % 2) return fail(FCR_ERR_BAD_ARG, "rotary must be even and lie in [0, D]");
   if ((r.Hq > 0 && (!q || !q_out)) || (r.Hk > 0 && (!k || !k_out)) || !positions || (r.rotary > 0 && !inv_freq))
@@ -325,6 +335,7 @@ int fcr_kv_append(const fcr_kv_cache* cache, void* k_cache, void* v_cache, void*
   int rc = check_cache(c, k_cache, v_cache, k_scales, v_scales);
   if (rc != FCR_OK) return rc;
   if (M <= 0) return fail(FCR_ERR_BAD_ARG, "sizes must be positive");
+  if (M > kMaxRows) return too_many("tokens");
   if (index_bits != 32 && index_bits != 64) return fail(FCR_ERR_BAD_ARG, "index_bits must be 32 or 64");
   if (key_strides[3] != 1 || value_strides[3] != 1) return fail(FCR_ERR_UNSUPPORTED, "innermost stride must be 1");
   KvAppendParams p;
@@ -371,6 +382,7 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
   int rc = check_cache(c, k_cache, v_cache, k_scales, v_scales);
   if (rc != FCR_OK) return rc;
   if (n <= 0) return fail(FCR_ERR_BAD_ARG, "sizes must be positive");
+  if (n > kMaxRows) return too_many("positions");
   if (positions && index_bits != 32 && index_bits != 64) return fail(FCR_ERR_BAD_ARG, "index_bits must be 32 or 64");
   KvReadParams p;
   memset(&p, 0, sizeof(p));

@@ -52,6 +52,15 @@ def _check_no_grad(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} has no forward-mode derivative: pass the primal (torch.autograd.forward_ad.unpack_dual).")
 
 
+_MAX_ROWS = 2 ** 30  # rows, positions and heads are counted in 32 bits
+
+
+def _check_sizes(**counts) -> None:
+    for name, count in counts.items():
+        if count > _MAX_ROWS:
+            raise ValueError(f"{count} {name.replace('_', ' ')} exceed {_MAX_ROWS}.")
+
+
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` with an innermost stride of 1 (a copy when it has another)."""
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 and x.is_contiguous() else x.contiguous()
@@ -137,6 +146,7 @@ def _plan_rope(signature, query, key, positions, inv_freq, q_weight, k_weight, e
         raise TypeError(f"qk_norm_rope takes fp16, bf16 or fp32 tensors of one dtype; got query {query.dtype}, key {key.dtype}.")
     b, hq, m, d = query.shape
     hk = key.shape[1]
+    _check_sizes(sequences=b, tokens=m, heads=hq + hk)
     if d > 256:
         raise ValueError(f"Head dimension {d} exceeds 256.")
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > d:
@@ -171,6 +181,7 @@ def _cache_problem(key_cache, value_cache, key_scales, value_scales, dtype) -> n
         raise TypeError(f"a cache holds fp16 or bf16 values; got {dtype}.")
     fmt = _FORMATS[key_cache.dtype]
     b, h, n, d = key_cache.shape
+    _check_sizes(positions=n, heads_of_sequences=b * h)
     if d > 256:
         raise ValueError(f"Head dimension {d} exceeds 256.")
     if fmt == nat.FCR_KV_16BIT:
@@ -260,6 +271,7 @@ def _plan_append(signature, key, value, key_cache, value_cache, lengths, key_sca
     b, h, n, d = key_cache.shape
     if key.dim() != 4 or key.shape != value.shape or key.shape[:2] != (b, h) or key.shape[3] != d:
         raise ValueError(f"key and value must be ({b}, {h}, M, {d}); got {tuple(key.shape)} and {tuple(value.shape)}.")
+    _check_sizes(tokens=key.shape[2])
     for name, x in (("key_cache", key_cache), ("value_cache", value_cache), ("key_scales", key_scales), ("value_scales", value_scales)):
         if x is not None and any(x.shape[i] > 1 and x.stride(i) == 0 for i in range(3)):
             raise ValueError(f"{name} is written: it cannot be an expanded tensor.")
@@ -342,6 +354,7 @@ def _plan_read(signature, key_cache, value_cache, key_scales, value_scales, posi
         if n is not None and n != positions.shape[2]:
             raise ValueError(f"n = {n} and positions of shape {tuple(positions.shape)} disagree.")
         n = positions.shape[2]
+        _check_sizes(positions=n)
         positions = positions.contiguous()
     else:
         n = cap if n is None else n
@@ -435,6 +448,7 @@ def _plan_tree(signature, query, key_cache, value_cache, lengths, tree_mask, sca
     hq, m = query.shape[1], query.shape[2]
     if m > 256:
         raise ValueError(f"{m} drafted tokens exceed 256.")
+    _check_sizes(query_rows_per_cache_head=hq // h * m)
     if tree_mask is not None and (tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((m, m), (1, m, m), (b, m, m))):
         raise ValueError(f"tree_mask must be bool of shape ({m}, {m}) or ({b}, {m}, {m}); got {tree_mask.dtype} {tuple(tree_mask.shape)}.")
     given = (query, lengths, tree_mask)

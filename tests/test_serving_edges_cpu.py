@@ -102,3 +102,49 @@ def test_a_scale_that_overflows_in_base_2_is_refused(scale):
         tree = nat.Tree(2, 3, (96, 48, 16, 1), 32, (0, 0), s)
         assert (nat.lib.fcr_tree_workspace_bytes(C.byref(cache), C.byref(tree), 148) > 0) == fine
         assert fine or "scale" in nat.last_error()
+
+
+BIG = 2 ** 30 + 1
+
+
+def _wide(*shape, dtype=torch.float16):
+    return torch.zeros((1,) * (len(shape) - 1) + (shape[-1] if len(shape) == 4 else 1,), dtype=dtype).expand(shape)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: fc.qk_norm_rope(_wide(1, 1, BIG, 2), _wide(1, 1, BIG, 2), _wide(BIG, dtype=torch.int32), torch.zeros(1)),
+    lambda: fc.qk_norm_rope(_wide(1, BIG, 1, 2), _wide(1, 1, 1, 2), torch.zeros(1, dtype=torch.int32), torch.zeros(1)),
+    lambda: fc.qk_norm_rope(_wide(1, BIG // 2 + 1, 1, 2), _wide(1, BIG // 2 + 1, 1, 2), torch.zeros(1, dtype=torch.int32), torch.zeros(1)),
+    lambda: fc.kv_cache_read(_wide(1, 1, 2 ** 32 + 5, 8), _wide(1, 1, 2 ** 32 + 5, 8)),
+    lambda: fc.kv_cache_read(_wide(2 ** 20, 2 ** 11, 1, 8), _wide(2 ** 20, 2 ** 11, 1, 8)),
+    lambda: fc.kv_cache_read(_wide(1, 1, 5, 8), _wide(1, 1, 5, 8), positions=_wide(1, 1, BIG, dtype=torch.int32)),
+    lambda: fc.kv_cache_append(_wide(1, 1, BIG, 8), _wide(1, 1, BIG, 8), torch.zeros(1, 1, 5, 8, dtype=torch.float16),
+                               torch.zeros(1, 1, 5, 8, dtype=torch.float16), torch.zeros(1, dtype=torch.int32)),
+    lambda: fc.tree_attention(_wide(1, 2 ** 23, 256, 8), _wide(1, 1, 5, 8), _wide(1, 1, 5, 8), torch.zeros(1, dtype=torch.int32)),
+    lambda: fc.tree_attention(_wide(1, 1, 1, 8), _wide(1, 1, BIG, 8), _wide(1, 1, BIG, 8), torch.zeros(1, dtype=torch.int32)),
+])
+def test_sizes_that_32_bits_do_not_hold_are_refused(call):
+    """The kernels count rows in 32 bits: a longer cache was cut to what those hold."""
+    with pytest.raises(ValueError, match=str(2 ** 30)):
+        call()
+
+
+def test_the_c_entries_refuse_sizes_that_32_bits_do_not_hold():
+    p, st = C.c_void_p(4096), nat.strides4((1, 1, 1, 1))  # never dereferenced: every refusal comes before any device work
+
+    def cache(b=1, h=1, n=5):
+        return C.byref(nat.KvCache(b, h, n, 8, nat.FCR_KV_16BIT, nat.FCR_F16, (40, 40, 8, 1), (40, 40, 8, 1), (0, 0, 0), (0, 0, 0)))
+
+    def tree(hq=1, m=1):
+        return C.byref(nat.Tree(hq, m, (8, 8, 8, 1), 32, (0, 0), 0.1))
+
+    for c, t in ((cache(n=BIG), tree()), (cache(b=2 ** 16, h=2 ** 15), tree(hq=2 ** 15)), (cache(), tree(hq=2 ** 23, m=256))):
+        assert nat.lib.fcr_tree_workspace_bytes(c, t, 148) == 0 and str(2 ** 30) in nat.last_error()
+        assert nat.lib.fcr_tree_attention(c, t, p, p, p, None, None, p, None, p, None, p, 1 << 40, None) == nat.FCR_ERR_UNSUPPORTED
+    assert nat.lib.fcr_kv_append(cache(n=BIG), p, p, None, None, p, st, p, st, 1, p, None, 32, None) == nat.FCR_ERR_UNSUPPORTED
+    assert nat.lib.fcr_kv_append(cache(), p, p, None, None, p, st, p, st, BIG, p, None, 32, None) == nat.FCR_ERR_UNSUPPORTED
+    assert nat.lib.fcr_kv_read(cache(n=BIG), p, p, None, None, None, 64, 1, p, p, None) == nat.FCR_ERR_UNSUPPORTED
+    assert nat.lib.fcr_kv_read(cache(), p, p, None, None, p, 64, BIG, p, p, None) == nat.FCR_ERR_UNSUPPORTED
+    for sizes in ((1, 1, 1, BIG), (1, BIG, 0, 1), (1, BIG // 2 + 1, BIG // 2 + 1, 1)):
+        r = nat.Rope(*sizes, 16, 16, (1, 1, 1, 1), (1, 1, 1, 1), nat.FCR_F16, nat.FCR_F16, 0, 32, (0, 1), 1e-6)
+        assert nat.lib.fcr_qk_norm_rope(C.byref(r), *[p] * 8, None) == nat.FCR_ERR_UNSUPPORTED, sizes
