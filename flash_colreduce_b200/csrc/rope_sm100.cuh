@@ -106,7 +106,7 @@ template <typename T, int LPR, bool INTERLEAVED>
 __global__ void __launch_bounds__(256)
 rope_vector_kernel(const RopeParams p) {
   constexpr int kHeads = 32 / LPR;            // heads at a time
-  constexpr int K = LPR >= 4 ? LPR / 4 : 1;   // angles per lane
+  constexpr int K = LPR / 4;                  // angles per lane
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.heads[0] + p.heads[1];
   const int chunks = (heads + p.heads_per_warp - 1) / p.heads_per_warp;
