@@ -105,16 +105,17 @@ FCR_HD T hd_max(T a, T b) { return a > b ? a : b; }
 constexpr int kTreeTile = 128;  // keys per tile
 
 // Cached positions in front of the drafted tokens, and 128-key tiles up to the last one of them.  A sequence of negative length
-// has no positions, drafted ones neither (have = -1, end = 0); its one tile, all masked, is there for its rows to be written.
-FCR_HD int tree_have(long long length, int N) { return (int)(length < 0 ? -1 : length > N ? N : length); }
-FCR_HD int tree_end(int have, int M, int N) { return have < 0 ? 0 : N - have < M ? N : have + M; }
-FCR_HD int tree_tiles(int have, int M, int N) { return have < 0 ? 1 : (tree_end(have, M, N) + kTreeTile - 1) / kTreeTile; }
+// has no positions, drafted ones neither (have = -M puts their end at 0: every role computes that end for every segment, and
+// a case of its own there cost registers); its one tile, all masked, is there for its rows to be written.
+FCR_HD int tree_have(long long length, int M, int N) { return (int)(length < 0 ? -M : length > N ? N : length); }
+FCR_HD int tree_end(int have, int M, int N) { return N - have < M ? N : have + M; }
+FCR_HD int tree_tiles(int have, int M, int N) { return (hd_max(tree_end(have, M, N), 1) + kTreeTile - 1) / kTreeTile; }
 
 // One CTA's walk over its piece: segments are runs of tiles of one group.
 struct TreeSegment {
   int b, group;          // sequence; key head * row tiles + row tile
   int lo, hi, tiles;     // tiles [lo, hi) of the group's `tiles`
-  int have, end;         // cached positions (-1: no positions at all), end of the drafted tokens' positions
+  int have, end;         // cached positions (-M: no positions at all), end of the drafted tokens' positions
   FCR_HD bool whole() const { return lo == 0 && hi == tiles; }
   FCR_HD int slot() const { return lo == 0 ? 1 : 0; }  // which of its CTA's two partial results it leaves, when not whole
 };
@@ -135,7 +136,7 @@ struct TreeWalk {
     t = (int)(offset - (long long)group * tiles);
   }
   FCR_HD void sequence() {
-    have = tree_have(lengths(b), N);
+    have = tree_have(lengths(b), M, N);
     tiles = tree_tiles(have, M, N);
   }
   FCR_HD bool next(TreeSegment& s) {

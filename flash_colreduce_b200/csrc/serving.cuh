@@ -433,14 +433,14 @@ int fcr_tree_segment(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t nu
   if (cta < 0 || cta >= pl.ctas || index < 0) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
   const int groups = c.H * pl.row_tiles;
   long long total = 0;
-  for (int b = 0; b < c.B; ++b) total += (long long)tree_tiles(tree_have(lengths[b], c.N), tree->M, c.N) * groups;
+  for (int b = 0; b < c.B; ++b) total += (long long)tree_tiles(tree_have(lengths[b], tree->M, c.N), tree->M, c.N) * groups;
   const int ctas = tree_ctas(total, pl.ctas);
   if (cta >= ctas) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
   const long long lo = tree_piece(total, ctas, cta), hi = tree_piece(total, ctas, cta + 1);
   long long before = 0;
   int first = 0;
   for (; first < c.B; ++first) {
-    const long long mine = (long long)tree_tiles(tree_have(lengths[first], c.N), tree->M, c.N) * groups;
+    const long long mine = (long long)tree_tiles(tree_have(lengths[first], tree->M, c.N), tree->M, c.N) * groups;
     if (lo < before + mine) break;
     before += mine;
   }
@@ -450,7 +450,7 @@ int fcr_tree_segment(const fcr_kv_cache* cache, const fcr_tree* tree, int32_t nu
   for (int i = 0; i <= index; ++i)
     if (!walk.next(s)) return fail(FCR_ERR_BAD_ARG, "no such CTA or segment");
   long long group_first = (long long)s.group * s.tiles;
-  for (int b = 0; b < s.b; ++b) group_first += (long long)tree_tiles(tree_have(lengths[b], c.N), tree->M, c.N) * groups;
+  for (int b = 0; b < s.b; ++b) group_first += (long long)tree_tiles(tree_have(lengths[b], tree->M, c.N), tree->M, c.N) * groups;
   const int v[10] = {s.b, s.group / pl.row_tiles, s.group % pl.row_tiles, s.lo, s.hi, s.tiles, s.whole() ? -1 : s.slot(),
                      tree_owner(total, ctas, group_first), tree_owner(total, ctas, group_first + s.tiles - 1), ctas};
   for (int i = 0; i < 10; ++i) out[i] = v[i];

@@ -600,7 +600,7 @@ __device__ __forceinline__ void tree_load_roles(const TreeParams& p, const TreeR
 // One warp: this CTA's piece of the line of tiles, as the sequence it begins in, the tile there and its length.
 __device__ __forceinline__ void tree_find_piece(const TreeParams& p, const TreeLengths& lengths, int lane, volatile int* start_b,
                                                 volatile long long* start_off, volatile long long* start_n) {
-  auto tiles_of = [&](int b) { return b < p.B ? tree_tiles(tree_have(lengths(b), p.N), p.M, p.N) : 0; };
+  auto tiles_of = [&](int b) { return b < p.B ? tree_tiles(tree_have(lengths(b), p.M, p.N), p.M, p.N) : 0; };
   const int mine0 = tiles_of(lane);
   long long total = mine0;
   for (int b = lane + 32; b < p.B; b += 32) total += tiles_of(b);
@@ -1110,7 +1110,7 @@ tree_combine_kernel(const __grid_constant__ TreeParams p, int ctas, int rows_per
   const TreeLengths lengths{p.lengths, p.index_bits};
   long long before = 0, total = 0;
   for (int i = threadIdx.x; i < p.B; i += 256) {
-    const int t = tree_tiles(tree_have(lengths(i), p.N), p.M, p.N);
+    const int t = tree_tiles(tree_have(lengths(i), p.M, p.N), p.M, p.N);
     total += t;
     if (i < b) before += t;
   }
@@ -1131,7 +1131,7 @@ tree_combine_kernel(const __grid_constant__ TreeParams p, int ctas, int rows_per
   }
   total *= p.groups;
   ctas = tree_ctas(total, ctas);
-  const int tiles = tree_tiles(tree_have(lengths(b), p.N), p.M, p.N);
+  const int tiles = tree_tiles(tree_have(lengths(b), p.M, p.N), p.M, p.N);
   const long long first = before * p.groups + (long long)group * tiles;
   const int c0 = tree_owner(total, ctas, first), c1 = tree_owner(total, ctas, first + tiles - 1);
   if (c0 == c1) return;  // one CTA took all of it and has written the result
