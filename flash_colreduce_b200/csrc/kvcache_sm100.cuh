@@ -118,9 +118,9 @@ __device__ __forceinline__ float kv_largest() {
 
 // Both kernels: a block takes kKvRows rows per lane group of one (K or V, sequence, head); `group` lanes per row, eight
 // consecutive values each.  A thread's rows are read together, so that four loads are under way.  2 x 8 heads of 32768 tokens,
-// D = 128, e4m3: 125 us to write (3.2 TB/s, short of the memory's rate by the quantiser's instructions, about 100 per eight
-// values) and 72 us to read (5.6 TB/s); two rows per thread take 234 us for both, eight 186, one with its place found by
-// 64-bit divisions 295.
+// D = 128, e4m3: 111 us to write (3.6 TB/s, short of the memory's rate by the quantiser's instructions, about 100 per eight
+// values) and 71 us to read (5.7 TB/s); int8 118 and 81; 16 bits 83 each (6.5 TB/s).  For both in e4m3, 181 us: two rows per
+// thread take 234, eight 186, one with its place found by 64-bit divisions 295.
 constexpr int kKvRows = 4;
 struct KvPlace {
   int kv, b, h, row0, step;  // first row of this thread, distance to its next

@@ -9,8 +9,9 @@
 // to sincospif.
 //
 // Bound by HBM: each row is read and written once and the arithmetic is about ten operations per element.  Two kernels: rows
-// that can be read 16 bytes at a time, and all others.  2 x 16384 tokens of 32 + 8 heads of 128 in bf16: 139 us (4.8 TB/s) with
-// the first, 638 us with the second; one token of one sequence 2.6 us.
+// that can be read 16 bytes at a time, and all others.  2 x 16384 tokens of 32 + 8 heads of 128 in bf16: 137 us (4.9 TB/s) with
+// the first, 638 us with the second; in fp32 211 us (6.4 TB/s); heads of 80 with 80 or 64 rotated dimensions 130 us, with 40 or 20
+// (half of them is no multiple of 8: the second kernel) 550 us; one token of one sequence 2.6 us.
 //
 // Included by colreduce_sm100.cu.
 #pragma once

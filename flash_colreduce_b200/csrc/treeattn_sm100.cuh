@@ -28,7 +28,7 @@
 // the swizzled tile that TMA writes for a 16-bit cache.  Multiplying codes as they are (kind::f8f6f4) would need the queries and
 // the weights in 8 bits.
 //
-// What bounds it: 64 tokens of 8 sequences over 8 heads of up to 16384 bf16 keys (256 rows per head) take 143 us against 54 of
+// What bounds it: 64 tokens of 8 sequences over 8 heads of up to 16384 bf16 keys (256 rows per head) take 145 us against 54 of
 // the tensor cores: a warpgroup's exponentials (3400 cycles per tile, in two passes over tensor memory) and its two products
 // follow one another, and the other warpgroup's products hide only part of that.
 //
@@ -75,7 +75,7 @@ enum {
 // A bounded wait as elsewhere, but with its loop out of line.  These kernels have up to seven kinds of warps, and the code
 // that is running must fit the instruction cache: with the loops inline and the converters unrolled 44 % of its
 // requests missed, warps waited for instructions nearly as much as for data (4.8 against 5.4 of them at each issue), and a
-// change of a few instructions anywhere moved the time of 16 x 8 heads of 4096 int8 keys between 82 and 129 us; it is 59 now, with 10 % misses.
+// change of a few instructions anywhere moved the time of 16 x 8 heads of 4096 int8 keys between 82 and 129 us; it is 58 now, with 9 % misses.
 __device__ __noinline__ bool tree_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, const WaitParams* p, int code, int bounds) {
   const long long t0 = clock64();
   while (true) {

@@ -12,11 +12,22 @@
 // rows' maxima are formed, O^T and the sums are rescaled and the reference moves.  Sums stay in registers, a
 // thread's keys apart from the others', and are added up when a segment ends.
 //
-// What bounds it: with a 16-bit cache reading it (32 x 8 heads of 8191 bf16 keys, 4 rows: 170 us, 1.02 of the measured copy
-// rate's floor; 8 heads of 131072 fp16 keys: 93 us, 1.12 of it).  With an 8-bit cache the converters: 32768 codes per pair of
-// tiles at seven integer instructions per four, half rate, beside the waits; 32 x 8 heads of 8191 int8 keys take 163 us, the
-// floor is 84.  Up to 64 rows the rows-on-lanes form, with the rows held in 2 or 4 copies, was slower: 188 us and 501 us for
-// the same two, where this form's first version (8-bit codes loaded by the converters, as there) took 171 and 365.
+// What bounds it: with a 16-bit cache reading it (32 x 8 heads of 8191 bf16 keys, 4 rows: 171 us, 1.03 of the measured copy
+// rate's floor; 8 heads of 131072 fp16 keys: 93 us, 1.12 of it).  With an 8-bit cache the latency of the converters: 32 x 8
+// heads of 8191 int8 keys take 162 us, the floor is 84.  That is 2900 cycles per pair of tiles, of which the converters' seven
+// integer instructions per four codes fill about 900; the rest are load, conversion and store of one step after the other, and
+// waits.  So an 8-bit cache saves memory, and time only for single tokens: 16 x 8 heads of 4096 keys take 52 us in bf16 and 54 in 8
+// bits with 4 rows, 64 and 70 with 32, 70 and 86 with 64.
+//
+// Up to 16 and 32 rows the rows-on-lanes form, with the rows held in 4 or 2 copies, was slower (188 and 501 us for 32 x 8 heads
+// of 8191 keys in bf16 and int8, where this form's first version took 171 and 365).  For 33 to 64 rows the two present forms,
+// keys on the lanes / rows on the lanes:
+//   D = 128   16 x 8 heads of 4096 keys: bf16 68..71 / 70..74 us, 8 bits 82..86 / 99..103;
+//             8 heads of 32768: bf16 55..57 / 52..54, 8 bits 59..62 / 65..67
+//   D = 64    16 x 8 heads of 4096 keys: bf16 59..62 / 58..60, 8 bits 71..74 / 68..70;
+//             8 heads of 32768: bf16 44..47 / 41..42, 8 bits 50..53 / 46..47
+// This form gains up to 17 % with long rows and an 8-bit cache and loses up to 12 % with short rows; one border, 64 rows, is
+// kept for all.
 //
 // Included by colreduce_sm100.cu after treeattn_sm100.cuh (TreeParams, the rings, the walk over the tiles).
 #pragma once

@@ -98,7 +98,8 @@ def qk_norm_rope(
 
     ``y = x * rsqrt(mean(x^2) + eps) * weight`` over the head dimension (without a weight ``y = x``), then the pairs
     ``(i, i + R/2)`` -- or ``(2 i, 2 i + 1)`` with ``interleaved`` -- of the first ``R = 2 * len(inv_freq)`` dimensions are
-    rotated by ``position * inv_freq[i]``.  Computed in fp32, the angle in fp64, and rounded once.
+    rotated by ``position * inv_freq[i]``.  Computed in fp32, the angle in fp64, and rounded once; a row whose sum of squares
+    passes fp32's range is normed to zeros.  No more than 2^30 tokens, heads or sequences.
 
     Args:
         query: (B, Hq, M, D) fp16, bf16 or fp32 CUDA tensor with D <= 256; any strides with innermost 1, e.g. a view of
@@ -230,7 +231,8 @@ def kv_cache_append(
     An 8-bit cache holds, per row (a token's head of K or V), codes and one power-of-two scale ``2^e``: ``e`` is the
     least exponent (at least -127) for which the row's largest magnitude is at most ``448 * 2^e`` (float8_e4m3fn) or
     ``127 * 2^e`` (int8), a code is ``x / 2^e`` rounded to nearest even.  Values that would read back as an infinity are
-    clamped to the largest that does not.  A row with a NaN or an infinity reads back as NaN.
+    clamped to the largest that does not.  A row with a NaN or an infinity reads back as NaN.  A cache has at most 2^30
+    positions, and as many heads of all sequences together.
 
     Args:
         key, value: (B, H, M, D) fp16 or bf16, D <= 256; any strides with innermost 1 (others are copied).
@@ -401,6 +403,11 @@ def tree_attention(
     Returns:
         (B, Hq, M, D) of ``query``'s type, and with ``return_lse`` also the fp32 (B, Hq, M) natural log-sum-exp of
         every row's scaled scores.  Run-to-run results are bitwise identical.
+
+    Scores, sums and accumulators are fp32.  Cached values are taken in ``query``'s type, and the softmax weights are rounded
+    to that type once before they multiply them: by half a step, 2^-8 of a weight in bf16, 2^-11 in fp16 (there at least 2^-32
+    of the row's sum per key).  An 8-bit cache takes about half the memory of a 16-bit one; for single tokens the attention is up to 7 %
+    faster over it, for drafted ones slower (by 8 % with 16 rows per cache head, up to 36 % with 128).
     """
     if _derivatives():
         _check_no_grad("tree_attention", query, key_cache, value_cache)

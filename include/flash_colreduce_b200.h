@@ -399,7 +399,7 @@ int fcr_select_above(const void* scores, int32_t dtype, int32_t rows, int32_t n,
  * (the angle in fp64) and rounded once.
  */
 typedef struct fcr_rope {
-  int32_t B, Hq, Hk, M, D;       /* D <= 256 */
+  int32_t B, Hq, Hk, M, D;       /* D <= 256; M and Hq + Hk at most 2^30 */
   int32_t rotary;                /* even, 0 <= rotary <= D */
   int64_t q_strides[4];          /* elements, (B,H,M,D) */
   int64_t k_strides[4];
@@ -429,7 +429,7 @@ int fcr_qk_norm_rope(const fcr_rope* problem, const void* q, const void* k, cons
 typedef enum fcr_kv_format { FCR_KV_16BIT = 0, FCR_KV_FP8 = 1, FCR_KV_INT8 = 2 } fcr_kv_format;
 
 typedef struct fcr_kv_cache {
-  int32_t B, H, N, D;            /* D <= 256 */
+  int32_t B, H, N, D;            /* D <= 256; N and B * H at most 2^30 */
   int32_t format;                /* fcr_kv_format */
   int32_t dtype;                 /* FCR_F16 or FCR_BF16: type of the values written and read */
   int64_t k_strides[4];          /* elements, (B,H,N,D) */
@@ -475,7 +475,7 @@ int fcr_kv_read(const fcr_kv_cache* cache, const void* k_cache, const void* v_ca
  * does not matter, NaN and infinities included.
  */
 typedef struct fcr_tree {
-  int32_t Hq, M;                 /* M <= 256 */
+  int32_t Hq, M;                 /* M <= 256, Hq / H * M at most 2^30 */
   int64_t q_strides[4];
   int32_t index_bits;            /* of lengths: 32 or 64 */
   int64_t mask_strides[2];       /* bytes, (B,M); the innermost stride is 1; 0 for a mask that sequences share */
